@@ -27,7 +27,8 @@
  * there is none or it is too small.  (A harness may opt in to a buffer the
  * library allocates and grows by itself: swc_hip_enable_auto_workspace.)
  * Layouts are the reference's: 4-D activations NHWC, conv filters
- * [oC, kH, kW, iC], matrices row-major.  All data is fp32.
+ * [oC, kH, kW, iC], matrices row-major.  All data is fp32, except where an
+ * entry point's name ends in _bf: those take bfloat16 (below).
  */
 #ifndef SWC_HIP_H_
 #define SWC_HIP_H_
@@ -46,6 +47,11 @@ enum {
     SWC_HIP_ERUNTIME = 3,    /* a HIP call failed; message holds hipGetErrorString */
     SWC_HIP_ENOTINIT = 4     /* swc_hip_init has not succeeded in this process */
 };
+
+/* A bfloat16: the upper 16 bits of an fp32 (1 sign, 8 exponent, 7 mantissa bits).
+ * The entry points whose names end in _bf take matrices of it; every sum inside
+ * them is held in fp32 and each result is rounded once, to nearest even. */
+typedef uint16_t swc_hip_bf16;
 
 /* ---- runtime: replaces the cudaSetDevice/cudaMalloc/cudaMemcpy/cudaFree and
  * stream set-up lines the reference prints (src/codegen/Codegen.cpp:154-172,
@@ -418,6 +424,150 @@ size_t swc_hip_conv2dFusedMaxpool_workspace_bytes(const size_t *cdims, const siz
                                                   const size_t *pool_kernels,
                                                   const size_t *pool_strides,
                                                   const size_t *pool_pads);
+
+/* ---- operators of language models.  No counterparts in the reference: each
+ * stands next to an op above whose work it does in the form that such models
+ * need.  Matrices are row-major with leading dimensions in elements (at most
+ * 4194240 for the _bf forms); outputs must not overlap inputs except where it
+ * is said.  Workspace: the size queries below, which answer for every alignment
+ * of the operands. ---- */
+
+/* the activations */
+enum {
+    SWC_HIP_ACT_NONE = 0,
+    SWC_HIP_ACT_RELU = 1,
+    SWC_HIP_ACT_GELU = 2,       /* z/2 (1 + erf(z / sqrt 2)) */
+    SWC_HIP_ACT_GELU_TANH = 3,  /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+    SWC_HIP_ACT_SILU = 4        /* z / (1 + e^-z) */
+};
+
+/* matrixMatrixFCBias with any of the activations and a second summand behind it:
+ *     Z[m,n] = A[m,k] * B[k,n] + bias[n]      C = act(Z) + residual[m,n]
+ * bias, residual and preact may be NULL.  preact receives Z (in the matrices'
+ * type), which the gradient call needs unless act is SWC_HIP_ACT_NONE.
+ * residual may be C itself.  k == 0 gives Z = bias. */
+int swc_hip_matrixMatrixFCActAdd_f(int m, int n, int k, const float *a, int lda,
+                                   const float *b, int ldb, const float *bias, int act,
+                                   const float *residual, int ldr, float *preact, int ldp,
+                                   float *c, int ldc);
+int swc_hip_matrixMatrixFCActAdd_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda,
+                                    const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *bias,
+                                    int act, const swc_hip_bf16 *residual, int ldr,
+                                    swc_hip_bf16 *preact, int ldp, swc_hip_bf16 *c, int ldc);
+size_t swc_hip_matrixMatrixFCActAdd_workspace_bytes(int m, int n, int k, int bf);
+
+/* Its gradients from cGrad, the gradient of C:
+ *     dZ = cGrad * act'(preact)      aGrad[m,k] = dZ * B^T
+ *     bGrad[k,n] = A^T * dZ          biasGrad[n] = column sums of dZ
+ * (the gradient of the residual is cGrad itself).  Any of aGrad, bGrad and
+ * biasGrad may be NULL and is then not computed; all are overwritten.  preact
+ * may be NULL when act is SWC_HIP_ACT_NONE.  The _bf form holds dZ in bfloat16
+ * for the two products and in fp32 for the column sums. */
+int swc_hip_matrixMatrixFCActAddGrad_f(int m, int n, int k, const float *cGrad, int ldcg,
+                                       const float *a, int lda, const float *b, int ldb,
+                                       const float *preact, int ldp, int act, float *aGrad,
+                                       int ldag, float *bGrad, int ldbg, float *biasGrad);
+int swc_hip_matrixMatrixFCActAddGrad_bf(int m, int n, int k, const swc_hip_bf16 *cGrad, int ldcg,
+                                        const swc_hip_bf16 *a, int lda, const swc_hip_bf16 *b,
+                                        int ldb, const swc_hip_bf16 *preact, int ldp, int act,
+                                        swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad,
+                                        int ldbg, swc_hip_bf16 *biasGrad);
+size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int bf);
+
+/* MatrixMatrixFCBias followed by MatrixSoftmaxWithLoss over a large vocabulary,
+ * without ever storing the m x n matrix of logits z = A*B + bias (bias may be
+ * NULL): the vocabulary is taken in pieces.
+ *     lse[r] = log(sum_j exp(z[r,j]))     rowLoss[r] = lse[r] - z[r, selected[r]]
+ *     *loss = mean of rowLoss over the rows that count
+ * A row whose selected[r] lies outside [0, n) is left out: its rowLoss and lse
+ * are 0, it does not count in the mean, and nothing in its row of A (infinities
+ * and NaN included) reaches any result.  With no row left *loss is 0.
+ * rowLoss, lse and loss are fp32 device memory and must all be given. */
+int swc_hip_matrixFCSoftmaxWithLoss_f(int m, int n, int k, const float *a, int lda,
+                                      const float *b, int ldb, const float *bias,
+                                      const int *selected, float *rowLoss, float *lse, float *loss);
+int swc_hip_matrixFCSoftmaxWithLoss_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda,
+                                       const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *bias,
+                                       const int *selected, float *rowLoss, float *lse,
+                                       float *loss);
+size_t swc_hip_matrixFCSoftmaxWithLoss_workspace_bytes(int m, int n, int k, int bf);
+
+/* Its gradients, with the lse of the forward call:
+ *     dz[r,j] = rowGrad[r] * (exp(z[r,j] - lse[r]) - (j == selected[r]))
+ *     aGrad = dz * B^T      bGrad = A^T * dz      biasGrad[n] = column sums of dz
+ * rowGrad[m] (fp32, device) is the gradient of each rowLoss; NULL means 1: the
+ * gradient of the SUM of the rows' losses, as matrixSoftmaxWithLossGrad_f gives
+ * it.  Rows left out have a zero row in aGrad and no part in the others.  The
+ * logits are computed again piece by piece.  Any of the three outputs may be
+ * NULL; all are overwritten.  The _bf form holds dz in bfloat16 for the products. */
+int swc_hip_matrixFCSoftmaxWithLossGrad_f(int m, int n, int k, const float *a, int lda,
+                                          const float *b, int ldb, const float *bias,
+                                          const int *selected, const float *lse,
+                                          const float *rowGrad, float *aGrad, int ldag,
+                                          float *bGrad, int ldbg, float *biasGrad);
+int swc_hip_matrixFCSoftmaxWithLossGrad_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda,
+                                           const swc_hip_bf16 *b, int ldb,
+                                           const swc_hip_bf16 *bias, const int *selected,
+                                           const float *lse, const float *rowGrad,
+                                           swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad,
+                                           int ldbg, swc_hip_bf16 *biasGrad);
+size_t swc_hip_matrixFCSoftmaxWithLossGrad_workspace_bytes(int m, int n, int k, int bf);
+
+/* The AdamW step, next to sgd_f, over `count` tensors at once.  `state` is a
+ * device buffer of SWC_HIP_ADAMW_STATE_BYTES, zero before the first step; its
+ * first 32-bit word counts the steps.  adamwAdvance begins a step t = count + 1:
+ * it counts it and leaves 1/(1 - beta1^t) and 1/(1 - beta2^t) for the updates
+ * that follow (one call for any number of them: groups of parameters with their
+ * own rates share a state).  The count is on the device, so a recorded graph
+ * goes on counting when it is replayed.
+ *     g = dw * gradFactor
+ *     mom = beta1 mom + (1 - beta1) g        var = beta2 var + (1 - beta2) g^2
+ *     w = w (1 - lr' decay) - lr' (mom / (1 - beta1^t)) / (sqrt(var / (1 - beta2^t)) + eps)
+ * with lr' = lr * lrFactor; lrFactor and gradFactor are device floats (a
+ * schedule's factor, a clipping coefficient) or NULL for 1.  w, dw, mom, var:
+ * HOST arrays of `count` device pointers, sizes: their element counts, all read
+ * before the call returns; a size of 0 skips its tensor.  w is fp32; dw is fp32
+ * in the _f forms and bfloat16 in the _bf forms; copies (NULL, or `count`
+ * pointers of which any may be NULL) receive w rounded to bfloat16.
+ * No two tensors of a call may overlap.  (The betas are doubles: 1 - beta of a
+ * float beta near 1 has lost a few digits.) */
+#define SWC_HIP_ADAMW_STATE_BYTES 32u
+int swc_hip_adamwAdvance(void *state, double beta1, double beta2);
+int swc_hip_adamw_f(int count, float *const *w, const float *const *dw, float *const *mom,
+                    float *const *var, swc_hip_bf16 *const *copies, const size_t *sizes,
+                    const void *state, float lr, double beta1, double beta2, float eps, float decay,
+                    const float *lrFactor, const float *gradFactor);
+int swc_hip_adamw_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, float *const *mom,
+                     float *const *var, swc_hip_bf16 *const *copies, const size_t *sizes,
+                     const void *state, float lr, double beta1, double beta2, float eps, float decay,
+                     const float *lrFactor, const float *gradFactor);
+/* The same with the states in 8 bits: in blocks of SWC_HIP_ADAMW_BLOCK
+ * consecutive elements of a tensor (the last one may be short), element i of
+ * block b is
+ *     mom = momScale[b] * e4m3(mom8[i])       sqrt(var) = varScale[b] * e4m3(var8[i])
+ * (e4m3: 8-bit floats of 4 exponent and 3 mantissa bits, bias 7, largest value
+ * 448, no infinities).  A step decodes both, updates as above in fp32 and encodes
+ * them again with scale = (largest finite magnitude of the block) / 448: mom to
+ * the nearest value, ties to even; sqrt(var) up or down at random with the
+ * probabilities that keep its expectation (a variance decays by less per step
+ * than half the distance of two values, and would never move if it were rounded
+ * to the nearest), but a positive one never to zero.  The random number of
+ * element i of tensor t in step s is 20 bits of a hash of (i + t * 0x9E3779B9 +
+ * s * 0x85EBCA6B): the same step gives the same bits.  A value that is not
+ * finite is held as NaN.  w is updated from the unrounded states.  momScale and
+ * varScale hold (size + SWC_HIP_ADAMW_BLOCK - 1) / SWC_HIP_ADAMW_BLOCK floats per tensor;
+ * all zero is the state before the first step. */
+#define SWC_HIP_ADAMW_BLOCK 256u
+int swc_hip_adamw8_f(int count, float *const *w, const float *const *dw, uint8_t *const *mom8,
+                     float *const *momScale, uint8_t *const *var8, float *const *varScale,
+                     swc_hip_bf16 *const *copies, const size_t *sizes, const void *state, float lr,
+                     double beta1, double beta2, float eps, float decay, const float *lrFactor,
+                     const float *gradFactor);
+int swc_hip_adamw8_bf(int count, float *const *w, const swc_hip_bf16 *const *dw,
+                      uint8_t *const *mom8, float *const *momScale, uint8_t *const *var8,
+                      float *const *varScale, swc_hip_bf16 *const *copies, const size_t *sizes,
+                      const void *state, float lr, double beta1, double beta2, float eps, float decay,
+                      const float *lrFactor, const float *gradFactor);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,330 @@
+// The AdamW step over many tensors at once, with its states in 32 bits or in 8 (adamw_f/_bf, adamw8_f/_bf), next to
+// sgd_f (train.hip).
+//
+// Bound by memory: per element w 8 bytes, the gradient 4 or 2, the states 16 or 4, the bfloat16 copy 2 — and some
+// twenty fp32 operations.  One launch covers up to kTensors tensors: their pointers travel by value in the kernel
+// arguments (nothing to upload, so a recorded graph needs no buffer of its own), and a workgroup finds its tensor by
+// bisecting the running count of chunks (an entry per tensor, in scalar registers).
+#include "common.hpp"
+
+using namespace swc_hip;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = SWC_HIP_ADAMW_BLOCK;   // elements that share a scale: one wavefront, four elements a lane
+
+struct Header {       // what adamwAdvance leaves for the updates
+    int steps;
+    int pad;
+    float c1, c2;     // 1 / (1 - beta^t)
+    int rest[4];
+};
+static_assert(sizeof(Header) == SWC_HIP_ADAMW_STATE_BYTES, "");
+
+struct Step {
+    const Header *state;
+    const float *lr_factor, *grad_factor;
+    float lr, beta1, beta2, rest1, rest2, eps, decay;   // rest: 1 - beta, from doubles
+};
+
+// 1 - beta^t in double: the difference cancels at the first steps of a beta near 1.
+__global__ void adamw_advance(Header *state, double beta1, double beta2) {
+    const int t = state->steps + 1;
+    state->steps = t;
+    state->c1 = (float)(1.0 / (1.0 - pow(beta1, (double)t)));
+    state->c2 = (float)(1.0 / (1.0 - pow(beta2, (double)t)));
+}
+
+struct Tensor {
+    float *w;
+    const void *dw;
+    void *mom, *var;
+    uint16_t *copy;
+    size_t size;
+};
+struct Tensor8 : Tensor {
+    float *mom_scale, *var_scale;
+};
+// 4 KiB of kernel arguments: 56 tensors with the 8-bit states' scales, 72 without
+template <class T, int N> struct Table {
+    T t[N];
+    unsigned first[N + 1];   // first chunk of each tensor
+    int count, number0;      // number0: the first tensor's number in the call
+};
+constexpr int kTensors = 64, kTensors8 = 48;
+static_assert(sizeof(Table<Tensor, kTensors>) + sizeof(Step) <= 4000 && sizeof(Table<Tensor8, kTensors8>) + sizeof(Step) <= 4000, "");
+
+template <class T, int N> __device__ __forceinline__ int tensor_of(const Table<T, N> &tab, unsigned chunk) {
+    int lo = 0, hi = tab.count;   // first[lo] <= chunk < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (tab.first[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float grad_of(const float *p, size_t i) { return p[i]; }
+__device__ __forceinline__ float grad_of(const uint16_t *p, size_t i) { return __builtin_bit_cast(float, (unsigned)p[i] << 16); }
+__device__ __forceinline__ uint16_t to_bf16(float x) {
+#if __HIP_DEVICE_COMPILE__
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+#else
+    return 0;
+#endif
+}
+
+struct Scalars {
+    float lr, shrink, g, c1, c2;
+};
+__device__ __forceinline__ Scalars scalars(const Step &s) {
+    Scalars r;
+    r.lr = s.lr_factor ? s.lr * *s.lr_factor : s.lr;
+    r.shrink = 1.f - r.lr * s.decay;
+    r.g = s.grad_factor ? *s.grad_factor : 1.f;
+    r.c1 = r.lr * s.state->c1;
+    r.c2 = s.state->c2;
+    return r;
+}
+__device__ __forceinline__ void step_one(float &w, float g, float &mom, float &var, const Scalars &k, const Step &s) {
+    g *= k.g;
+    mom = s.beta1 * mom + s.rest1 * g;
+    var = s.beta2 * var + s.rest2 * (g * g);
+    w = w * k.shrink - k.c1 * mom / (sqrtf(var * k.c2) + s.eps);
+}
+
+// A chunk is four elements a thread.
+constexpr unsigned kChunk = 4 * kThreads;
+
+template <class G>
+__global__ __launch_bounds__(kThreads) void adamw_tensors(Table<Tensor, kTensors> tab, Step s) {
+    const int which = tensor_of(tab, blockIdx.x);
+    const Tensor &t = tab.t[which];
+    const Scalars k = scalars(s);
+    const size_t i0 = (size_t)(blockIdx.x - tab.first[which]) * kChunk + threadIdx.x;
+    float *mom = static_cast<float *>(t.mom), *var = static_cast<float *>(t.var);
+    const G *dw = static_cast<const G *>(t.dw);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const size_t i = i0 + e * kThreads;
+        if (i >= t.size) return;
+        float w = t.w[i], m = mom[i], v = var[i];
+        step_one(w, grad_of(dw, i), m, v, k, s);
+        t.w[i] = w, mom[i] = m, var[i] = v;
+        if (t.copy) t.copy[i] = to_bf16(w);
+    }
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+__device__ __forceinline__ unsigned random20(unsigned x) {
+    x = (x ^ (x >> 16)) * 0x7FEB352Du;
+    x = (x ^ (x >> 15)) * 0x846CA68Bu;
+    return (x ^ (x >> 16)) >> 12;
+}
+
+constexpr float kLargest = 448.f;        // of e4m3
+constexpr float kTiny = 0x1p-100f;       // a block whose largest magnitude is below this is held as zeros
+constexpr unsigned kNan8 = 0x7f;
+
+__device__ __forceinline__ float from_e4m3(unsigned byte) {
+#if __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0);
+#else
+    return 0.f;
+#endif
+}
+// to the nearest value, ties to even; |y| <= 448
+__device__ __forceinline__ unsigned to_e4m3(float y) {
+#if __HIP_DEVICE_COMPILE__
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xffu;
+#else
+    return 0;
+#endif
+}
+// 0 <= y <= 448 up or down by 20 random bits: with the exponent E of y (at least that of the least normal value) the
+// values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is 8 (E + 7) + q - 8 — also
+// where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the subnormal values).
+__device__ __forceinline__ unsigned to_e4m3_random(float y, unsigned bits20) {
+    const int e = max((int)(__builtin_bit_cast(unsigned, y) >> 23) - 127, -6);
+    const float units = __builtin_bit_cast(float, (unsigned)(127 + 3 - e) << 23);   // 2^(3 - E)
+    float q = floorf(y * units + (float)bits20 * 0x1p-20f);
+    if (y > 0.f) q = fmaxf(q, 1.f);
+    return (unsigned)(8 * (e + 7) + (int)q - 8);
+}
+
+// A wavefront owns a block of 256 elements, lane l its elements l, l + 64, l + 128, l + 192.
+template <class G>
+__global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTensors8> tab, Step s) {
+    const int which = tensor_of(tab, blockIdx.x);
+    const Tensor8 &t = tab.t[which];
+    const Scalars k = scalars(s);
+    const size_t block = (size_t)(blockIdx.x - tab.first[which]) * 4 + (threadIdx.x >> 6);
+    const size_t i0 = block * kBlock + (threadIdx.x & 63);
+    if (block * kBlock >= t.size) return;   // whole wavefronts leave together
+    uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);
+    const G *dw = static_cast<const G *>(t.dw);
+    const float ms = t.mom_scale[block], vs = t.var_scale[block];
+    float m[4], r[4], top = 0.f, peak = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const size_t i = i0 + e * 64;
+        m[e] = 0.f, r[e] = 0.f;
+        if (i < t.size) {
+            float w = t.w[i];
+            m[e] = ms * from_e4m3(mom8[i]);
+            const float root = vs * from_e4m3(var8[i]);
+            float v = root * root;
+            step_one(w, grad_of(dw, i), m[e], v, k, s);
+            r[e] = sqrtf(v);
+            t.w[i] = w;
+            if (t.copy) t.copy[i] = to_bf16(w);
+            if (fabsf(m[e]) < __builtin_inff()) top = fmaxf(top, fabsf(m[e]));
+            if (r[e] < __builtin_inff()) peak = fmaxf(peak, r[e]);
+        }
+    }
+    top = wave_max(top), peak = wave_max(peak);
+    const bool has_m = top > kTiny, has_v = peak > kTiny;
+    const float im = has_m ? kLargest / top : 0.f, iv = has_v ? kLargest / peak : 0.f;
+    const unsigned number = (unsigned)(tab.number0 + which) * 0x9E3779B9u + (unsigned)s.state->steps * 0x85EBCA6Bu;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const size_t i = i0 + e * 64;
+        if (i < t.size) {
+            const float x = fminf(fmaxf(m[e] * im, -kLargest), kLargest), y = fminf(r[e] * iv, kLargest);
+            mom8[i] = (uint8_t)(fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8);
+            var8[i] = (uint8_t)(r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)i + number)) : kNan8);
+        }
+    }
+    if ((threadIdx.x & 63) == 0) {
+        t.mom_scale[block] = has_m ? top / kLargest : 0.f;
+        t.var_scale[block] = has_v ? peak / kLargest : 0.f;
+    }
+}
+
+int check(const char *who, int count, const void *const *w, const void *const *dw, const void *const *mom,
+          const void *const *var, const void *const *mom_scale, const void *const *var_scale, const size_t *sizes,
+          const void *state, bool eight, float lr, double beta1, double beta2, float eps, float decay) {
+    if (count < 0) return fail(SWC_HIP_EINVAL, "%s: count is negative", who);
+    if (!state) return fail(SWC_HIP_EINVAL, "%s: state is null", who);
+    if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1))
+        return fail(SWC_HIP_EINVAL, "%s: beta1 and beta2 must lie in [0, 1)", who);
+    if (!(eps >= 0.f) || !(lr == lr) || !(decay == decay)) return fail(SWC_HIP_EINVAL, "%s: eps is negative, or a rate is NaN", who);
+    if (count && (!w || !dw || !mom || !var || !sizes || (eight && (!mom_scale || !var_scale))))
+        return fail(SWC_HIP_EINVAL, "%s: null array of pointers", who);
+    for (int i = 0; i < count; ++i)
+        if (sizes[i] && (!w[i] || !dw[i] || !mom[i] || !var[i] || (eight && (!mom_scale[i] || !var_scale[i]))))
+            return fail(SWC_HIP_EINVAL, "%s: null pointer for tensor %d", who, i);
+    return SWC_HIP_OK;
+}
+
+// Fills tables of up to N tensors and launches one kernel for each.
+template <class T, int N, class Fill, class Launch>
+int launch_tables(const char *who, int count, const size_t *sizes, Fill fill, Launch launch) {
+    Table<T, N> tab;
+    int next = 0;
+    while (next < count) {
+        unsigned chunks = 0;
+        tab.count = 0;
+        tab.number0 = next;
+        for (; next < count && tab.count < N; ++next) {
+            const size_t need = (sizes[next] + kChunk - 1) / kChunk;
+            if (need > 0x7fffffffu) return fail(SWC_HIP_EUNSUPPORTED, "%s: tensor %d has %zu elements", who, next, sizes[next]);
+            if (chunks + need > 0x7fffffffu) break;
+            fill(tab.t[tab.count], next);
+            tab.first[tab.count++] = chunks;
+            chunks += (unsigned)need;
+        }
+        tab.first[tab.count] = chunks;
+        if (!chunks) continue;
+        launch(tab, chunks);
+        SWC_LAUNCH_CHECK();
+    }
+    return SWC_HIP_OK;
+}
+
+template <class G>
+int adamw(const char *who, int count, float *const *w, const G *const *dw, float *const *mom, float *const *var,
+          uint16_t *const *copies, const size_t *sizes, const void *state, float lr, double beta1, double beta2, float eps,
+          float decay, const float *lr_factor, const float *grad_factor) {
+    if (int rc = check(who, count, (const void *const *)w, (const void *const *)dw, (const void *const *)mom,
+                       (const void *const *)var, nullptr, nullptr, sizes, state, false, lr, beta1, beta2, eps, decay))
+        return rc;
+    if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
+    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1), (float)(1. - beta2), eps, decay};
+    return launch_tables<Tensor, kTensors>(
+        who, count, sizes,
+        [&](Tensor &t, int i) { t = Tensor{w[i], dw[i], mom[i], var[i], copies ? copies[i] : nullptr, sizes[i]}; },
+        [&](const Table<Tensor, kTensors> &tab, unsigned chunks) {
+            adamw_tensors<G><<<chunks, kThreads, 0, stream()>>>(tab, s);
+        });
+}
+
+template <class G>
+int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint8_t *const *mom8, float *const *mom_scale,
+           uint8_t *const *var8, float *const *var_scale, uint16_t *const *copies, const size_t *sizes, const void *state,
+           float lr, double beta1, double beta2, float eps, float decay, const float *lr_factor, const float *grad_factor) {
+    if (int rc = check(who, count, (const void *const *)w, (const void *const *)dw, (const void *const *)mom8,
+                       (const void *const *)var8, (const void *const *)mom_scale, (const void *const *)var_scale, sizes,
+                       state, true, lr, beta1, beta2, eps, decay))
+        return rc;
+    if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
+    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1), (float)(1. - beta2), eps, decay};
+    return launch_tables<Tensor8, kTensors8>(
+        who, count, sizes,
+        [&](Tensor8 &t, int i) {
+            t.w = w[i], t.dw = dw[i], t.mom = mom8[i], t.var = var8[i], t.copy = copies ? copies[i] : nullptr;
+            t.size = sizes[i], t.mom_scale = mom_scale[i], t.var_scale = var_scale[i];
+        },
+        [&](const Table<Tensor8, kTensors8> &tab, unsigned chunks) {
+            adamw8_tensors<G><<<chunks, kThreads, 0, stream()>>>(tab, s);
+        });
+}
+
+} // namespace
+
+extern "C" {
+
+int swc_hip_adamwAdvance(void *state, double beta1, double beta2) {
+    SWC_ARG(state);
+    SWC_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1);
+    SWC_REQUIRE_INIT();
+    adamw_advance<<<1, 1, 0, stream()>>>(static_cast<Header *>(state), beta1, beta2);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+int swc_hip_adamw_f(int count, float *const *w, const float *const *dw, float *const *mom, float *const *var,
+                    swc_hip_bf16 *const *copies, const size_t *sizes, const void *state, float lr, double beta1, double beta2,
+                    float eps, float decay, const float *lrFactor, const float *gradFactor) {
+    return adamw("swc_hip_adamw_f", count, w, dw, mom, var, copies, sizes, state, lr, beta1, beta2, eps, decay, lrFactor, gradFactor);
+}
+
+int swc_hip_adamw_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, float *const *mom, float *const *var,
+                     swc_hip_bf16 *const *copies, const size_t *sizes, const void *state, float lr, double beta1, double beta2,
+                     float eps, float decay, const float *lrFactor, const float *gradFactor) {
+    return adamw("swc_hip_adamw_bf", count, w, dw, mom, var, copies, sizes, state, lr, beta1, beta2, eps, decay, lrFactor, gradFactor);
+}
+
+int swc_hip_adamw8_f(int count, float *const *w, const float *const *dw, uint8_t *const *mom8, float *const *momScale,
+                     uint8_t *const *var8, float *const *varScale, swc_hip_bf16 *const *copies, const size_t *sizes,
+                     const void *state, float lr, double beta1, double beta2, float eps, float decay, const float *lrFactor,
+                     const float *gradFactor) {
+    return adamw8("swc_hip_adamw8_f", count, w, dw, mom8, momScale, var8, varScale, copies, sizes, state, lr, beta1, beta2,
+                  eps, decay, lrFactor, gradFactor);
+}
+
+int swc_hip_adamw8_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, uint8_t *const *mom8,
+                      float *const *momScale, uint8_t *const *var8, float *const *varScale, swc_hip_bf16 *const *copies,
+                      const size_t *sizes, const void *state, float lr, double beta1, double beta2, float eps, float decay,
+                      const float *lrFactor, const float *gradFactor) {
+    return adamw8("swc_hip_adamw8_bf", count, w, dw, mom8, momScale, var8, varScale, copies, sizes, state, lr, beta1, beta2,
+                  eps, decay, lrFactor, gradFactor);
+}
+
+} // extern "C"

@@ -1,0 +1,452 @@
+// The fully connected layer with its activation and a second summand (matrixMatrixFCActAdd_f/_bf) and its gradients,
+// next to matrixMatrixFCBias_f (gemm.hip).
+//
+//     Z = A B + bias, C = act(Z) + residual;    dZ = dC act'(Z), dA = dZ B^T, dB = A^T dZ, dbias = column sums of dZ
+//
+// bf16: three products on the core of gemm_bf16.hpp with no matrix transposed in memory.  fp32: the kernels of
+// gemm.hip (row-major operands; the gradients' operands are transposed into the workspace first), the activation in a
+// pass of its own — 12 bytes per element against 2 k flops at the fp32 matrix rate, 4 % at k = 4096.
+#include "act.hpp"
+#include "product_bf16.hpp"
+
+using namespace swc_hip;
+using namespace swc_hip::mfma16;
+
+namespace {
+
+struct FcEpilogue {
+    const uint16_t *bias, *residual;
+    uint16_t *preact, *c;
+    long ldr, ldp, ldc;
+    int act;
+    bool vec_r, vec_p, vec_c;
+#if __HIP_DEVICE_COMPILE__
+    template <int TM, int TN>
+    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
+                                               int) const {
+        const int l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) {
+            const int cb = col0 + tn * 32;
+            float b[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int col = cb + 8 * (v / 4) + 4 * h + v % 4;
+                b[v] = bias && col < n ? bf16_to_float(bias[col]) : 0.f;
+            }
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                const int row = row0 + tm * 32 + l32;
+                const bool ok = row < m;
+                float z[16], r[16];
+                if (residual) load_block(residual + row * ldr, ok, cb, n, vec_r, h, r);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) z[v] = acc[tm][tn][v] + b[v];
+                if (preact) store_block(preact + row * ldp, ok, cb, n, vec_p, h, z);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) z[v] = act_value(z[v], act) + (residual ? r[v] : 0.f);
+                store_block(c + row * ldc, ok, cb, n, vec_c, h, z);
+            }
+        }
+    }
+#endif
+};
+
+// The end of a layer from fp32 sums: `parts` matrices of m x n to be added in order, then bias, activation, residual.
+// z == nullptr: parts are the sums; otherwise (fp32) one matrix that already holds Z.
+template <class T>
+__global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long ldpart, long part_stride, const T *bias, int act,
+                                                 const T *residual, long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
+#if __HIP_DEVICE_COMPILE__
+    const size_t total = (size_t)m * n, step = (size_t)gridDim.x * 256;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+        const long r = i / n, j = i - r * n;
+        float z = 0.f;
+        for (int p = 0; p < parts; ++p) z += part[p * part_stride + r * ldpart + j];
+        if (bias) z += load_any(bias + j);
+        if (preact) store_any(preact + r * ldp + j, z);
+        z = act_value(z, act);
+        if (residual) z += load_any(residual + r * ldr + j);
+        store_any(c + r * ldc + j, z);
+    }
+#endif
+}
+
+// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.
+constexpr int kSumRows = 64;
+template <class T>
+__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int act, int m,
+                                                int n, float *sums) {
+#if __HIP_DEVICE_COMPILE__
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    const int r0 = blockIdx.y * kSumRows;
+    const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
+    if (j >= ld && j >= n) return;
+    float sum = 0.f;
+    for (int r = r0; r < r1; ++r) {
+        float g = 0.f;
+        if (j < n) {
+            g = load_any(dc + r * ldc + j);
+            if (act != SWC_HIP_ACT_NONE) g *= act_slope(load_any(z + r * ldz + j), act);
+            sum += g;
+        }
+        if (dz && j < ld) store_any(dz + r * ld + j, g);
+    }
+    if (sums && j < n) sums[(size_t)blockIdx.y * n + j] = sum;
+#endif
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index,
+                                                 const int *count) {
+    const int have = count ? *count : rows;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const bool ok = r < have;
+        const T *p = ok ? src + (index ? index[r] : r) * lds : src;
+        for (long j = (long)blockIdx.x * 256 + threadIdx.x; j < ld; j += (long)gridDim.x * 256)
+            dst[r * ld + j] = ok && j < cols ? p[j] : T(0);
+    }
+}
+template <class T>
+int launch_copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index, const int *count) {
+    if (!rows || !ld) return SWC_HIP_OK;
+    const unsigned x = ceil_div(ld, 256), y = rows < 32768 ? rows : 32768;
+    copy_rows<T><<<dim3(x > 64 ? 64 : x, y), 256, 0, stream()>>>(dst, ld, src, lds, rows, cols, index, count);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+__global__ __launch_bounds__(256) void add_parts(uint16_t *out_bf, float *out_f, const float *part, int parts, int n) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= n) return;
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) s += part[(size_t)p * n + j];
+    if (out_bf) store_any(out_bf + j, s);
+    if (out_f) out_f[j] = s;
+}
+
+bool known_act(int act) { return act >= SWC_HIP_ACT_NONE && act <= SWC_HIP_ACT_SILU; }
+
+template <class T>
+int check_forward(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb, int act, const T *residual,
+                  int ldr, const T *preact, int ldp, const T *c, int ldc) {
+    if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
+    if (!known_act(act)) return fail(SWC_HIP_EINVAL, "%s: unknown activation %d", who, act);
+    if (m == 0 || n == 0) return SWC_HIP_OK;
+    if (!c || (k && (!a || !b))) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
+    if ((k && (lda < k || ldb < n)) || ldc < n || (residual && ldr < n) || (preact && ldp < n))
+        return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
+    if ((const void *)c == a || (const void *)c == b || (preact && (preact == a || preact == b || preact == c || preact == residual)))
+        return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
+    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd))
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
+    return SWC_HIP_OK;
+}
+
+struct ForwardSpace {
+    uint16_t *a, *b;
+    float *part;
+    size_t bytes;
+};
+ForwardSpace forward_space(char *base, const Plan &p, int m, int n, int k, bool pack_a, bool pack_b) {
+    Carver c{base};
+    ForwardSpace s{};
+    s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
+    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
+    s.part = p.splits > 1 ? c.take<float>((size_t)p.splits * m * n) : nullptr;
+    s.bytes = c.used;
+    return s;
+}
+
+int forward_bf16(const char *who, int m, int n, int k, const uint16_t *a, long lda, const uint16_t *b, long ldb,
+                 const uint16_t *bias, int act, const uint16_t *residual, long ldr, uint16_t *preact, long ldp, uint16_t *c,
+                 long ldc) {
+    const Plan p = plan_product(m, n, k);
+    const bool pack_a = !aligned_rows(a, lda) || k % 8, pack_b = !aligned_rows(b, ldb);
+    const size_t need = forward_space(nullptr, p, m, n, k, pack_a, pack_b).bytes;
+    ForwardSpace w{};
+    if (need) {
+        char *base = static_cast<char *>(workspace(need, who));
+        if (!base) return fail_code();
+        w = forward_space(base, p, m, n, k, pack_a, pack_b);
+    }
+    if (pack_a) {
+        if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, nullptr, nullptr)) return rc;
+        a = w.a, lda = round8(k);
+    }
+    if (pack_b) {
+        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = round8(n);
+    }
+    const Shape s{a, b, lda, ldb, m, n, k, 0, nullptr};
+    if (p.splits == 1) {
+        const FcEpilogue ep{bias, residual, preact, c, ldr, ldp, ldc, act, aligned_rows(residual, ldr), aligned_rows(preact, ldp),
+                            aligned_rows(c, ldc)};
+        return run_product<kAlongK, kAcross>(p, s, ep, who);
+    }
+    if (int rc = run_product<kAlongK, kAcross>(p, s, StorePartial{w.part, (long)m * n, n, false}, who)) return rc;
+    fc_finish<uint16_t><<<grid_of((size_t)m * n), 256, 0, stream()>>>(w.part, p.splits, n, (long)m * n, bias, act, residual, ldr,
+                                                                      preact, ldp, c, ldc, m, n);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+template <class T>
+int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda, const T *b, int ldb,
+               const T *preact, int ldp, int act, const T *da, int ldda, const T *db, int lddb, const T *dbias) {
+    if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
+    if (!known_act(act)) return fail(SWC_HIP_EINVAL, "%s: unknown activation %d", who, act);
+    if (m && n && !dc) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
+    if (act != SWC_HIP_ACT_NONE && m && n && !preact) return fail(SWC_HIP_EINVAL, "%s: preact is needed for this activation", who);
+    if ((da && m && n && k && !b) || (db && m && n && k && !a)) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
+    if (lddc < n || (da && (ldda < k || ldb < n)) || (db && (lddb < n || lda < k)) || (act != SWC_HIP_ACT_NONE && ldp < n))
+        return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
+    const void *in[4] = {dc, a, b, preact};
+    for (const void *p : in)
+        if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
+    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd || lddc > kMaxLd))
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
+    return SWC_HIP_OK;
+}
+
+int sum_blocks(int m) { return (m + kSumRows - 1) / kSumRows; }
+
+template <class T>
+int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
+    const dim3 grid(ceil_div(dz && ld > n ? ld : n, 256), sum_blocks(m));
+    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
+    act_grad<T><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, act, m, n, sums);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+struct GradSpace {
+    uint16_t *dz, *a, *b;
+    float *part, *sums;
+    size_t bytes;
+};
+GradSpace grad_space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool pack_b, size_t partials, bool bias) {
+    Carver c{base};
+    GradSpace s{};
+    s.dz = own_dz ? c.take<uint16_t>((size_t)m * round8(n)) : nullptr;
+    s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
+    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
+    s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
+    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
+    s.bytes = c.used;
+    return s;
+}
+
+// one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
+template <Layout LA, Layout LB>
+int grad_product(const char *who, const Plan &p, const Shape &s, uint16_t *out, long ld, float *part) {
+    if (p.splits == 1) return run_product<LA, LB>(p, s, StoreBf16{out, ld, aligned_rows(out, ld)}, who);
+    if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
+    fc_finish<uint16_t><<<grid_of((size_t)s.m * s.n), 256, 0, stream()>>>(part, p.splits, s.n, (long)s.m * s.n, nullptr,
+                                                                          SWC_HIP_ACT_NONE, nullptr, 0, nullptr, 0, out, ld, s.m, s.n);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+size_t max2(size_t a, size_t b) { return a > b ? a : b; }
+
+int grad_bf16(const char *who, int m, int n, int k, const uint16_t *dc, long lddc, const uint16_t *a, long lda,
+              const uint16_t *b, long ldb, const uint16_t *preact, long ldp, int act, uint16_t *da, long ldda, uint16_t *db,
+              long lddb, uint16_t *dbias) {
+    const Plan pa = plan_product(m, k, n), pb = plan_product(k, n, m);
+    // dZ is dC itself without an activation; a copy when its rows do not start on 16-byte boundaries, or when dA would
+    // read past the end of a row
+    const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || (da && n % 8));
+    const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || n % 8);
+    const size_t partials = max2(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
+    const size_t need = grad_space(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
+    GradSpace w{};
+    if (need) {
+        char *base = static_cast<char *>(workspace(need, who));
+        if (!base) return fail_code();
+        w = grad_space(base, m, n, k, own_dz, pack_a, pack_b, partials, dbias);
+    }
+    if (own_dz || dbias) {
+        if (int rc = launch_act_grad<uint16_t>(w.dz, round8(n), dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
+        if (dbias)
+            if (int rc = sum_parts(dbias, nullptr, w.sums, sum_blocks(m), n)) return rc;
+    }
+    const uint16_t *dz = own_dz ? w.dz : dc;
+    const long lddz = own_dz ? round8(n) : lddc;
+    if (pack_b) {
+        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = round8(n);
+    }
+    if (pack_a) {
+        if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, nullptr, nullptr)) return rc;
+        a = w.a, lda = round8(k);
+    }
+    if (da)
+        if (int rc = grad_product<kAlongK, kAlongK>(who, pa, Shape{dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
+    if (db)
+        if (int rc = grad_product<kAcross, kAcross>(who, pb, Shape{a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
+    return SWC_HIP_OK;
+}
+
+struct GradSpaceF {
+    float *dz, *at, *bt, *part, *sums;
+    size_t bytes;
+};
+GradSpaceF grad_space_f(char *base, int m, int n, int k, bool own_dz, bool da, bool db, size_t partials, bool bias) {
+    Carver c{base};
+    GradSpaceF s{};
+    s.dz = own_dz ? c.take<float>((size_t)m * n) : nullptr;
+    s.at = db ? c.take<float>((size_t)m * k) : nullptr;
+    s.bt = da ? c.take<float>((size_t)k * n) : nullptr;
+    s.part = c.take<float>(partials / sizeof(float) + 1);
+    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
+    s.bytes = c.used;
+    return s;
+}
+
+int grad_f32(const char *who, int m, int n, int k, const float *dc, int lddc, const float *a, int lda, const float *b, int ldb,
+             const float *preact, int ldp, int act, float *da, int ldda, float *db, int lddb, float *dbias) {
+    const bool own_dz = (da || db) && act != SWC_HIP_ACT_NONE;
+    const size_t partials = max2(da ? swc_hip_gemm_workspace_bytes(m, k, n) : 0, db ? swc_hip_gemm_workspace_bytes(k, n, m) : 0);
+    const size_t need = grad_space_f(nullptr, m, n, k, own_dz, da, db, partials, dbias).bytes;
+    char *base = static_cast<char *>(workspace(need, who));
+    if (!base) return fail_code();
+    const GradSpaceF w = grad_space_f(base, m, n, k, own_dz, da, db, partials, dbias);
+    if (own_dz || dbias) {
+        if (int rc = launch_act_grad<float>(w.dz, n, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
+        if (dbias)
+            if (int rc = sum_parts(nullptr, dbias, w.sums, sum_blocks(m), n)) return rc;
+    }
+    const float *dz = own_dz ? w.dz : dc;
+    const int lddz = own_dz ? n : lddc;
+    if (da) {
+        if (int rc = swc_hip_matrixTrans_f(k, n, b, ldb, w.bt, k)) return rc;
+        if (int rc = gemm_f32(who, m, k, n, dz, lddz, w.bt, k, nullptr, da, ldda, 0, w.part, partials)) return rc;
+    }
+    if (db) {
+        if (int rc = swc_hip_matrixTrans_f(m, k, a, lda, w.at, m)) return rc;
+        if (int rc = gemm_f32(who, k, n, m, w.at, m, dz, lddz, nullptr, db, lddb, 0, w.part, partials)) return rc;
+    }
+    return SWC_HIP_OK;
+}
+
+// what every form of the gradient call answers with when there is nothing to sum over
+template <class T>
+int grad_of_nothing(int m, int n, int k, T *da, int ldda, T *db, int lddb, T *dbias) {
+    if (int rc = zero_rows(da, ldda, m, k)) return rc;
+    if (int rc = zero_rows(db, lddb, k, n)) return rc;
+    return zero_rows(dbias, n, 1, n);
+}
+
+} // namespace
+
+int swc_hip::mfma16::copy_rows_bf16(uint16_t *dst, long ld, const uint16_t *src, long lds, int rows, int cols, const int *index,
+                                    const int *count) {
+    return launch_copy_rows(dst, ld, src, lds, rows, cols, index, count);
+}
+int swc_hip::mfma16::copy_rows_f32(float *dst, long ld, const float *src, long lds, int rows, int cols, const int *index,
+                                   const int *count) {
+    return launch_copy_rows(dst, ld, src, lds, rows, cols, index, count);
+}
+int swc_hip::mfma16::sum_parts(uint16_t *out_bf, float *out_f, const float *part, int parts, int n) {
+    if (!n) return SWC_HIP_OK;
+    add_parts<<<ceil_div(n, 256), 256, 0, stream()>>>(out_bf, out_f, part, parts, n);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+extern "C" {
+
+int swc_hip_matrixMatrixFCActAdd_f(int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
+                                   int act, const float *residual, int ldr, float *preact, int ldp, float *c, int ldc) {
+    const char *who = "swc_hip_matrixMatrixFCActAdd_f";
+    if (int rc = check_forward(who, m, n, k, a, lda, b, ldb, act, residual, ldr, preact, ldp, c, ldc)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return SWC_HIP_OK;
+    // Z goes to preact, or to C, or to the workspace where C still holds the second summand
+    const size_t split = k ? swc_hip_gemm_workspace_bytes(m, n, k) : 0;
+    const bool apart = !preact && residual == c;
+    Carver size{nullptr};
+    size.take<float>(split / sizeof(float) + 1);
+    if (apart) size.take<float>((size_t)m * n);
+    char *base = nullptr;
+    if (split || apart) {
+        base = static_cast<char *>(workspace(size.used, who));
+        if (!base) return fail_code();
+    }
+    Carver w{base};
+    float *part = w.take<float>(split / sizeof(float) + 1);
+    float *z = apart ? w.take<float>((size_t)m * n) : preact ? preact : c;
+    const int ldz = apart ? n : preact ? ldp : ldc;
+    if (k) {
+        // (no scratch needed: any address that is not null stands for the empty array)
+        if (int rc = gemm_f32(who, m, n, k, a, lda, b, ldb, bias, z, ldz, 0, part ? part : z, split)) return rc;
+        bias = nullptr;
+    } else {
+        if (int rc = zero_rows(z, ldz, m, n)) return rc;
+    }
+    if (act == SWC_HIP_ACT_NONE && !residual && z == c && !bias) return SWC_HIP_OK;
+    fc_finish<float><<<grid_of((size_t)m * n), 256, 0, stream()>>>(z, 1, ldz, 0, bias, act, residual, ldr, k ? nullptr : preact, ldp,
+                                                                   c, ldc, m, n);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+int swc_hip_matrixMatrixFCActAdd_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda, const swc_hip_bf16 *b, int ldb,
+                                    const swc_hip_bf16 *bias, int act, const swc_hip_bf16 *residual, int ldr,
+                                    swc_hip_bf16 *preact, int ldp, swc_hip_bf16 *c, int ldc) {
+    const char *who = "swc_hip_matrixMatrixFCActAdd_bf";
+    if (int rc = check_forward(who, m, n, k, a, lda, b, ldb, act, residual, ldr, preact, ldp, c, ldc)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return SWC_HIP_OK;
+    if (k == 0) {
+        fc_finish<uint16_t><<<grid_of((size_t)m * n), 256, 0, stream()>>>(nullptr, 0, 0, 0, bias, act, residual, ldr, preact, ldp, c,
+                                                                          ldc, m, n);
+        SWC_LAUNCH_CHECK();
+        return SWC_HIP_OK;
+    }
+    return forward_bf16(who, m, n, k, a, lda, b, ldb, bias, act, residual, ldr, preact, ldp, c, ldc);
+}
+
+size_t swc_hip_matrixMatrixFCActAdd_workspace_bytes(int m, int n, int k, int bf) {
+    if (!ready() || m <= 0 || n <= 0 || k <= 0) return 0;
+    if (bf) return forward_space(nullptr, plan_product(m, n, k), m, n, k, true, true).bytes;
+    Carver c{nullptr};
+    c.take<float>(swc_hip_gemm_workspace_bytes(m, n, k) / sizeof(float) + 1);
+    c.take<float>((size_t)m * n);
+    return c.used;
+}
+
+int swc_hip_matrixMatrixFCActAddGrad_f(int m, int n, int k, const float *cGrad, int ldcg, const float *a, int lda, const float *b,
+                                       int ldb, const float *preact, int ldp, int act, float *aGrad, int ldag, float *bGrad,
+                                       int ldbg, float *biasGrad) {
+    const char *who = "swc_hip_matrixMatrixFCActAddGrad_f";
+    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
+    if (k == 0) aGrad = bGrad = nullptr;
+    return grad_f32(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+}
+
+int swc_hip_matrixMatrixFCActAddGrad_bf(int m, int n, int k, const swc_hip_bf16 *cGrad, int ldcg, const swc_hip_bf16 *a, int lda,
+                                        const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *preact, int ldp, int act,
+                                        swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad, int ldbg, swc_hip_bf16 *biasGrad) {
+    const char *who = "swc_hip_matrixMatrixFCActAddGrad_bf";
+    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
+    if (k == 0) aGrad = bGrad = nullptr;
+    return grad_bf16(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+}
+
+size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int bf) {
+    if (!ready() || m <= 0 || n <= 0) return 0;
+    if (bf) {
+        const size_t partials = k > 0 ? max2(plan_product(m, k, n).partial_bytes(m, k), plan_product(k, n, m).partial_bytes(k, n)) : 0;
+        return grad_space(nullptr, m, n, k, true, true, true, partials, true).bytes;
+    }
+    const size_t partials = max2(swc_hip_gemm_workspace_bytes(m, k, n), swc_hip_gemm_workspace_bytes(k, n, m));
+    return grad_space_f(nullptr, m, n, k, true, true, true, partials, true).bytes;
+}
+
+} // extern "C"

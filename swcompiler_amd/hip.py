@@ -33,7 +33,18 @@ EXPORTS = [
     "swc_hip_set_workspace", "swc_hip_matrixMatrixFCBiasSoftmax_f", "swc_hip_gemm_workspace_bytes", "swc_hip_conv2d_workspace_bytes", "swc_hip_host_malloc", "swc_hip_host_free", "swc_hip_matrixTrans_f", "swc_hip_matrixTanhGrad_f", "swc_hip_matrixSoftmaxWithLoss_f",
     "swc_hip_matrixSoftmaxGrad_f", "swc_hip_matrixSoftmaxWithLossGrad_f", "swc_hip_conv2dGrad_f",
     "swc_hip_maxpoolGrad_f", "swc_hip_batchedreduceadd_f", "swc_hip_sgd_f", "swc_hip_reluGrad_f",
+    "swc_hip_matrixMatrixFCActAdd_f", "swc_hip_matrixMatrixFCActAdd_bf", "swc_hip_matrixMatrixFCActAdd_workspace_bytes",
+    "swc_hip_matrixMatrixFCActAddGrad_f", "swc_hip_matrixMatrixFCActAddGrad_bf",
+    "swc_hip_matrixMatrixFCActAddGrad_workspace_bytes",
+    "swc_hip_matrixFCSoftmaxWithLoss_f", "swc_hip_matrixFCSoftmaxWithLoss_bf",
+    "swc_hip_matrixFCSoftmaxWithLoss_workspace_bytes", "swc_hip_matrixFCSoftmaxWithLossGrad_f",
+    "swc_hip_matrixFCSoftmaxWithLossGrad_bf", "swc_hip_matrixFCSoftmaxWithLossGrad_workspace_bytes",
+    "swc_hip_adamwAdvance", "swc_hip_adamw_f", "swc_hip_adamw_bf", "swc_hip_adamw8_f", "swc_hip_adamw8_bf",
 ]
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}   # the SWC_HIP_ACT_* values
+ADAMW_STATE_WORDS = 8     # SWC_HIP_ADAMW_STATE_BYTES in 32-bit words
+ADAMW_BLOCK = 256         # elements that share a scale of the 8-bit states
 
 
 class SwcHipError(RuntimeError):
@@ -53,6 +64,12 @@ def load_library():
     lib = C.CDLL(path)
     vp, sz, i32, f32 = C.c_void_p, C.c_size_t, C.c_int, C.c_float
     szp = C.POINTER(C.c_size_t)
+    f64 = C.c_double
+    fc = [i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32]
+    fc_grad = [i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, i32, vp, i32, vp, i32, vp]
+    loss = [i32, i32, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp]
+    loss_grad = [i32, i32, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, i32, vp, i32, vp]
+    adamw_tail = [vp, szp, vp, f32, f64, f64, f32, f32, vp, vp]
     sig = {
         "swc_hip_init": (i32, [i32]),
         "swc_hip_shutdown": (i32, []),
@@ -130,6 +147,23 @@ def load_library():
         "swc_hip_batchedreduceadd_f": (i32, [vp, vp, sz, sz]),
         "swc_hip_sgd_f": (i32, [sz, vp, vp, vp, vp, f32, f32, f32, sz]),
         "swc_hip_reluGrad_f": (i32, [vp, vp, vp, sz]),
+        "swc_hip_matrixMatrixFCActAdd_f": (i32, fc),
+        "swc_hip_matrixMatrixFCActAdd_bf": (i32, fc),
+        "swc_hip_matrixMatrixFCActAdd_workspace_bytes": (sz, [i32] * 4),
+        "swc_hip_matrixMatrixFCActAddGrad_f": (i32, fc_grad),
+        "swc_hip_matrixMatrixFCActAddGrad_bf": (i32, fc_grad),
+        "swc_hip_matrixMatrixFCActAddGrad_workspace_bytes": (sz, [i32] * 4),
+        "swc_hip_matrixFCSoftmaxWithLoss_f": (i32, loss),
+        "swc_hip_matrixFCSoftmaxWithLoss_bf": (i32, loss),
+        "swc_hip_matrixFCSoftmaxWithLoss_workspace_bytes": (sz, [i32] * 4),
+        "swc_hip_matrixFCSoftmaxWithLossGrad_f": (i32, loss_grad),
+        "swc_hip_matrixFCSoftmaxWithLossGrad_bf": (i32, loss_grad),
+        "swc_hip_matrixFCSoftmaxWithLossGrad_workspace_bytes": (sz, [i32] * 4),
+        "swc_hip_adamwAdvance": (i32, [vp, f64, f64]),
+        "swc_hip_adamw_f": (i32, [i32] + [vp] * 4 + adamw_tail),
+        "swc_hip_adamw_bf": (i32, [i32] + [vp] * 4 + adamw_tail),
+        "swc_hip_adamw8_f": (i32, [i32] + [vp] * 6 + adamw_tail),
+        "swc_hip_adamw8_bf": (i32, [i32] + [vp] * 6 + adamw_tail),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -148,8 +182,46 @@ def pool_out_dims(idims, kernels, strides, pads):
             (w + pads[1] + pads[3] - kernels[1]) // strides[1] + 1, c)
 
 
+class _Arg:
+    """What an op needs of an operand: its address, shape, element type and row stride.  Operands are DeviceArrays or
+    torch tensors on the runtime's device (taken as they are: any row stride, columns contiguous)."""
+
+    __slots__ = ("ptr", "shape", "type", "ld", "size")
+
+    def __init__(self, rt, x, what):
+        self.shape = tuple(x.shape)
+        self.size = 1
+        for n in self.shape:
+            self.size *= n
+        if isinstance(x, DeviceArray):
+            self.ptr, self.type = x.ptr, _NUMPY_TYPES.get(x.dtype.name)
+            self.ld = self.shape[-1] if self.shape else 1
+            return
+        if not hasattr(x, "data_ptr"):
+            raise SwcHipError(f"{what}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
+        if x.device.type != "cuda" or x.device.index != rt.device:
+            raise SwcHipError(f"{what}: the tensor is on {x.device}, the runtime on device {rt.device}")
+        self.ptr, self.type = x.data_ptr() or None, _TORCH_TYPES.get(str(x.dtype))
+        stride = x.stride()
+        for n, st in zip(self.shape[-1:], stride[-1:]):
+            if n > 1 and st != 1:
+                raise SwcHipError(f"{what}: the elements of a row are not contiguous (stride {st})")
+        self.ld = self.shape[-1] if self.shape else 1
+        if len(self.shape) == 2 and self.shape[0] > 1:
+            self.ld = stride[0]
+            if self.ld < self.shape[1]:
+                raise SwcHipError(f"{what}: rows overlap (stride {self.ld}, {self.shape[1]} columns)")
+        elif len(self.shape) > 2 and not x.is_contiguous():
+            raise SwcHipError(f"{what}: the tensor is not contiguous")
+
+
+_NUMPY_TYPES = {"float32": "f32", "int32": "i32", "uint16": "bf16", "uint8": "u8"}   # bfloat16 travels as its bits
+_TORCH_TYPES = {"torch.float32": "f32", "torch.int32": "i32", "torch.bfloat16": "bf16", "torch.uint16": "bf16",
+                "torch.uint8": "u8", "torch.float8_e4m3fn": "u8"}
+
+
 class DeviceArray:
-    """A device allocation with a shape and dtype (float32 or int32)."""
+    """A device allocation with a shape and dtype (float32, int32, uint16 for bfloat16 bits, or uint8)."""
 
     def __init__(self, rt, shape, dtype=np.float32):
         self.rt = rt
@@ -206,6 +278,7 @@ class SwcHip:
         self.lib = load_library()
         self._check(self.lib.swc_hip_init(device), "swc_hip_init")
         self._check(self.lib.swc_hip_enable_auto_workspace(int(auto_workspace)), "swc_hip_enable_auto_workspace")
+        self.device = device
         self._pinned = {}   # address of a pinned numpy array -> the pointer to free
         self._bench_lib = None
 
@@ -222,6 +295,10 @@ class SwcHip:
     def reload_switches(self):
         """have the library read the SWC_HIP_* environment variables again (it reads them once, at init)"""
         self._check(self.lib.swc_hip_reload_switches(), "swc_hip_reload_switches")
+
+    def use_default_stream(self):
+        """launch on the device's default (null) stream, the one torch uses unless told otherwise"""
+        self._check(self.lib.swc_hip_set_stream(C.c_void_p(1)), "swc_hip_set_stream")   # hipStreamLegacy
 
     # -- plumbing --------------------------------------------------------
     def _check(self, rc, what):
@@ -245,7 +322,7 @@ class SwcHip:
 
     def upload(self, host):
         host = np.ascontiguousarray(host)
-        assert host.dtype in (np.float32, np.int32)
+        assert host.dtype in (np.float32, np.int32, np.uint16, np.uint8)
         d = DeviceArray(self, host.shape, host.dtype)
         self._check(self.lib.swc_hip_h2d(d.ptr, host.ctypes.data, host.nbytes), "swc_hip_h2d")
         return d
@@ -599,6 +676,158 @@ class SwcHip:
         out = out if out is not None else self.empty(src.shape)
         self._check(self.lib.swc_hip_reluGrad_f(out.ptr, src.ptr, dest_grad.ptr, src.size), "reluGrad_f")
         return out
+
+    # -- operators of language models (matrices fp32 or bfloat16; DeviceArrays or torch tensors) --
+    def _arg(self, x, what, types, shape=None):
+        """the operand as an _Arg; None for None"""
+        if x is None:
+            return None
+        a = _Arg(self, x, what)
+        if a.type not in types:
+            raise SwcHipError(f"{what}: element type {a.type or x.dtype} is not one of {', '.join(types)}")
+        if shape is not None and a.shape != tuple(shape):
+            raise SwcHipError(f"{what}: shape {a.shape}, expected {tuple(shape)}")
+        return a
+
+    @staticmethod
+    def _p(a):
+        return None if a is None else a.ptr
+
+    @staticmethod
+    def _ld(a, other=0):
+        return other if a is None else a.ld
+
+    def _out(self, out, shape, like):
+        return out if out is not None else self.empty(shape, np.float32 if like == "f32" else np.uint16)
+
+    def _product(self, a, b, what):
+        a, b = self._arg(a, what + ": a", ("f32", "bf16")), self._arg(b, what + ": b", ("f32", "bf16"))
+        if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0] or a.type != b.type:
+            raise SwcHipError(f"{what}: a {a.shape} {a.type} and b {b.shape} {b.type} do not multiply")
+        return a, b, a.shape[0], b.shape[1], a.shape[1], (a.type,), "_f" if a.type == "f32" else "_bf"
+
+    @staticmethod
+    def _activation(act):
+        if act not in ACTIVATIONS:
+            raise SwcHipError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+        return ACTIVATIONS[act]
+
+    def matrixMatrixFCActAdd(self, a, b, bias=None, act="none", residual=None, preact=None, out=None):
+        """act(a b + bias) + residual; preact receives a b + bias"""
+        what = "matrixMatrixFCActAdd"
+        a, b, m, n, k, t, suffix = self._product(a, b, what)
+        act = self._activation(act)
+        out = self._out(out, (m, n), t[0])
+        c = self._arg(out, what + ": out", t, (m, n))
+        bias, r = self._arg(bias, what + ": bias", t, (n,)), self._arg(residual, what + ": residual", t, (m, n))
+        z = self._arg(preact, what + ": preact", t, (m, n))
+        self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAdd" + suffix)(
+            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), act, self._p(r), self._ld(r), self._p(z),
+            self._ld(z), c.ptr, c.ld), what)
+        return out
+
+    def matrixMatrixFCActAddGrad(self, dc, a, b, preact=None, act="none", da=None, db=None, dbias=None):
+        """the gradients of matrixMatrixFCActAdd into those of da, db and dbias that are given; all three, new, if none is"""
+        what = "matrixMatrixFCActAddGrad"
+        a, b, m, n, k, t, suffix = self._product(a, b, what)
+        act = self._activation(act)
+        if da is None and db is None and dbias is None:
+            da, db, dbias = self._out(None, (m, k), t[0]), self._out(None, (k, n), t[0]), self._out(None, (n,), t[0])
+        g, z = self._arg(dc, what + ": dc", t, (m, n)), self._arg(preact, what + ": preact", t, (m, n))
+        ga, gb = self._arg(da, what + ": da", t, (m, k)), self._arg(db, what + ": db", t, (k, n))
+        gbias = self._arg(dbias, what + ": dbias", t, (n,))
+        self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAddGrad" + suffix)(
+            m, n, k, g.ptr, g.ld, a.ptr, a.ld, b.ptr, b.ld, self._p(z), self._ld(z), act, self._p(ga),
+            self._ld(ga), self._p(gb), self._ld(gb), self._p(gbias)), what)
+        return da, db, dbias
+
+    def matrixFCSoftmaxWithLoss(self, a, b, bias, selected, row_loss=None, lse=None, loss=None):
+        """-> (loss, row_loss, lse) of the softmax over the rows of a b + bias, whose logits are never stored"""
+        what = "matrixFCSoftmaxWithLoss"
+        a, b, m, n, k, t, suffix = self._product(a, b, what)
+        loss, row_loss, lse = self._out(loss, (), "f32"), self._out(row_loss, (m,), "f32"), self._out(lse, (m,), "f32")
+        bias, sel = self._arg(bias, what + ": bias", t, (n,)), self._arg(selected, what + ": selected", ("i32",), (m,))
+        one = self._arg(loss, what + ": loss", ("f32",))
+        if one.size != 1:
+            raise SwcHipError(f"{what}: loss: shape {one.shape}, expected one value")
+        rl, ls = self._arg(row_loss, what + ": row_loss", ("f32",), (m,)), self._arg(lse, what + ": lse", ("f32",), (m,))
+        self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLoss" + suffix)(
+            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, rl.ptr, ls.ptr, one.ptr), what)
+        return loss, row_loss, lse
+
+    def matrixFCSoftmaxWithLossGrad(self, a, b, bias, selected, lse, row_grad=None, da=None, db=None, dbias=None):
+        """the gradients of the rows' losses (times row_grad) into those of da, db and dbias that are given; all three,
+        new, if none is"""
+        what = "matrixFCSoftmaxWithLossGrad"
+        a, b, m, n, k, t, suffix = self._product(a, b, what)
+        if da is None and db is None and dbias is None:
+            da, db, dbias = self._out(None, (m, k), t[0]), self._out(None, (k, n), t[0]), self._out(None, (n,), t[0])
+        bias, sel = self._arg(bias, what + ": bias", t, (n,)), self._arg(selected, what + ": selected", ("i32",), (m,))
+        ls, rg = self._arg(lse, what + ": lse", ("f32",), (m,)), self._arg(row_grad, what + ": row_grad", ("f32",), (m,))
+        ga, gb = self._arg(da, what + ": da", t, (m, k)), self._arg(db, what + ": db", t, (k, n))
+        gbias = self._arg(dbias, what + ": dbias", t, (n,))
+        self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLossGrad" + suffix)(
+            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, ls.ptr, self._p(rg), self._p(ga), self._ld(ga),
+            self._p(gb), self._ld(gb), self._p(gbias)), what)
+        return da, db, dbias
+
+    def adamw_state(self):
+        """a new step counter for adamwAdvance, at zero"""
+        state = self.empty((ADAMW_STATE_WORDS,), np.int32)
+        self._check(self.lib.swc_hip_fill_i(state.ptr, 0, ADAMW_STATE_WORDS), "swc_hip_fill_i")
+        return state
+
+    def _state(self, state, what):
+        return self._arg(state, what + ": state", ("i32",), (ADAMW_STATE_WORDS,)).ptr
+
+    def adamwAdvance(self, state, beta1, beta2):
+        """begins a step: counts it and prepares the bias corrections of the updates that follow"""
+        state = self._state(state, "adamwAdvance")
+        self._check(self.lib.swc_hip_adamwAdvance(state, beta1, beta2), "adamwAdvance")
+
+    def _adamw(self, what, w, dw, states, scales, copies, state, lr, beta1, beta2, eps, decay, lr_factor, grad_factor):
+        count = len(w)
+        sizes, dtype = (C.c_size_t * count)(), None
+        lists = [w, dw] + states + scales + ([copies] if copies is not None else [])
+        if any(len(x) != count for x in lists):
+            raise SwcHipError(f"{what}: lists of different lengths")
+        pointers = [(C.c_void_p * count)() for _ in lists]
+        state_type = ("u8",) if scales else ("f32",)
+        types = [("f32",), ("f32", "bf16")] + [state_type] * 2 + [("f32",)] * len(scales) + [("bf16",)]
+        for i in range(count):
+            for j, values in enumerate(lists):
+                if values[i] is None and copies is not None and j == len(lists) - 1:
+                    continue
+                x = self._arg(values[i], f"{what}: tensor {i}", types[j])
+                if len(x.shape) == 2 and x.ld != x.shape[1]:
+                    raise SwcHipError(f"{what}: tensor {i} is not contiguous")
+                if j == 0:
+                    sizes[i] = x.size
+                want = -(-sizes[i] // ADAMW_BLOCK) if 4 <= j < 4 + len(scales) else sizes[i]
+                if x.size != want:
+                    raise SwcHipError(f"{what}: tensor {i}: {x.size} elements, expected {want}")
+                if j == 1:
+                    if dtype not in (None, x.type):
+                        raise SwcHipError(f"{what}: gradients of different types")
+                    dtype = x.type
+                pointers[j][i] = x.ptr
+        if scales:   # w, dw, mom8, momScale, var8, varScale
+            pointers[3], pointers[4] = pointers[4], pointers[3]
+        if copies is None:
+            pointers.append(None)
+        one = [self._p(self._arg(x, f"{what}: factor", ("f32",))) for x in (lr_factor, grad_factor)]
+        fn = getattr(self.lib, f"swc_hip_{what}" + ("_bf" if dtype == "bf16" else "_f"))
+        self._check(fn(count, *pointers, sizes, self._state(state, what), lr, beta1, beta2, eps, decay, *one), what)
+
+    def adamw(self, w, dw, mom, var, state, lr, beta1, beta2, eps, decay, copies=None, lr_factor=None, grad_factor=None):
+        """one AdamW step of the tensors in the lists w, dw, mom, var (and their bfloat16 copies), in place"""
+        self._adamw("adamw", w, dw, [mom, var], [], copies, state, lr, beta1, beta2, eps, decay, lr_factor, grad_factor)
+
+    def adamw8(self, w, dw, mom, mom_scale, var, var_scale, state, lr, beta1, beta2, eps, decay, copies=None, lr_factor=None,
+               grad_factor=None):
+        """the same with the states in 8 bits and a scale per ADAMW_BLOCK elements"""
+        self._adamw("adamw8", w, dw, [mom, var], [mom_scale, var_scale], copies, state, lr, beta1, beta2, eps, decay,
+                    lr_factor, grad_factor)
 
     def pinned_empty(self, shape, dtype=np.float32):
         """a numpy array in page-locked host memory (kept alive by the returned array; freed with free_pinned)"""
