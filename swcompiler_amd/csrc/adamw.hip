@@ -87,10 +87,15 @@ __device__ __forceinline__ Scalars scalars(const Step &s) {
     r.c2 = s.state->c2;
     return r;
 }
+// The states' operations are rounded one by one, as sgd_f's are: they are the same bits wherever they are computed, and
+// with them the 8-bit codes that a later step starts from.
 __device__ __forceinline__ void step_one(float &w, float g, float &mom, float &var, const Scalars &k, const Step &s) {
-    g *= k.g;
-    mom = s.beta1 * mom + s.rest1 * g;
-    var = s.beta2 * var + s.rest2 * (g * g);
+    {
+#pragma clang fp contract(off)
+        g = g * k.g;
+        mom = mom * s.beta1 + g * s.rest1;
+        var = var * s.beta2 + (g * g) * s.rest2;
+    }
     w = w * k.shrink - k.c1 * mom / (sqrtf(var * k.c2) + s.eps);
 }
 
@@ -139,10 +144,14 @@ __device__ __forceinline__ float from_e4m3(unsigned byte) {
     return 0.f;
 #endif
 }
-// to the nearest value, ties to even; |y| <= 448
-__device__ __forceinline__ unsigned to_e4m3(float y) {
+// The codes are settled in 64 bits (a float by the reciprocal of a float: nothing that fp32 would round across a border).
+// To the nearest value, ties to even; |y| <= 448.  The conversion instruction rounds an fp32: y goes there cut to 20
+// mantissa bits with the last one set if anything was cut off, which keeps it on its side of every border.
+__device__ __forceinline__ unsigned to_e4m3(double y) {
 #if __HIP_DEVICE_COMPILE__
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xffu;
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, y);
+    const float x = (float)__builtin_bit_cast(double, (b & ~0xffffffffull) | ((b & 0xffffffffull) ? 1ull << 32 : 0));
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu;
 #else
     return 0;
 #endif
@@ -150,12 +159,12 @@ __device__ __forceinline__ unsigned to_e4m3(float y) {
 // 0 <= y <= 448 up or down by 20 random bits: with the exponent E of y (at least that of the least normal value) the
 // values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is 8 (E + 7) + q - 8 — also
 // where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the subnormal values).
-__device__ __forceinline__ unsigned to_e4m3_random(float y, unsigned bits20) {
-    const int e = max((int)(__builtin_bit_cast(unsigned, y) >> 23) - 127, -6);
-    const float units = __builtin_bit_cast(float, (unsigned)(127 + 3 - e) << 23);   // 2^(3 - E)
-    float q = floorf(y * units + (float)bits20 * 0x1p-20f);
-    if (y > 0.f) q = fmaxf(q, 1.f);
-    return (unsigned)(8 * (e + 7) + (int)q - 8);
+__device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
+    const int e = max((int)(__builtin_bit_cast(unsigned long long, y) >> 52) - 1023, -6);
+    const double units = __builtin_bit_cast(double, (unsigned long long)(1023 + 3 - e) << 52);   // 2^(3 - E)
+    int q = (int)(y * units + (double)bits20 * 0x1p-20);
+    if (y > 0) q = max(q, 1);
+    return (unsigned)(8 * (e + 7) + q - 8);
 }
 
 // A wavefront owns a block of 256 elements, lane l its elements l, l + 64, l + 128, l + 192.
@@ -189,21 +198,21 @@ __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTenso
         }
     }
     top = wave_max(top), peak = wave_max(peak);
-    const bool has_m = top > kTiny, has_v = peak > kTiny;
-    const float im = has_m ? kLargest / top : 0.f, iv = has_v ? kLargest / peak : 0.f;
+    const float mscale = top > kTiny ? top / kLargest : 0.f, vscale = peak > kTiny ? peak / kLargest : 0.f;
+    const double im = mscale > 0.f ? 1.0 / (double)mscale : 0.0, iv = vscale > 0.f ? 1.0 / (double)vscale : 0.0;
     const unsigned number = (unsigned)(tab.number0 + which) * 0x9E3779B9u + (unsigned)s.state->steps * 0x85EBCA6Bu;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const size_t i = i0 + e * 64;
         if (i < t.size) {
-            const float x = fminf(fmaxf(m[e] * im, -kLargest), kLargest), y = fminf(r[e] * iv, kLargest);
+            const double x = fmin(fmax(m[e] * im, -(double)kLargest), (double)kLargest), y = fmin(r[e] * iv, (double)kLargest);
             mom8[i] = (uint8_t)(fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8);
             var8[i] = (uint8_t)(r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)i + number)) : kNan8);
         }
     }
     if ((threadIdx.x & 63) == 0) {
-        t.mom_scale[block] = has_m ? top / kLargest : 0.f;
-        t.var_scale[block] = has_v ? peak / kLargest : 0.f;
+        t.mom_scale[block] = mscale;
+        t.var_scale[block] = vscale;
     }
 }
 

@@ -14,48 +14,55 @@ using namespace swc_hip::mfma16;
 
 namespace {
 
-struct FcEpilogue {
+template <int ACT> struct FcEpilogue {
+    static constexpr bool kHeavy = true, kTall = true;
     const uint16_t *bias, *residual;
     uint16_t *preact, *c;
     long ldr, ldp, ldc;
-    int act;
-    bool vec_r, vec_p, vec_c;
+    bool vec;   // every matrix given has 16-byte aligned rows, and the bias an 8-byte aligned start
 #if __HIP_DEVICE_COMPILE__
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
+    template <bool WHOLE, int TM, int TN>
+    __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
+        v2u b[TN][4];
+        v4u r[TN][2];
+        if (bias)
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
-            const int cb = col0 + tn * 32;
-            float b[16];
+            for (int tn = 0; tn < TN; ++tn) load_columns<WHOLE>(bias, col0 + tn * 32, n, h, b[tn]);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int col = cb + 8 * (v / 4) + 4 * h + v % 4;
-                b[v] = bias && col < n ? bf16_to_float(bias[col]) : 0.f;
-            }
+        for (int tm = 0; tm < TM; ++tm) {
+            const int row = row0 + tm * 32 + l32;
+            const bool ok = row < m;
+            // a row block's second summand is requested together, before its first use
+            if (residual)
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
-                const int row = row0 + tm * 32 + l32;
-                const bool ok = row < m;
-                float z[16], r[16];
-                if (residual) load_block(residual + row * ldr, ok, cb, n, vec_r, h, r);
+                for (int tn = 0; tn < TN; ++tn) load_block<WHOLE>(residual + row * ldr, ok, col0 + tn * 32, n, vec, h, r[tn]);
 #pragma unroll
-                for (int v = 0; v < 16; ++v) z[v] = acc[tm][tn][v] + b[v];
-                if (preact) store_block(preact + row * ldp, ok, cb, n, vec_p, h, z);
+            for (int tn = 0; tn < TN; ++tn) {
+                const int cb = col0 + tn * 32;
+                float z[16], x[16];
 #pragma unroll
-                for (int v = 0; v < 16; ++v) z[v] = act_value(z[v], act) + (residual ? r[v] : 0.f);
-                store_block(c + row * ldc, ok, cb, n, vec_c, h, z);
+                for (int v = 0; v < 16; ++v) z[v] = acc[tm][tn][v] + (bias ? column_value(b[tn], v) : 0.f);
+                if (preact) store_block<WHOLE>(preact + row * ldp, ok, cb, n, vec, h, z);
+                if (residual) unpack_block(r[tn], x);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) z[v] = act_value<ACT, true>(z[v]) + (residual ? x[v] : 0.f);
+                store_block<WHOLE>(c + row * ldc, ok, cb, n, vec, h, z);
             }
         }
+    }
+    template <int TM, int TN>
+    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
+        if (vec && row0 + 32 * TM <= m && col0 + 32 * TN <= n) finish<true>(acc, row0, col0, m, n, lane);
+        else finish<false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
 
 // The end of a layer from fp32 sums: `parts` matrices of m x n to be added in order, then bias, activation, residual.
-// z == nullptr: parts are the sums; otherwise (fp32) one matrix that already holds Z.
-template <class T>
-__global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long ldpart, long part_stride, const T *bias, int act,
+// (part may be c itself: fp32, one part)
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long ldpart, long part_stride, const T *bias,
                                                  const T *residual, long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
 #if __HIP_DEVICE_COMPILE__
     const size_t total = (size_t)m * n, step = (size_t)gridDim.x * 256;
@@ -65,34 +72,88 @@ __global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, l
         for (int p = 0; p < parts; ++p) z += part[p * part_stride + r * ldpart + j];
         if (bias) z += load_any(bias + j);
         if (preact) store_any(preact + r * ldp + j, z);
-        z = act_value(z, act);
+        z = act_value<ACT, sizeof(T) == 2>(z);
         if (residual) z += load_any(residual + r * ldr + j);
         store_any(c + r * ldc + j, z);
     }
 #endif
 }
-
-// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.
-constexpr int kSumRows = 64;
 template <class T>
-__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int act, int m,
-                                                int n, float *sums) {
+int launch_finish(int act, const float *part, int parts, long ldpart, long part_stride, const T *bias, const T *residual, long ldr,
+                  T *preact, long ldp, T *c, long ldc, int m, int n) {
+    return with_act(act, [&]<int ACT>() {
+        fc_finish<T, ACT><<<grid_of((size_t)m * n), 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact,
+                                                                        ldp, c, ldc, m, n);
+        SWC_LAUNCH_CHECK();
+        return (int)SWC_HIP_OK;
+    });
+}
+
+// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of kSumRows rows' column sums of the unrounded
+// values.  32 threads side by side hold eight columns each, eight rows at a time; VEC: 16 bytes of a row at once.
+constexpr int kSumRows = 64;
+template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int j, int n, float (&x)[8]) {
+    if constexpr (VEC && sizeof(T) == 2) {
+        const uint4 d = *reinterpret_cast<const uint4 *>(p + j);
+        const unsigned w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else if constexpr (VEC) {
+        const float4 a = *reinterpret_cast<const float4 *>(p + j), b = *reinterpret_cast<const float4 *>(p + j + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = j + e < n ? load_any(p + j + e) : 0.f;
+    }
+}
+template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int j, int n, const float (&x)[8]) {
 #if __HIP_DEVICE_COMPILE__
-    const int j = blockIdx.x * 256 + threadIdx.x;
+    if constexpr (VEC && sizeof(T) == 2) {
+        *reinterpret_cast<uint4 *>(p + j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    } else if constexpr (VEC) {
+        *reinterpret_cast<float4 *>(p + j) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + j + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (j + e < n) store_any(p + j + e, x[e]);
+    }
+#endif
+}
+
+template <class T, int ACT, bool VEC>
+__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums) {
+#if __HIP_DEVICE_COMPILE__
+    __shared__ float part[8][257];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int j = (blockIdx.x * 32 + tx) * 8;
     const int r0 = blockIdx.y * kSumRows;
     const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
-    if (j >= ld && j >= n) return;
-    float sum = 0.f;
-    for (int r = r0; r < r1; ++r) {
-        float g = 0.f;
-        if (j < n) {
-            g = load_any(dc + r * ldc + j);
-            if (act != SWC_HIP_ACT_NONE) g *= act_slope(load_any(z + r * ldz + j), act);
-            sum += g;
+    float sum[8] = {};
+    if (j < (n > ld ? n : ld))
+#pragma unroll 2
+        for (int r = r0 + ty; r < r1; r += 8) {
+            float g[8];
+            load8<T, VEC>(dc + r * ldc, j, n, g);
+            if constexpr (ACT != SWC_HIP_ACT_NONE) {
+                float y[8];
+                load8<T, VEC>(z + r * ldz, j, n, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, sizeof(T) == 2>(y[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += j + e < n ? g[e] : 0.f;
+            if (dz) store8<T, VEC>(dz + r * ld, j, (int)ld, g);
         }
-        if (dz && j < ld) store_any(dz + r * ld + j, g);
-    }
-    if (sums && j < n) sums[(size_t)blockIdx.y * n + j] = sum;
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    float s = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) s += part[y][threadIdx.x];
+    if (col < n) sums[(size_t)blockIdx.y * n + col] = s;
 #endif
 }
 
@@ -143,6 +204,9 @@ int check_forward(const char *who, int m, int n, int k, const T *a, int lda, con
     return SWC_HIP_OK;
 }
 
+// Few rows, or a cut contraction: sums to the workspace, the end of the layer in fc_finish.
+bool partial_sums(const Plan &p) { return p.splits > 1 || p.kind == kLow || p.kind == kThin; }
+
 struct ForwardSpace {
     uint16_t *a, *b;
     float *part;
@@ -153,7 +217,7 @@ ForwardSpace forward_space(char *base, const Plan &p, int m, int n, int k, bool 
     ForwardSpace s{};
     s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
     s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
-    s.part = p.splits > 1 ? c.take<float>((size_t)p.splits * m * n) : nullptr;
+    s.part = partial_sums(p) ? c.take<float>((size_t)p.splits * m * n) : nullptr;
     s.bytes = c.used;
     return s;
 }
@@ -179,16 +243,15 @@ int forward_bf16(const char *who, int m, int n, int k, const uint16_t *a, long l
         b = w.b, ldb = round8(n);
     }
     const Shape s{a, b, lda, ldb, m, n, k, 0, nullptr};
-    if (p.splits == 1) {
-        const FcEpilogue ep{bias, residual, preact, c, ldr, ldp, ldc, act, aligned_rows(residual, ldr), aligned_rows(preact, ldp),
-                            aligned_rows(c, ldc)};
-        return run_product<kAlongK, kAcross>(p, s, ep, who);
+    if (!partial_sums(p)) {
+        const bool vec = (!residual || aligned_rows(residual, ldr)) && (!preact || aligned_rows(preact, ldp)) && aligned_rows(c, ldc) &&
+                         (reinterpret_cast<uintptr_t>(bias) & 7) == 0;
+        return with_act(act, [&]<int ACT>() {
+            return run_product<kAlongK, kAcross>(p, s, FcEpilogue<ACT>{bias, residual, preact, c, ldr, ldp, ldc, vec}, who);
+        });
     }
     if (int rc = run_product<kAlongK, kAcross>(p, s, StorePartial{w.part, (long)m * n, n, false}, who)) return rc;
-    fc_finish<uint16_t><<<grid_of((size_t)m * n), 256, 0, stream()>>>(w.part, p.splits, n, (long)m * n, bias, act, residual, ldr,
-                                                                      preact, ldp, c, ldc, m, n);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
+    return launch_finish<uint16_t>(act, w.part, p.splits, n, (long)m * n, bias, residual, ldr, preact, ldp, c, ldc, m, n);
 }
 
 template <class T>
@@ -213,11 +276,18 @@ int sum_blocks(int m) { return (m + kSumRows - 1) / kSumRows; }
 
 template <class T>
 int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
-    const dim3 grid(ceil_div(dz && ld > n ? ld : n, 256), sum_blocks(m));
+    if (!dz) ld = 0;
+    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m));
     if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
-    act_grad<T><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, act, m, n, sums);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
+    constexpr int kPer = 16 / sizeof(T);
+    const bool vec = n % 8 == 0 && aligned16(dc) && lddc % kPer == 0 && (act == SWC_HIP_ACT_NONE || (aligned16(z) && ldz % kPer == 0)) &&
+                     (!dz || (aligned16(dz) && ld % kPer == 0));
+    return with_act(act, [&]<int ACT>() {
+        if (vec) act_grad<T, ACT, true><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        else act_grad<T, ACT, false><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        SWC_LAUNCH_CHECK();
+        return (int)SWC_HIP_OK;
+    });
 }
 
 struct GradSpace {
@@ -242,10 +312,8 @@ template <Layout LA, Layout LB>
 int grad_product(const char *who, const Plan &p, const Shape &s, uint16_t *out, long ld, float *part) {
     if (p.splits == 1) return run_product<LA, LB>(p, s, StoreBf16{out, ld, aligned_rows(out, ld)}, who);
     if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
-    fc_finish<uint16_t><<<grid_of((size_t)s.m * s.n), 256, 0, stream()>>>(part, p.splits, s.n, (long)s.m * s.n, nullptr,
-                                                                          SWC_HIP_ACT_NONE, nullptr, 0, nullptr, 0, out, ld, s.m, s.n);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
+    return launch_finish<uint16_t>(SWC_HIP_ACT_NONE, part, p.splits, s.n, (long)s.m * s.n, nullptr, nullptr, 0, nullptr, 0, out, ld, s.m,
+                                   s.n);
 }
 
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
@@ -386,10 +454,7 @@ int swc_hip_matrixMatrixFCActAdd_f(int m, int n, int k, const float *a, int lda,
         if (int rc = zero_rows(z, ldz, m, n)) return rc;
     }
     if (act == SWC_HIP_ACT_NONE && !residual && z == c && !bias) return SWC_HIP_OK;
-    fc_finish<float><<<grid_of((size_t)m * n), 256, 0, stream()>>>(z, 1, ldz, 0, bias, act, residual, ldr, k ? nullptr : preact, ldp,
-                                                                   c, ldc, m, n);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
+    return launch_finish<float>(act, z, 1, ldz, 0, bias, residual, ldr, k ? nullptr : preact, ldp, c, ldc, m, n);
 }
 
 int swc_hip_matrixMatrixFCActAdd_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda, const swc_hip_bf16 *b, int ldb,
@@ -399,12 +464,7 @@ int swc_hip_matrixMatrixFCActAdd_bf(int m, int n, int k, const swc_hip_bf16 *a, 
     if (int rc = check_forward(who, m, n, k, a, lda, b, ldb, act, residual, ldr, preact, ldp, c, ldc)) return rc;
     SWC_REQUIRE_INIT();
     if (m == 0 || n == 0) return SWC_HIP_OK;
-    if (k == 0) {
-        fc_finish<uint16_t><<<grid_of((size_t)m * n), 256, 0, stream()>>>(nullptr, 0, 0, 0, bias, act, residual, ldr, preact, ldp, c,
-                                                                          ldc, m, n);
-        SWC_LAUNCH_CHECK();
-        return SWC_HIP_OK;
-    }
+    if (k == 0) return launch_finish<uint16_t>(act, nullptr, 0, 0, 0, bias, residual, ldr, preact, ldp, c, ldc, m, n);
     return forward_bf16(who, m, n, k, a, lda, b, ldb, bias, act, residual, ldr, preact, ldp, c, ldc);
 }
 

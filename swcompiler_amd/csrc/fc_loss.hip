@@ -60,35 +60,41 @@ __global__ __launch_bounds__(kPickThreads) void pick_rows(const int *selected, i
 
 // ---------------------------------------------------------------- bf16 forward
 struct RowStats {
+    static constexpr bool kHeavy = true, kTall = false;
     float2 *part;     // [row][block]: maximum, sum of exp(z - maximum)
     int blocks;
     float *picked;    // [row]: z of the row's class
     const int *sel;
     const uint16_t *bias;
 #if __HIP_DEVICE_COMPILE__
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
+    template <bool WHOLE, int TM, int TN>
+    __device__ __forceinline__ void reduce(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
-        if (col0 >= n) return;
+        v2u b[TN][4];
+        if (bias)
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) load_columns<WHOLE>(bias, col0 + tn * 32, n, h, b[tn]);
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int row = row0 + tm * 32 + l32;
-            const int want = row < m ? sel[row] : -1;
+            const int want = (row < m ? sel[row] : -1) - col0;
             float z[TN * 16];
             float top = -__builtin_inff();
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const int col = col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4;
                     float x = acc[tm][tn][v];
-                    if (bias && col < n) x += bf16_to_float(bias[col]);
-                    if (col == want) picked[row] = x;
-                    x = col < n ? x : -__builtin_inff();
+                    if (bias) x += column_value(b[tn], v);
+                    if (!WHOLE && col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4 >= n) x = -__builtin_inff();
                     z[tn * 16 + v] = x;
                     top = fmaxf(top, x);
                 }
+            if (__any(want >= 0 && want < 32 * TN)) {   // a row of these 32 has its class here
+#pragma unroll
+                for (int v = 0; v < TN * 16; ++v)
+                    if (v / 16 * 32 + 8 * (v % 16 / 4) + 4 * h + v % 4 == want) picked[row] = z[v];
+            }
             top = fmaxf(top, __shfl_xor(top, 32));
             const float from = top == -__builtin_inff() ? 0.f : top;   // a block of impossible classes only
             float sum = 0.f;
@@ -97,6 +103,13 @@ struct RowStats {
             sum += __shfl_xor(sum, 32);
             if (h == 0 && row < m) part[(size_t)row * blocks + col0 / (32 * TN)] = make_float2(top, sum);
         }
+    }
+    template <int TM, int TN>
+    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
+                                               int) const {
+        if (col0 >= n) return;
+        if (col0 + 32 * TN <= n && (reinterpret_cast<uintptr_t>(bias) & 7) == 0) reduce<true>(acc, row0, col0, m, n, lane);
+        else reduce<false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
@@ -142,6 +155,7 @@ __global__ __launch_bounds__(1024) void mean_loss(const float *row_loss, Rows ro
 // ---------------------------------------------------------------- bf16 gradients
 // dz of a piece of the vocabulary whose first class is `first`, zeros in the columns that pad it to whole 16 bytes
 struct StoreDz {
+    static constexpr bool kHeavy = true, kTall = false;
     uint16_t *dz;
     long ld;
     int first;
@@ -149,30 +163,49 @@ struct StoreDz {
     const float *lse, *grad;
     const uint16_t *bias;   // of the piece
 #if __HIP_DEVICE_COMPILE__
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
+    template <bool WHOLE, int TM, int TN>
+    __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
+        v2u b[TN][4];
+        if (bias)
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) load_columns<WHOLE>(bias, col0 + tn * 32, n, h, b[tn]);
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int row = row0 + tm * 32 + l32;
-            const bool ok = row < m;
-            const int want = ok ? sel[row] - first : -1;
+            const bool ok = WHOLE || row < m;
+            const int want = (ok ? sel[row] : -1) - first - col0;
             const float l = ok ? lse[row] : 0.f, g = ok ? grad[row] : 0.f;
+            const bool here = __any(ok && want >= 0 && want < 32 * TN);   // a row of these 32 has its class here
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) {
                 float x[16];
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const int col = col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4;
                     float z = acc[tm][tn][v];
-                    if (bias && col < n) z += bf16_to_float(bias[col]);
-                    const float p = fast_exp(z - l);
-                    x[v] = col < n ? g * (col == want ? p - 1.f : p) : 0.f;
+                    if (bias) z += column_value(b[tn], v);
+                    x[v] = fast_exp(z - l);
                 }
-                store_block(dz + row * ld, ok, col0 + tn * 32, (int)ld, true, h, x);
+                if (here) {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (tn * 32 + 8 * (v / 4) + 4 * h + v % 4 == want) x[v] -= 1.f;
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    x[v] *= g;
+                    if (!WHOLE && col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4 >= n) x[v] = 0.f;
+                }
+                store_block<WHOLE>(dz + row * ld, ok, col0 + tn * 32, (int)ld, true, h, x);
             }
         }
+    }
+    template <int TM, int TN>
+    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
+                                               int) const {
+        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n && (reinterpret_cast<uintptr_t>(bias) & 7) == 0)
+            store<true>(acc, row0, col0, m, n, lane);
+        else store<false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
@@ -298,7 +331,8 @@ Plan whole_plan(int m, int n, int k) {
     p.k_per_split = ((k + 63) / 64 ? (k + 63) / 64 : 1) * 64;
     return p;
 }
-int block_columns(const Plan &p) { return p.kind == kThin ? 32 : 64; }
+int block_columns(const Plan &p) { return p.kind == kThin ? Thin::TN * 32 : 64; }
+static_assert(Big::TN == 2 && Mid::TN == 2 && Low::TN == 2, "64 columns a wavefront");
 
 // ---------------------------------------------------------------- spaces
 struct ForwardSpace {

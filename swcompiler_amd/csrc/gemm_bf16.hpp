@@ -55,22 +55,27 @@ struct Shape {
                        // exist, at most m resp. k; null: all of them
 };
 
-// TM x TN accumulators of 32 x 32 per wavefront, WM x WN wavefronts, slices of BK, STAGES of them in LDS.
-template <int TM_, int TN_, int WM_, int WN_, int BK_, int STAGES_>
+// TM x TN accumulators of 32 x 32 per wavefront, WM x WN wavefronts, slices of BK; SA slices of A and SB of B in LDS
+// (SA = SB, or SA = SB + 1).
+template <int TM_, int TN_, int WM_, int WN_, int BK_, int SA_, int SB_>
 struct Cfg {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, SA = SA_, SB = SB_;
     static constexpr int NW = WM * WN;
     static constexpr int kThreads = 64 * NW;
     static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     static constexpr int kABytes = BM * BK * 2, kBBytes = BN * BK * 2;
-    static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kLdsBytes = STAGES * kStageBytes;
+    static constexpr int kBBase = SA * kABytes;   // the stages of A, then those of B
+    static constexpr int kLdsBytes = SA * kABytes + SB * kBBytes;
     static constexpr int kALoads = kABytes / 1024 / NW, kBLoads = kBBytes / 1024 / NW;
     static constexpr int kLoads = kALoads + kBLoads;
     static constexpr int kSteps = BK / 16;
+    static constexpr bool kEarlyA = SA > SB;      // A's loads go out a slice ahead of B's (see tile_product)
+    static constexpr int kRound = SA == SB ? SA : SA * SB;   // slices after which both rings are where they were
+    // loads that may be pending where the next slice must have landed
+    static constexpr int kPending = kEarlyA ? (SB - 2) * kBLoads + (SB - 1) * kALoads : (SB - 2) * kLoads;
     static_assert(kALoads * 1024 * NW == kABytes && kBLoads * 1024 * NW == kBBytes, "whole 1-KiB loads per wavefront");
-    static_assert(kLdsBytes <= swc::devices::HipDevice::ldsBytesPerCU, "the ring must fit one CU's LDS");
-    static_assert(STAGES >= 2 && (STAGES - 1) * kLoads < 64, "pending loads must fit the vmcnt field");
+    static_assert(kLdsBytes <= swc::devices::HipDevice::ldsBytesPerCU, "the rings must fit one CU's LDS");
+    static_assert(SB >= 2 && (SA == SB || SA == SB + 1) && SB * kLoads < 64, "pending loads must fit the vmcnt field");
     static_assert(BK == 32 || BK == 64, "");
     static_assert(kSteps >= 2, "");
 };
@@ -138,10 +143,11 @@ struct Loader {
             }
         }
     }
-    __device__ __forceinline__ void issue(char *__restrict__ stage, int j, int wave) {
+    // WHOLE: the slice lies inside the contraction, no chunk has to be checked against its end
+    template <bool WHOLE> __device__ __forceinline__ void issue(char *__restrict__ stage, int j, int wave) {
         const long reach = left < 0 ? 0 : left < 0x7fffff00L ? left : 0x7fffff00L;
         const __amdgpu_buffer_rsrc_t rsrc = mfma::make_rsrc(base, (unsigned)reach);
-        const int v = k0 + BK <= k_end || k0 + kk[j] < k_end ? off[j] : mfma::kOutOfRange;
+        const int v = WHOLE || k0 + kk[j] < k_end ? off[j] : mfma::kOutOfRange;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (mfma::lds_void_t *)(stage + (wave * kLoads + j) * 1024), 16, v, 0, 0, 0);
     }
     __device__ __forceinline__ void next() {
@@ -201,8 +207,12 @@ template <class C> struct Frags {
 //
 // One barrier per slice, before its last step: by then every wavefront holds the slice's last fragments in registers
 // and its own part of the next slice has landed, so behind the barrier the next slice may be read (its first fragments
-// are fetched under the last step's MFMAs) and the slice's own stage refilled.  The matrix pipe never waits at a slice
-// boundary.
+// are fetched under the last step's MFMAs) and the slice's own stages refilled.  The matrix pipe never waits at a slice
+// boundary for LDS.
+//
+// A load issued behind the barrier has one slice's time to arrive, and if all of a slice's loads are issued there the
+// last of them comes too late: 64 KiB per CU in one burst.  With one more stage for A, A's loads are a slice further
+// ahead and go out during the slice's other steps: what is behind the barrier is B's half.
 template <class C, Layout LA, Layout LB>
 __device__ __forceinline__ void tile_product(const Shape &s, int m, int k_all, int m0, int n0, int k_begin, int k_end,
                                              char *__restrict__ lds, v16f (&acc)[C::TM][C::TN]) {
@@ -224,63 +234,85 @@ __device__ __forceinline__ void tile_product(const Shape &s, int m, int k_all, i
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
 
     const int nk = (k_end - k_begin + C::BK - 1) / C::BK;
-    auto issue = [&](char *__restrict__ stage, int j) {
-        if (j < C::kALoads) la.issue(stage, j, wave);
-        else lb.issue(stage + C::kABytes, j - C::kALoads, wave);
-    };
     // (slices past the end are loaded too, as zeros: the count of pending loads is then the same everywhere)
 #pragma unroll
-    for (int st = 0; st < C::STAGES; ++st) {
+    for (int st = 0; st < C::SB; ++st) {
 #pragma unroll
-        for (int j = 0; j < C::kLoads; ++j) issue(lds + st * C::kStageBytes, j);
+        for (int j = 0; j < C::kALoads; ++j) la.template issue<false>(lds + st * C::kABytes, j, wave);
+#pragma unroll
+        for (int j = 0; j < C::kBLoads; ++j) lb.template issue<false>(lds + C::kBBase + st * C::kBBytes, j, wave);
         la.next();
         lb.next();
     }
     Frags<C> f[2];
     constexpr int kReads = C::TM * decltype(ra)::kPieces + C::TN * decltype(rb)::kPieces;
-    auto read = [&](Frags<C> &to, const char *__restrict__ stage, int step, int q) {
+    auto read = [&](Frags<C> &to, const char *__restrict__ a, const char *__restrict__ b, int step, int q) {
         constexpr int kA = C::TM * decltype(ra)::kPieces;
-        if (q < kA) ra.piece(to.a[q / decltype(ra)::kPieces], stage, step, q / decltype(ra)::kPieces, q % decltype(ra)::kPieces);
+        if (q < kA) ra.piece(to.a[q / decltype(ra)::kPieces], a, step, q / decltype(ra)::kPieces, q % decltype(ra)::kPieces);
         else {
             const int t = q - kA;
-            rb.piece(to.b[t / decltype(rb)::kPieces], stage + C::kABytes, step, t / decltype(rb)::kPieces,
-                     t % decltype(rb)::kPieces);
+            rb.piece(to.b[t / decltype(rb)::kPieces], b, step, t / decltype(rb)::kPieces, t % decltype(rb)::kPieces);
         }
     };
-    ring_sync<(C::STAGES - 1) * C::kLoads>();
+    ring_sync<(C::SB - 1) * C::kLoads>();
 #pragma unroll
-    for (int q = 0; q < kReads; ++q) read(f[0], lds, 0, q);
-    int rd = 0;
+    for (int q = 0; q < kReads; ++q) read(f[0], lds, lds + C::kBBase, 0, q);
     constexpr int kMfmas = C::TM * C::TN;
-    for (int kt = 0; kt < nk; ++kt) {
-        const int nx = rd + 1 == C::STAGES ? 0 : rd + 1;
-        char *__restrict__ cur = lds + rd * C::kStageBytes;
-        const char *__restrict__ nxt = lds + nx * C::kStageBytes;
+    // a, b: the slice's stages; an, bn: the next slice's; ap: the previous slice's stage of A (to be refilled here
+    // when A runs ahead; this slice's otherwise)
+    auto slice = [&]<bool WHOLE>(char *__restrict__ a, char *__restrict__ b, const char *__restrict__ an,
+                                 const char *__restrict__ bn, char *__restrict__ ap) {
 #pragma unroll
         for (int step = 0; step < C::kSteps; ++step) {
             const bool last = step + 1 == C::kSteps;
             const Frags<C> &now = f[step & 1];
             Frags<C> &then = f[(step + 1) & 1];
-            if (last) ring_sync<(C::STAGES - 2) * C::kLoads>();
+            if (last) ring_sync<C::kPending>();
 #pragma unroll
             for (int i = 0; i < kMfmas; ++i) {
-                const int tm = i / C::TN, tn = i % C::TN;
+                const int tm = i / C::TN, tn = (tm & 1) ? C::TN - 1 - i % C::TN : i % C::TN;
                 mfma_acc(acc[tm][tn], now.b[tn], now.a[tm]);
-                // the next step's fragments in the first half of the step, the loads of a later slice behind the barrier
+                // the next step's fragments in the first half of the step, loads in the second half or behind the barrier
 #pragma unroll
                 for (int q = 0; q < kReads; ++q)
-                    if (q * ((kMfmas + 1) / 2) / kReads == i) read(then, last ? nxt : cur, last ? 0 : step + 1, q);
+                    if (q * ((kMfmas + 1) / 2) / kReads == i) read(then, last ? an : a, last ? bn : b, last ? 0 : step + 1, q);
+                constexpr int kLate = C::kEarlyA ? C::kBLoads : C::kLoads;
                 if (last) {
 #pragma unroll
-                    for (int j = 0; j < C::kLoads; ++j)
-                        if (j * kMfmas / C::kLoads == i) issue(cur, j);
+                    for (int j = 0; j < kLate; ++j)
+                        if (j * kMfmas / kLate == i) {
+                            if (C::kEarlyA) lb.template issue<WHOLE>(b, j, wave);
+                            else if (j < C::kALoads) la.template issue<WHOLE>(a, j, wave);
+                            else lb.template issue<WHOLE>(b, j - C::kALoads, wave);
+                        }
+                } else if (C::kEarlyA) {
+                    constexpr int kSlots = (C::kSteps - 1) * kMfmas;
+#pragma unroll
+                    for (int j = 0; j < C::kALoads; ++j)
+                        if ((2 * j + 1) * kSlots / (2 * C::kALoads) == step * kMfmas + i) la.template issue<WHOLE>(ap, j, wave);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         la.next();
         lb.next();
-        rd = nx;
+    };
+    // Every vector instruction between the MFMAs costs matrix cycles.  While the slices being loaded lie inside the
+    // contraction there are none: whole rounds of the rings, unrolled, so that every LDS address is a lane's constant.
+    const int whole = (k_end - k_begin) / C::BK - C::SB;   // slices whose successors in the rings are whole
+    int kt = 0;
+    for (; kt + C::kRound <= whole; kt += C::kRound) {
+#pragma unroll
+        for (int st = 0; st < C::kRound; ++st)
+            slice.template operator()<true>(lds + st % C::SA * C::kABytes, lds + C::kBBase + st % C::SB * C::kBBytes,
+                                            lds + (st + 1) % C::SA * C::kABytes, lds + C::kBBase + (st + 1) % C::SB * C::kBBytes,
+                                            lds + (st + C::SA - 1) % C::SA * C::kABytes);
+    }
+    for (int sa = 0, sb = 0; kt < nk; ++kt) {
+        const int na = sa + 1 == C::SA ? 0 : sa + 1, nb = sb + 1 == C::SB ? 0 : sb + 1, pa = sa ? sa - 1 : C::SA - 1;
+        slice.template operator()<false>(lds + sa * C::kABytes, lds + C::kBBase + sb * C::kBBytes, lds + na * C::kABytes,
+                                         lds + C::kBBase + nb * C::kBBytes, lds + pa * C::kABytes);
+        sa = na, sb = nb;
     }
     mfma::wait_vmcnt<0>();   // the trailing loads of zeros still target this workgroup's LDS
     acc_settle(acc);
@@ -327,53 +359,85 @@ __device__ __forceinline__ void unpack_block(const v4u (&in)[2], float (&x)[16])
         }
 }
 
-// A row's 32-column block at column `col` to (from) memory; vec: rows start on 16-byte boundaries.
-// Every lane of the wavefront calls these; `ok` says whether its row exists.
+// A row's 32-column block at column `col` to (from) memory; vec: rows start on 16-byte boundaries.  Every lane of the
+// wavefront calls these; `ok` says whether its row exists.  WHOLE: it does, with all its columns and vec (the path
+// without control flow: a branch per row makes the compiler wait for every store before it).
+template <bool WHOLE>
 __device__ __forceinline__ void store_block(uint16_t *row, bool ok, int col, int n, bool vec, int h, const float (&x)[16]) {
     v4u out[2];
     pack_block(x, out);
-    if (!ok) return;
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int c = col + 16 * q + 8 * h;
-        if (vec && c + 8 <= n) {
-            *reinterpret_cast<v4u *>(row + c) = out[q];
-        } else {
+        for (int q = 0; q < 2; ++q) *reinterpret_cast<v4u *>(row + col + 16 * q + 8 * h) = out[q];
+    } else {
+        if (!ok) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e < n) row[c + e] = (uint16_t)(out[q][e / 2] >> (16 * (e & 1)));
+        for (int q = 0; q < 2; ++q) {
+            const int c = col + 16 * q + 8 * h;
+            if (vec && c + 8 <= n) {
+                *reinterpret_cast<v4u *>(row + c) = out[q];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < n) row[c + e] = (uint16_t)(out[q][e / 2] >> (16 * (e & 1)));
+            }
         }
     }
 }
-__device__ __forceinline__ void load_block(const uint16_t *row, bool ok, int col, int n, bool vec, int h, float (&x)[16]) {
-    v4u in[2];
+template <bool WHOLE>
+__device__ __forceinline__ void load_block(const uint16_t *row, bool ok, int col, int n, bool vec, int h, v4u (&in)[2]) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int c = col + 16 * q + 8 * h;
-        in[q] = v4u{0, 0, 0, 0};
-        if (!ok) continue;
-        if (vec && c + 8 <= n) {
+        if constexpr (WHOLE) {
             in[q] = *reinterpret_cast<const v4u *>(row + c);
         } else {
+            in[q] = v4u{0, 0, 0, 0};
+            if (!ok) continue;
+            if (vec && c + 8 <= n) {
+                in[q] = *reinterpret_cast<const v4u *>(row + c);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e < n) in[q][e / 2] |= (unsigned)row[c + e] << (16 * (e & 1));
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < n) in[q][e / 2] |= (unsigned)row[c + e] << (16 * (e & 1));
+            }
         }
     }
-    unpack_block(in, x);
+}
+
+// The sixteen values a lane needs of a row vector (bias) for its part of the block at column `col`, as loaded: two a
+// dword.  WHOLE: all columns exist and the vector lies on an 8-byte boundary.
+template <bool WHOLE>
+__device__ __forceinline__ void load_columns(const uint16_t *v, int col, int n, int h, v2u (&out)[4]) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int c = col + 8 * g + 4 * h;
+        if constexpr (WHOLE) {
+            out[g] = *reinterpret_cast<const v2u *>(v + c);
+        } else {
+            out[g] = v2u{0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < n) out[g][e / 2] |= (unsigned)v[c + e] << (16 * (e & 1));
+        }
+    }
+}
+__device__ __forceinline__ float column_value(const v2u (&c)[4], int v) {
+    const unsigned d = c[v / 4][(v % 4) / 2];
+    return __builtin_bit_cast(float, v & 1 ? d & 0xffff0000u : d << 16);
 }
 
 #endif  // __HIP_DEVICE_COMPILE__
 
 // A bf16 matrix of the product, rows 16-byte aligned or not.
 struct StoreBf16 {
+    static constexpr bool kHeavy = false, kTall = false;
     uint16_t *out;
     long ld;
     bool vec;
 #if __HIP_DEVICE_COMPILE__
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
+    template <bool WHOLE, int TM, int TN>
+    __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
@@ -383,9 +447,15 @@ struct StoreBf16 {
                 float x[16];
 #pragma unroll
                 for (int v = 0; v < 16; ++v) x[v] = acc[tm][tn][v];
-                store_block(out + row * ld, row < m, col0 + tn * 32, n, vec, h, x);
+                store_block<WHOLE>(out + row * ld, row < m, col0 + tn * 32, n, vec, h, x);
             }
         }
+    }
+    template <int TM, int TN>
+    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
+                                               int) const {
+        if (vec && row0 + 32 * TM <= m && col0 + 32 * TN <= n) store<true>(acc, row0, col0, m, n, lane);
+        else store<false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
@@ -427,6 +497,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_bf16(Shape s, Ep ep) {
 
 // fp32 partial sums of split blockIdx.y (or the whole product when there is one): out[split][m][n], ld = n
 struct StorePartial {
+    static constexpr bool kHeavy = false, kTall = false;
     float *out;
     long split_stride;   // elements between the splits' matrices
     long ld;
@@ -470,7 +541,7 @@ template <class C, Layout LA, Layout LB, class Ep>
 int launch_gemm_bf16(const Shape &s, int splits, const Ep &ep, const char *who) {
     const long tiles = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN);
     if (tiles > 0x7fffffffL || splits > 65535) return fail(SWC_HIP_EINVAL, "%s: too many tiles", who);
-    note_kernel("gemm_bf16<%dx%d,%d,%d,%s%s> x%d", C::BM, C::BN, C::BK, C::STAGES, LA == kAlongK ? "k" : "m",
+    note_kernel("gemm_bf16<%dx%d,%d,%d,%s%s> x%d", C::BM, C::BN, C::SA, C::SB, LA == kAlongK ? "k" : "m",
                 LB == kAlongK ? "k" : "n", splits);
     auto kern = gemm_bf16<C, LA, LB, Ep>;
     static bool attr_set = false;

@@ -6,12 +6,14 @@
 namespace swc_hip {
 namespace mfma16 {
 
-using Big = Cfg<4, 2, 2, 4, 64, 2>;      // 256 x 256, eight wavefronts, one workgroup per CU
-using Mid = Cfg<2, 2, 2, 2, 64, 2>;      // 128 x 128, four wavefronts, two workgroups per CU
-using Low = Cfg<1, 2, 2, 2, 64, 3>;      // 64 x 128
-using Thin = Cfg<1, 1, 1, 4, 64, 4>;     // 32 x 128: few rows, the other operand streams
+using Big = Cfg<4, 2, 2, 4, 64, 3, 2>;      // 256 x 256, eight wavefronts, one workgroup per CU
+using Mid = Cfg<2, 2, 2, 2, 64, 3, 2>;      // 128 x 128, four wavefronts, two workgroups per CU
+using Low = Cfg<1, 2, 2, 2, 64, 3, 3>;      // 64 x 128
+using Thin = Cfg<1, 1, 1, 4, 64, 4, 4>;     // 32 x 128: few rows, the other operand streams
 
-enum Kind { kBig, kMid, kLow, kThin };
+using Deep = Cfg<4, 4, 2, 2, 64, 3, 2>;  // 256 x 256, four wavefronts of 128 x 128: a third less LDS traffic, a longer end
+
+enum Kind { kBig, kDeep, kMid, kLow, kThin };
 struct Plan {
     Kind kind;
     int splits, k_per_split;
@@ -29,7 +31,7 @@ inline Plan plan_product(int m, int n, int k) {
     int per_cu;
     if (m <= 32) p.kind = kThin, have = tiles(32, 128), per_cu = 2;
     else if (m <= 64) p.kind = kLow, have = tiles(64, 128), per_cu = 2;
-    else if (tiles(256, 256) * 4 >= 3L * cus) p.kind = kBig, have = tiles(256, 256), per_cu = 1;
+    else if (tiles(256, 256) * 4 >= 3L * cus) p.kind = k >= 6144 ? kDeep : kBig, have = tiles(256, 256), per_cu = 1;
     else p.kind = kMid, have = tiles(128, 128), per_cu = 2;
     // too few tiles: ranges of the contraction, at least four slices each
     const int slices = (k + 63) / 64;
@@ -46,16 +48,20 @@ inline Plan plan_product(int m, int n, int k) {
     return p;
 }
 
+// The epilogues with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
+// wavefront per SIMD has nothing beside it while they run; those with kTall exist for the large and middle tiles only.
 template <Layout LA, Layout LB, class Ep>
 int run_product(const Plan &p, const Shape &s, const Ep &ep, const char *who) {
     Shape t = s;
     t.k_per_split = p.k_per_split;
-    switch (p.kind) {
-    case kBig: return launch_gemm_bf16<Big, LA, LB>(t, p.splits, ep, who);
-    case kMid: return launch_gemm_bf16<Mid, LA, LB>(t, p.splits, ep, who);
-    case kLow: return launch_gemm_bf16<Low, LA, LB>(t, p.splits, ep, who);
-    default: return launch_gemm_bf16<Thin, LA, LB>(t, p.splits, ep, who);
+    if constexpr (!Ep::kHeavy)
+        if (p.kind == kDeep) return launch_gemm_bf16<Deep, LA, LB>(t, p.splits, ep, who);
+    if constexpr (!Ep::kTall) {
+        if (p.kind == kLow) return launch_gemm_bf16<Low, LA, LB>(t, p.splits, ep, who);
+        if (p.kind == kThin) return launch_gemm_bf16<Thin, LA, LB>(t, p.splits, ep, who);
     }
+    if (p.kind == kMid) return launch_gemm_bf16<Mid, LA, LB>(t, p.splits, ep, who);
+    return launch_gemm_bf16<Big, LA, LB>(t, p.splits, ep, who);
 }
 
 inline bool aligned_rows(const void *p, long ld) { return aligned16(p) && ld % 8 == 0; }
