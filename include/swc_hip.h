@@ -547,8 +547,8 @@ int swc_hip_adamw_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, 
  *     mom = momScale[b] * e4m3(mom8[i])       sqrt(var) = varScale[b] * e4m3(var8[i])
  * (e4m3: 8-bit floats of 4 exponent and 3 mantissa bits, bias 7, largest value
  * 448, no infinities).  A step decodes both, updates as above in fp32 and encodes
- * them again with scale = (largest finite magnitude of the block) / 448: mom to
- * the nearest value, ties to even; sqrt(var) up or down at random with the
+ * them again with scale = (largest finite magnitude of the block) * (1/448 as an
+ * fp32): mom / scale, as an fp32, to the nearest value, ties to even; sqrt(var) up or down at random with the
  * probabilities that keep its expectation (a variance decays by less per step
  * than half the distance of two values, and would never move if it were rounded
  * to the nearest), but a positive one never to zero.  The random number of

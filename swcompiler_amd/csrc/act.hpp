@@ -76,6 +76,8 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_slope(float z
 }
 #endif
 
+inline bool known_act(int act) { return act >= SWC_HIP_ACT_NONE && act <= SWC_HIP_ACT_SILU; }
+
 // Calls f with the activation as a compile-time constant.
 template <class F> int with_act(int act, F f) {
     switch (act) {

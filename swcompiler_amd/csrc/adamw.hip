@@ -7,6 +7,8 @@
 // bisecting the running count of chunks (an entry per tensor, in scalar registers).
 #include "common.hpp"
 
+#include <cmath>
+
 using namespace swc_hip;
 
 namespace {
@@ -28,12 +30,12 @@ struct Step {
     float lr, beta1, beta2, rest1, rest2, eps, decay;   // rest: 1 - beta, from doubles
 };
 
-// 1 - beta^t in double: the difference cancels at the first steps of a beta near 1.
-__global__ void adamw_advance(Header *state, double beta1, double beta2) {
+// 1 - beta^t = -expm1(t log beta) in double: the difference of a beta near 1 cancels at the first steps.
+__global__ void adamw_advance(Header *state, double log1, double log2) {
     const int t = state->steps + 1;
     state->steps = t;
-    state->c1 = (float)(1.0 / (1.0 - pow(beta1, (double)t)));
-    state->c2 = (float)(1.0 / (1.0 - pow(beta2, (double)t)));
+    state->c1 = (float)(-1.0 / expm1(t * log1));
+    state->c2 = (float)(-1.0 / expm1(t * log2));
 }
 
 struct Tensor {
@@ -45,14 +47,15 @@ struct Tensor {
 };
 struct Tensor8 : Tensor {
     float *mom_scale, *var_scale;
+    bool aligned;   // every pointer on the boundary of four of its elements
 };
-// 4 KiB of kernel arguments: 56 tensors with the 8-bit states' scales, 72 without
+// (the tables fill the 4 KiB that kernel arguments may take)
 template <class T, int N> struct Table {
     T t[N];
     unsigned first[N + 1];   // first chunk of each tensor
     int count, number0;      // number0: the first tensor's number in the call
 };
-constexpr int kTensors = 64, kTensors8 = 48;
+constexpr int kTensors = 64, kTensors8 = 44;
 static_assert(sizeof(Table<Tensor, kTensors>) + sizeof(Step) <= 4000 && sizeof(Table<Tensor8, kTensors8>) + sizeof(Step) <= 4000, "");
 
 template <class T, int N> __device__ __forceinline__ int tensor_of(const Table<T, N> &tab, unsigned chunk) {
@@ -134,6 +137,7 @@ __device__ __forceinline__ unsigned random20(unsigned x) {
 }
 
 constexpr float kLargest = 448.f;        // of e4m3
+constexpr float kPer = 1.f / 448.f;
 constexpr float kTiny = 0x1p-100f;       // a block whose largest magnitude is below this is held as zeros
 constexpr unsigned kNan8 = 0x7f;
 
@@ -144,19 +148,15 @@ __device__ __forceinline__ float from_e4m3(unsigned byte) {
     return 0.f;
 #endif
 }
-// The codes are settled in 64 bits (a float by the reciprocal of a float: nothing that fp32 would round across a border).
-// To the nearest value, ties to even; |y| <= 448.  The conversion instruction rounds an fp32: y goes there cut to 20
-// mantissa bits with the last one set if anything was cut off, which keeps it on its side of every border.
-__device__ __forceinline__ unsigned to_e4m3(double y) {
+// An fp32 quotient of at most 448 to the nearest value, ties to even.
+__device__ __forceinline__ unsigned to_e4m3(float y) {
 #if __HIP_DEVICE_COMPILE__
-    const unsigned long long b = __builtin_bit_cast(unsigned long long, y);
-    const float x = (float)__builtin_bit_cast(double, (b & ~0xffffffffull) | ((b & 0xffffffffull) ? 1ull << 32 : 0));
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu;
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xffu;
 #else
     return 0;
 #endif
 }
-// 0 <= y <= 448 up or down by 20 random bits: with the exponent E of y (at least that of the least normal value) the
+// 0 <= y <= 448 up or down by 20 random bits, which side settled in 64 bits: with the exponent E of y (at least that of the least normal value) the
 // values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is 8 (E + 7) + q - 8 — also
 // where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the subnormal values).
 __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
@@ -167,53 +167,97 @@ __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
     return (unsigned)(8 * (e + 7) + q - 8);
 }
 
-// A wavefront owns a block of 256 elements, lane l its elements l, l + 64, l + 128, l + 192.
+// A wavefront owns a block of 256 elements, a lane four of them: consecutive ones (FULL: the block is whole and every
+// tensor starts on the boundary of four of its elements), or one of every 64.
+template <class G, bool FULL>
+__device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int lane, unsigned number, const Scalars &k, const Step &s) {
+    uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);
+    const G *dw = static_cast<const G *>(t.dw);
+    const float ms = t.mom_scale[block], vs = t.var_scale[block];
+    const size_t i0 = block * kBlock + (FULL ? lane * 4 : lane);
+    constexpr int kStep = FULL ? 1 : 64;
+    float w[4], g[4], m[4], r[4], top = 0.f, peak = 0.f;
+    unsigned mc[4], vc[4];
+    bool in[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) in[e] = FULL || i0 + e * kStep < t.size;
+    if constexpr (FULL) {
+        const float4 x = *reinterpret_cast<const float4 *>(t.w + i0);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        if constexpr (sizeof(G) == 4) {
+            const float4 y = *reinterpret_cast<const float4 *>(dw + i0);
+            g[0] = y.x, g[1] = y.y, g[2] = y.z, g[3] = y.w;
+        } else {
+            const uint2 y = *reinterpret_cast<const uint2 *>(dw + i0);
+            g[0] = __builtin_bit_cast(float, y.x << 16), g[1] = __builtin_bit_cast(float, y.x & 0xffff0000u);
+            g[2] = __builtin_bit_cast(float, y.y << 16), g[3] = __builtin_bit_cast(float, y.y & 0xffff0000u);
+        }
+        const unsigned a = *reinterpret_cast<const unsigned *>(mom8 + i0), b = *reinterpret_cast<const unsigned *>(var8 + i0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mc[e] = (a >> (8 * e)) & 0xffu, vc[e] = (b >> (8 * e)) & 0xffu;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const size_t i = i0 + e * kStep;
+            w[e] = in[e] ? t.w[i] : 0.f;
+            g[e] = in[e] ? grad_of(dw, i) : 0.f;
+            mc[e] = in[e] ? mom8[i] : 0u, vc[e] = in[e] ? var8[i] : 0u;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        m[e] = ms * from_e4m3(mc[e]);
+        const float root = vs * from_e4m3(vc[e]);
+        float v = root * root;
+        step_one(w[e], g[e], m[e], v, k, s);
+        r[e] = sqrtf(v);
+        if (in[e] && fabsf(m[e]) < __builtin_inff()) top = fmaxf(top, fabsf(m[e]));
+        if (in[e] && r[e] < __builtin_inff()) peak = fmaxf(peak, r[e]);
+    }
+    top = wave_max(top), peak = wave_max(peak);
+    const float mscale = top > kTiny ? top * kPer : 0.f, vscale = peak > kTiny ? peak * kPer : 0.f;
+    const double im = mscale > 0.f ? 1.0 / (double)mscale : 0.0, iv = vscale > 0.f ? 1.0 / (double)vscale : 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const size_t i = i0 + e * kStep;
+        // (the quotients by a reciprocal in 64 bits: the fp32 quotient of mom correctly rounded)
+        const float x = fminf(fmaxf((float)(m[e] * im), -kLargest), kLargest);
+        const double y = fmin(r[e] * iv, (double)kLargest);
+        mc[e] = fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8;
+        vc[e] = r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)i + number)) : kNan8;
+    }
+    if constexpr (FULL) {
+        *reinterpret_cast<float4 *>(t.w + i0) = make_float4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<unsigned *>(mom8 + i0) = mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24;
+        *reinterpret_cast<unsigned *>(var8 + i0) = vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24;
+        if (t.copy)
+            *reinterpret_cast<uint2 *>(t.copy + i0) = make_uint2(to_bf16(w[0]) | (unsigned)to_bf16(w[1]) << 16,
+                                                                 to_bf16(w[2]) | (unsigned)to_bf16(w[3]) << 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const size_t i = i0 + e * kStep;
+            if (!in[e]) continue;
+            t.w[i] = w[e], mom8[i] = (uint8_t)mc[e], var8[i] = (uint8_t)vc[e];
+            if (t.copy) t.copy[i] = to_bf16(w[e]);
+        }
+    }
+    if (lane == 0) {
+        t.mom_scale[block] = mscale;
+        t.var_scale[block] = vscale;
+    }
+}
+
 template <class G>
 __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTensors8> tab, Step s) {
     const int which = tensor_of(tab, blockIdx.x);
     const Tensor8 &t = tab.t[which];
     const Scalars k = scalars(s);
     const size_t block = (size_t)(blockIdx.x - tab.first[which]) * 4 + (threadIdx.x >> 6);
-    const size_t i0 = block * kBlock + (threadIdx.x & 63);
     if (block * kBlock >= t.size) return;   // whole wavefronts leave together
-    uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);
-    const G *dw = static_cast<const G *>(t.dw);
-    const float ms = t.mom_scale[block], vs = t.var_scale[block];
-    float m[4], r[4], top = 0.f, peak = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const size_t i = i0 + e * 64;
-        m[e] = 0.f, r[e] = 0.f;
-        if (i < t.size) {
-            float w = t.w[i];
-            m[e] = ms * from_e4m3(mom8[i]);
-            const float root = vs * from_e4m3(var8[i]);
-            float v = root * root;
-            step_one(w, grad_of(dw, i), m[e], v, k, s);
-            r[e] = sqrtf(v);
-            t.w[i] = w;
-            if (t.copy) t.copy[i] = to_bf16(w);
-            if (fabsf(m[e]) < __builtin_inff()) top = fmaxf(top, fabsf(m[e]));
-            if (r[e] < __builtin_inff()) peak = fmaxf(peak, r[e]);
-        }
-    }
-    top = wave_max(top), peak = wave_max(peak);
-    const float mscale = top > kTiny ? top / kLargest : 0.f, vscale = peak > kTiny ? peak / kLargest : 0.f;
-    const double im = mscale > 0.f ? 1.0 / (double)mscale : 0.0, iv = vscale > 0.f ? 1.0 / (double)vscale : 0.0;
     const unsigned number = (unsigned)(tab.number0 + which) * 0x9E3779B9u + (unsigned)s.state->steps * 0x85EBCA6Bu;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const size_t i = i0 + e * 64;
-        if (i < t.size) {
-            const double x = fmin(fmax(m[e] * im, -(double)kLargest), (double)kLargest), y = fmin(r[e] * iv, (double)kLargest);
-            mom8[i] = (uint8_t)(fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8);
-            var8[i] = (uint8_t)(r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)i + number)) : kNan8);
-        }
-    }
-    if ((threadIdx.x & 63) == 0) {
-        t.mom_scale[block] = mscale;
-        t.var_scale[block] = vscale;
-    }
+    if (t.aligned && (block + 1) * kBlock <= t.size) adamw8_block<G, true>(t, block, threadIdx.x & 63, number, k, s);
+    else adamw8_block<G, false>(t, block, threadIdx.x & 63, number, k, s);
 }
 
 int check(const char *who, int count, const void *const *w, const void *const *dw, const void *const *mom,
@@ -289,6 +333,8 @@ int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint
         [&](Tensor8 &t, int i) {
             t.w = w[i], t.dw = dw[i], t.mom = mom8[i], t.var = var8[i], t.copy = copies ? copies[i] : nullptr;
             t.size = sizes[i], t.mom_scale = mom_scale[i], t.var_scale = var_scale[i];
+            auto on = [](const void *p, size_t step) { return reinterpret_cast<uintptr_t>(p) % step == 0; };
+            t.aligned = on(t.w, 16) && on(t.dw, 4 * sizeof(G)) && on(t.mom, 4) && on(t.var, 4) && on(t.copy, 8);
         },
         [&](const Table<Tensor8, kTensors8> &tab, unsigned chunks) {
             adamw8_tensors<G><<<chunks, kThreads, 0, stream()>>>(tab, s);
@@ -303,7 +349,8 @@ int swc_hip_adamwAdvance(void *state, double beta1, double beta2) {
     SWC_ARG(state);
     SWC_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1);
     SWC_REQUIRE_INIT();
-    adamw_advance<<<1, 1, 0, stream()>>>(static_cast<Header *>(state), beta1, beta2);
+    // (log 0 is -infinity, and expm1 of that -1: the correction of beta 0 is 1)
+    adamw_advance<<<1, 1, 0, stream()>>>(static_cast<Header *>(state), log(beta1), log(beta2));
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }

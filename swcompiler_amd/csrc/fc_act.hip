@@ -15,7 +15,7 @@ using namespace swc_hip::mfma16;
 namespace {
 
 template <int ACT> struct FcEpilogue {
-    static constexpr bool kHeavy = true, kTall = true;
+    static constexpr bool kHeavy = true, kThinToo = false;
     const uint16_t *bias, *residual;
     uint16_t *preact, *c;
     long ldr, ldp, ldc;
@@ -60,133 +60,116 @@ template <int ACT> struct FcEpilogue {
 };
 
 // The end of a layer from fp32 sums: `parts` matrices of m x n to be added in order, then bias, activation, residual.
-// (part may be c itself: fp32, one part)
-template <class T, int ACT>
+// (part may be c itself: fp32, one part.)  Four columns of a row a thread; VEC: rows of sums on 16-byte boundaries.
+template <class T, int ACT, bool VEC>
 __global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long ldpart, long part_stride, const T *bias,
                                                  const T *residual, long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
 #if __HIP_DEVICE_COMPILE__
-    const size_t total = (size_t)m * n, step = (size_t)gridDim.x * 256;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        const long r = i / n, j = i - r * n;
-        float z = 0.f;
-        for (int p = 0; p < parts; ++p) z += part[p * part_stride + r * ldpart + j];
-        if (bias) z += load_any(bias + j);
-        if (preact) store_any(preact + r * ldp + j, z);
-        z = act_value<ACT, sizeof(T) == 2>(z);
-        if (residual) z += load_any(residual + r * ldr + j);
-        store_any(c + r * ldc + j, z);
+    const int j = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    if (j >= n) return;
+    float b[4] = {};
+    if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = j + e < n ? load_any(bias + j + e) : 0.f;
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < m; r += gridDim.y * 4) {
+        float z[4] = {}, x[4] = {};
+        const float *p = part + r * ldpart + j;
+        if (residual)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = j + e < n ? load_any(residual + r * ldr + j + e) : 0.f;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) {
+            if (VEC) {
+                const float4 d = *reinterpret_cast<const float4 *>(p + i * part_stride);
+                z[0] += d.x, z[1] += d.y, z[2] += d.z, z[3] += d.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] += j + e < n ? p[i * part_stride + e] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (j + e >= n) continue;
+            z[e] += b[e];
+            if (preact) store_any(preact + r * ldp + j + e, z[e]);
+            store_any(c + r * ldc + j + e, act_value<ACT, sizeof(T) == 2>(z[e]) + x[e]);
+        }
     }
 #endif
 }
 template <class T>
 int launch_finish(int act, const float *part, int parts, long ldpart, long part_stride, const T *bias, const T *residual, long ldr,
                   T *preact, long ldp, T *c, long ldc, int m, int n) {
+    const unsigned rows = ceil_div(m, 4);
+    const dim3 grid(ceil_div(n, 256), rows > 16384 ? 16384 : rows);
+    const bool vec = aligned16(part) && ldpart % 4 == 0 && part_stride % 4 == 0 && n % 4 == 0;
     return with_act(act, [&]<int ACT>() {
-        fc_finish<T, ACT><<<grid_of((size_t)m * n), 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact,
-                                                                        ldp, c, ldc, m, n);
+        if (vec) fc_finish<T, ACT, true><<<grid, 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact, ldp, c, ldc, m, n);
+        else fc_finish<T, ACT, false><<<grid, 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact, ldp, c, ldc, m, n);
         SWC_LAUNCH_CHECK();
         return (int)SWC_HIP_OK;
     });
 }
 
-// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of kSumRows rows' column sums of the unrounded
-// values.  32 threads side by side hold eight columns each, eight rows at a time; VEC: 16 bytes of a row at once.
-constexpr int kSumRows = 64;
-template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int j, int n, float (&x)[8]) {
-    if constexpr (VEC && sizeof(T) == 2) {
-        const uint4 d = *reinterpret_cast<const uint4 *>(p + j);
-        const unsigned w[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-    } else if constexpr (VEC) {
-        const float4 a = *reinterpret_cast<const float4 *>(p + j), b = *reinterpret_cast<const float4 *>(p + j + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = j + e < n ? load_any(p + j + e) : 0.f;
-    }
+// Rows into a copy whose rows start on 16-byte boundaries, zeros behind their end and in the rows that do not exist:
+// 16 bytes a thread.  A source at any alignment is read in the two aligned 16-byte pieces that hold the thread's eight
+// values (each of them holds at least one that exists, so neither leaves the allocation's pages), shifted together.
+__device__ __forceinline__ uint4 eight_at(const uint16_t *p, int have) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint4 *q = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
+    const int shift = (int)(at & 15) * 8;
+    const uint4 lo = q[0], hi = shift / 16 + have > 8 ? q[1] : make_uint4(0, 0, 0, 0);
+    typedef unsigned __int128 u128;
+    const u128 l = (u128)(((uint64_t)lo.y << 32) | lo.x) | ((u128)(((uint64_t)lo.w << 32) | lo.z) << 64);
+    const u128 h = (u128)(((uint64_t)hi.y << 32) | hi.x) | ((u128)(((uint64_t)hi.w << 32) | hi.z) << 64);
+    u128 v = shift ? (l >> shift) | (h << (128 - shift)) : l;
+    if (have < 8) v &= ((u128)1 << (16 * have)) - 1;
+    const uint64_t a = (uint64_t)v, b = (uint64_t)(v >> 64);
+    return make_uint4((unsigned)a, (unsigned)(a >> 32), (unsigned)b, (unsigned)(b >> 32));
 }
-template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int j, int n, const float (&x)[8]) {
-#if __HIP_DEVICE_COMPILE__
-    if constexpr (VEC && sizeof(T) == 2) {
-        *reinterpret_cast<uint4 *>(p + j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-    } else if constexpr (VEC) {
-        *reinterpret_cast<float4 *>(p + j) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(p + j + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (j + e < n) store_any(p + j + e, x[e]);
-    }
-#endif
-}
-
-template <class T, int ACT, bool VEC>
-__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums) {
-#if __HIP_DEVICE_COMPILE__
-    __shared__ float part[8][257];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int j = (blockIdx.x * 32 + tx) * 8;
-    const int r0 = blockIdx.y * kSumRows;
-    const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
-    float sum[8] = {};
-    if (j < (n > ld ? n : ld))
-#pragma unroll 2
-        for (int r = r0 + ty; r < r1; r += 8) {
-            float g[8];
-            load8<T, VEC>(dc + r * ldc, j, n, g);
-            if constexpr (ACT != SWC_HIP_ACT_NONE) {
-                float y[8];
-                load8<T, VEC>(z + r * ldz, j, n, y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, sizeof(T) == 2>(y[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += j + e < n ? g[e] : 0.f;
-            if (dz) store8<T, VEC>(dz + r * ld, j, (int)ld, g);
-        }
-    if (!sums) return;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
-    __syncthreads();
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    float s = 0.f;
-#pragma unroll
-    for (int y = 0; y < 8; ++y) s += part[y][threadIdx.x];
-    if (col < n) sums[(size_t)blockIdx.y * n + col] = s;
-#endif
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index,
-                                                 const int *count) {
+__global__ __launch_bounds__(256) void copy_rows16(uint16_t *dst, long ld, const uint16_t *src, long lds, int rows, int cols,
+                                                   const int *index, const int *count) {
     const int have = count ? *count : rows;
+    const long j = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (j >= ld) return;
     for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        const bool ok = r < have;
-        const T *p = ok ? src + (index ? index[r] : r) * lds : src;
-        for (long j = (long)blockIdx.x * 256 + threadIdx.x; j < ld; j += (long)gridDim.x * 256)
-            dst[r * ld + j] = ok && j < cols ? p[j] : T(0);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < have && j < cols) v = eight_at(src + (index ? index[r] : r) * lds + j, cols - j < 8 ? (int)(cols - j) : 8);
+        *reinterpret_cast<uint4 *>(dst + r * ld + j) = v;
     }
 }
-template <class T>
-int launch_copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index, const int *count) {
-    if (!rows || !ld) return SWC_HIP_OK;
-    const unsigned x = ceil_div(ld, 256), y = rows < 32768 ? rows : 32768;
-    copy_rows<T><<<dim3(x > 64 ? 64 : x, y), 256, 0, stream()>>>(dst, ld, src, lds, rows, cols, index, count);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
+// fp32 (dst and ld as the product wants them: any): four values a thread where everything is aligned
+template <bool VEC>
+__global__ __launch_bounds__(256) void copy_rows32(float *dst, long ld, const float *src, long lds, int rows, int cols, const int *index,
+                                                   const int *count) {
+    const int have = count ? *count : rows;
+    const long j = ((long)blockIdx.x * 256 + threadIdx.x) * (VEC ? 4 : 1);
+    if (j >= ld) return;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float *p = src + (index && r < have ? index[r] : r) * lds + j;
+        if (VEC) *reinterpret_cast<float4 *>(dst + r * ld + j) = r < have ? *reinterpret_cast<const float4 *>(p) : make_float4(0, 0, 0, 0);
+        else dst[r * ld + j] = r < have && j < cols ? *p : 0.f;
+    }
 }
 
+// 32 columns and eight ranges of the parts a workgroup: a range's parts are added in order, then the ranges in order.
 __global__ __launch_bounds__(256) void add_parts(uint16_t *out_bf, float *out_f, const float *part, int parts, int n) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= n) return;
+    __shared__ float sums[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int j = blockIdx.x * 32 + tx;
+    const int each = (parts + 7) / 8, p0 = ty * each, p1 = p0 + each < parts ? p0 + each : parts;
     float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += part[(size_t)p * n + j];
+    if (j < n)
+#pragma unroll 4
+        for (int p = p0; p < p1; ++p) s += part[(size_t)p * n + j];
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty || j >= n) return;
+#pragma unroll
+    for (int y = 1; y < 8; ++y) s += sums[y][tx];
     if (out_bf) store_any(out_bf + j, s);
     if (out_f) out_f[j] = s;
 }
-
-bool known_act(int act) { return act >= SWC_HIP_ACT_NONE && act <= SWC_HIP_ACT_SILU; }
 
 template <class T>
 int check_forward(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb, int act, const T *residual,
@@ -205,7 +188,7 @@ int check_forward(const char *who, int m, int n, int k, const T *a, int lda, con
 }
 
 // Few rows, or a cut contraction: sums to the workspace, the end of the layer in fc_finish.
-bool partial_sums(const Plan &p) { return p.splits > 1 || p.kind == kLow || p.kind == kThin; }
+bool partial_sums(const Plan &p) { return p.splits > 1 || p.kind == kThin; }
 
 struct ForwardSpace {
     uint16_t *a, *b;
@@ -254,171 +237,31 @@ int forward_bf16(const char *who, int m, int n, int k, const uint16_t *a, long l
     return launch_finish<uint16_t>(act, w.part, p.splits, n, (long)m * n, bias, residual, ldr, preact, ldp, c, ldc, m, n);
 }
 
-template <class T>
-int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda, const T *b, int ldb,
-               const T *preact, int ldp, int act, const T *da, int ldda, const T *db, int lddb, const T *dbias) {
-    if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
-    if (!known_act(act)) return fail(SWC_HIP_EINVAL, "%s: unknown activation %d", who, act);
-    if (m && n && !dc) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
-    if (act != SWC_HIP_ACT_NONE && m && n && !preact) return fail(SWC_HIP_EINVAL, "%s: preact is needed for this activation", who);
-    if ((da && m && n && k && !b) || (db && m && n && k && !a)) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
-    if (lddc < n || (da && (ldda < k || ldb < n)) || (db && (lddb < n || lda < k)) || (act != SWC_HIP_ACT_NONE && ldp < n))
-        return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
-    const void *in[4] = {dc, a, b, preact};
-    for (const void *p : in)
-        if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
-    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd || lddc > kMaxLd))
-        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
-    return SWC_HIP_OK;
-}
-
-int sum_blocks(int m) { return (m + kSumRows - 1) / kSumRows; }
-
-template <class T>
-int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
-    if (!dz) ld = 0;
-    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m));
-    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
-    constexpr int kPer = 16 / sizeof(T);
-    const bool vec = n % 8 == 0 && aligned16(dc) && lddc % kPer == 0 && (act == SWC_HIP_ACT_NONE || (aligned16(z) && ldz % kPer == 0)) &&
-                     (!dz || (aligned16(dz) && ld % kPer == 0));
-    return with_act(act, [&]<int ACT>() {
-        if (vec) act_grad<T, ACT, true><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
-        else act_grad<T, ACT, false><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
-        SWC_LAUNCH_CHECK();
-        return (int)SWC_HIP_OK;
-    });
-}
-
-struct GradSpace {
-    uint16_t *dz, *a, *b;
-    float *part, *sums;
-    size_t bytes;
-};
-GradSpace grad_space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool pack_b, size_t partials, bool bias) {
-    Carver c{base};
-    GradSpace s{};
-    s.dz = own_dz ? c.take<uint16_t>((size_t)m * round8(n)) : nullptr;
-    s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
-    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
-    s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
-    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
-    s.bytes = c.used;
-    return s;
-}
-
-// one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
-template <Layout LA, Layout LB>
-int grad_product(const char *who, const Plan &p, const Shape &s, uint16_t *out, long ld, float *part) {
-    if (p.splits == 1) return run_product<LA, LB>(p, s, StoreBf16{out, ld, aligned_rows(out, ld)}, who);
-    if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
-    return launch_finish<uint16_t>(SWC_HIP_ACT_NONE, part, p.splits, s.n, (long)s.m * s.n, nullptr, nullptr, 0, nullptr, 0, out, ld, s.m,
-                                   s.n);
-}
-
-size_t max2(size_t a, size_t b) { return a > b ? a : b; }
-
-int grad_bf16(const char *who, int m, int n, int k, const uint16_t *dc, long lddc, const uint16_t *a, long lda,
-              const uint16_t *b, long ldb, const uint16_t *preact, long ldp, int act, uint16_t *da, long ldda, uint16_t *db,
-              long lddb, uint16_t *dbias) {
-    const Plan pa = plan_product(m, k, n), pb = plan_product(k, n, m);
-    // dZ is dC itself without an activation; a copy when its rows do not start on 16-byte boundaries, or when dA would
-    // read past the end of a row
-    const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || (da && n % 8));
-    const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || n % 8);
-    const size_t partials = max2(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
-    const size_t need = grad_space(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
-    GradSpace w{};
-    if (need) {
-        char *base = static_cast<char *>(workspace(need, who));
-        if (!base) return fail_code();
-        w = grad_space(base, m, n, k, own_dz, pack_a, pack_b, partials, dbias);
-    }
-    if (own_dz || dbias) {
-        if (int rc = launch_act_grad<uint16_t>(w.dz, round8(n), dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
-        if (dbias)
-            if (int rc = sum_parts(dbias, nullptr, w.sums, sum_blocks(m), n)) return rc;
-    }
-    const uint16_t *dz = own_dz ? w.dz : dc;
-    const long lddz = own_dz ? round8(n) : lddc;
-    if (pack_b) {
-        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = round8(n);
-    }
-    if (pack_a) {
-        if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, nullptr, nullptr)) return rc;
-        a = w.a, lda = round8(k);
-    }
-    if (da)
-        if (int rc = grad_product<kAlongK, kAlongK>(who, pa, Shape{dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
-    if (db)
-        if (int rc = grad_product<kAcross, kAcross>(who, pb, Shape{a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
-    return SWC_HIP_OK;
-}
-
-struct GradSpaceF {
-    float *dz, *at, *bt, *part, *sums;
-    size_t bytes;
-};
-GradSpaceF grad_space_f(char *base, int m, int n, int k, bool own_dz, bool da, bool db, size_t partials, bool bias) {
-    Carver c{base};
-    GradSpaceF s{};
-    s.dz = own_dz ? c.take<float>((size_t)m * n) : nullptr;
-    s.at = db ? c.take<float>((size_t)m * k) : nullptr;
-    s.bt = da ? c.take<float>((size_t)k * n) : nullptr;
-    s.part = c.take<float>(partials / sizeof(float) + 1);
-    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
-    s.bytes = c.used;
-    return s;
-}
-
-int grad_f32(const char *who, int m, int n, int k, const float *dc, int lddc, const float *a, int lda, const float *b, int ldb,
-             const float *preact, int ldp, int act, float *da, int ldda, float *db, int lddb, float *dbias) {
-    const bool own_dz = (da || db) && act != SWC_HIP_ACT_NONE;
-    const size_t partials = max2(da ? swc_hip_gemm_workspace_bytes(m, k, n) : 0, db ? swc_hip_gemm_workspace_bytes(k, n, m) : 0);
-    const size_t need = grad_space_f(nullptr, m, n, k, own_dz, da, db, partials, dbias).bytes;
-    char *base = static_cast<char *>(workspace(need, who));
-    if (!base) return fail_code();
-    const GradSpaceF w = grad_space_f(base, m, n, k, own_dz, da, db, partials, dbias);
-    if (own_dz || dbias) {
-        if (int rc = launch_act_grad<float>(w.dz, n, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
-        if (dbias)
-            if (int rc = sum_parts(nullptr, dbias, w.sums, sum_blocks(m), n)) return rc;
-    }
-    const float *dz = own_dz ? w.dz : dc;
-    const int lddz = own_dz ? n : lddc;
-    if (da) {
-        if (int rc = swc_hip_matrixTrans_f(k, n, b, ldb, w.bt, k)) return rc;
-        if (int rc = gemm_f32(who, m, k, n, dz, lddz, w.bt, k, nullptr, da, ldda, 0, w.part, partials)) return rc;
-    }
-    if (db) {
-        if (int rc = swc_hip_matrixTrans_f(m, k, a, lda, w.at, m)) return rc;
-        if (int rc = gemm_f32(who, k, n, m, w.at, m, dz, lddz, nullptr, db, lddb, 0, w.part, partials)) return rc;
-    }
-    return SWC_HIP_OK;
-}
-
-// what every form of the gradient call answers with when there is nothing to sum over
-template <class T>
-int grad_of_nothing(int m, int n, int k, T *da, int ldda, T *db, int lddb, T *dbias) {
-    if (int rc = zero_rows(da, ldda, m, k)) return rc;
-    if (int rc = zero_rows(db, lddb, k, n)) return rc;
-    return zero_rows(dbias, n, 1, n);
-}
-
 } // namespace
 
+int swc_hip::mfma16::join_parts(uint16_t *out, long ld, const float *part, int parts, int m, int n) {
+    return launch_finish<uint16_t>(SWC_HIP_ACT_NONE, part, parts, n, (long)m * n, nullptr, nullptr, 0, nullptr, 0, out, ld, m, n);
+}
 int swc_hip::mfma16::copy_rows_bf16(uint16_t *dst, long ld, const uint16_t *src, long lds, int rows, int cols, const int *index,
                                     const int *count) {
-    return launch_copy_rows(dst, ld, src, lds, rows, cols, index, count);
+    if (!rows || !ld) return SWC_HIP_OK;
+    copy_rows16<<<dim3(ceil_div(ld / 8, 256), rows < 32768 ? rows : 32768), 256, 0, stream()>>>(dst, ld, src, lds, rows, cols, index, count);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
 }
 int swc_hip::mfma16::copy_rows_f32(float *dst, long ld, const float *src, long lds, int rows, int cols, const int *index,
                                    const int *count) {
-    return launch_copy_rows(dst, ld, src, lds, rows, cols, index, count);
+    if (!rows || !ld) return SWC_HIP_OK;
+    const bool vec = aligned16(dst) && aligned16(src) && ld % 4 == 0 && lds % 4 == 0 && cols == ld;
+    const dim3 grid(ceil_div(vec ? ld / 4 : ld, 256), rows < 32768 ? rows : 32768);
+    if (vec) copy_rows32<true><<<grid, 256, 0, stream()>>>(dst, ld, src, lds, rows, cols, index, count);
+    else copy_rows32<false><<<grid, 256, 0, stream()>>>(dst, ld, src, lds, rows, cols, index, count);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
 }
 int swc_hip::mfma16::sum_parts(uint16_t *out_bf, float *out_f, const float *part, int parts, int n) {
     if (!n) return SWC_HIP_OK;
-    add_parts<<<ceil_div(n, 256), 256, 0, stream()>>>(out_bf, out_f, part, parts, n);
+    add_parts<<<ceil_div(n, 32), 256, 0, stream()>>>(out_bf, out_f, part, parts, n);
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
@@ -475,38 +318,6 @@ size_t swc_hip_matrixMatrixFCActAdd_workspace_bytes(int m, int n, int k, int bf)
     c.take<float>(swc_hip_gemm_workspace_bytes(m, n, k) / sizeof(float) + 1);
     c.take<float>((size_t)m * n);
     return c.used;
-}
-
-int swc_hip_matrixMatrixFCActAddGrad_f(int m, int n, int k, const float *cGrad, int ldcg, const float *a, int lda, const float *b,
-                                       int ldb, const float *preact, int ldp, int act, float *aGrad, int ldag, float *bGrad,
-                                       int ldbg, float *biasGrad) {
-    const char *who = "swc_hip_matrixMatrixFCActAddGrad_f";
-    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
-    SWC_REQUIRE_INIT();
-    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
-    if (k == 0) aGrad = bGrad = nullptr;
-    return grad_f32(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
-}
-
-int swc_hip_matrixMatrixFCActAddGrad_bf(int m, int n, int k, const swc_hip_bf16 *cGrad, int ldcg, const swc_hip_bf16 *a, int lda,
-                                        const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *preact, int ldp, int act,
-                                        swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad, int ldbg, swc_hip_bf16 *biasGrad) {
-    const char *who = "swc_hip_matrixMatrixFCActAddGrad_bf";
-    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
-    SWC_REQUIRE_INIT();
-    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
-    if (k == 0) aGrad = bGrad = nullptr;
-    return grad_bf16(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
-}
-
-size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int bf) {
-    if (!ready() || m <= 0 || n <= 0) return 0;
-    if (bf) {
-        const size_t partials = k > 0 ? max2(plan_product(m, k, n).partial_bytes(m, k), plan_product(k, n, m).partial_bytes(k, n)) : 0;
-        return grad_space(nullptr, m, n, k, true, true, true, partials, true).bytes;
-    }
-    const size_t partials = max2(swc_hip_gemm_workspace_bytes(m, k, n), swc_hip_gemm_workspace_bytes(k, n, m));
-    return grad_space_f(nullptr, m, n, k, true, true, true, partials, true).bytes;
 }
 
 } // extern "C"

@@ -1,0 +1,270 @@
+// The gradients of the fully connected layer with its activation (matrixMatrixFCActAddGrad_f/_bf).
+//
+//     dZ = dC act'(Z), dA = dZ B^T, dB = A^T dZ, dbias = column sums of dZ
+//
+// bf16: the two products on the core of gemm_bf16.hpp, no matrix transposed in memory; dZ is rounded to bf16 once, for
+// both.  fp32: the kernels of gemm.hip take row-major operands, so A and B are transposed into the workspace first.
+#include "act.hpp"
+#include "product_bf16.hpp"
+
+using namespace swc_hip;
+using namespace swc_hip::mfma16;
+
+namespace {
+
+// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of kSumRows rows' column sums of the unrounded
+// values.  32 threads side by side hold eight columns each, eight rows at a time; VEC: 16 bytes of a row at once.
+constexpr int kSumRows = 32;
+template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int j, int n, float (&x)[8]) {
+    if constexpr (VEC && sizeof(T) == 2) {
+        const uint4 d = *reinterpret_cast<const uint4 *>(p + j);
+        const unsigned w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else if constexpr (VEC) {
+        const float4 a = *reinterpret_cast<const float4 *>(p + j), b = *reinterpret_cast<const float4 *>(p + j + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = j + e < n ? load_any(p + j + e) : 0.f;
+    }
+}
+template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int j, int n, const float (&x)[8]) {
+#if __HIP_DEVICE_COMPILE__
+    if constexpr (VEC && sizeof(T) == 2) {
+        *reinterpret_cast<uint4 *>(p + j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    } else if constexpr (VEC) {
+        *reinterpret_cast<float4 *>(p + j) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + j + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (j + e < n) store_any(p + j + e, x[e]);
+    }
+#endif
+}
+
+template <class T, int ACT, bool VEC>
+__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums) {
+#if __HIP_DEVICE_COMPILE__
+    __shared__ float part[8][257];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int j = (blockIdx.x * 32 + tx) * 8;
+    const int r0 = blockIdx.y * kSumRows;
+    const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
+    float sum[8] = {};
+    if (j < (n > ld ? n : ld))
+#pragma unroll 2
+        for (int r = r0 + ty; r < r1; r += 8) {
+            float g[8];
+            load8<T, VEC>(dc + r * ldc, j, n, g);
+            if constexpr (ACT != SWC_HIP_ACT_NONE) {
+                float y[8];
+                load8<T, VEC>(z + r * ldz, j, n, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, sizeof(T) == 2>(y[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += j + e < n ? g[e] : 0.f;
+            if (dz) store8<T, VEC>(dz + r * ld, j, (int)ld, g);
+        }
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    float s = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) s += part[y][threadIdx.x];
+    if (col < n) sums[(size_t)blockIdx.y * n + col] = s;
+#endif
+}
+
+template <class T>
+int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda, const T *b, int ldb,
+               const T *preact, int ldp, int act, const T *da, int ldda, const T *db, int lddb, const T *dbias) {
+    if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
+    if (!known_act(act)) return fail(SWC_HIP_EINVAL, "%s: unknown activation %d", who, act);
+    if (m && n && !dc) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
+    if (act != SWC_HIP_ACT_NONE && m && n && !preact) return fail(SWC_HIP_EINVAL, "%s: preact is needed for this activation", who);
+    if ((da && m && n && k && !b) || (db && m && n && k && !a)) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
+    if (lddc < n || (da && (ldda < k || ldb < n)) || (db && (lddb < n || lda < k)) || (act != SWC_HIP_ACT_NONE && ldp < n))
+        return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
+    const void *in[4] = {dc, a, b, preact};
+    for (const void *p : in)
+        if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
+    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd || lddc > kMaxLd))
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
+    return SWC_HIP_OK;
+}
+
+int sum_blocks(int m) { return (m + kSumRows - 1) / kSumRows; }
+
+template <class T>
+int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
+    if (!dz) ld = 0;
+    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m));
+    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
+    constexpr int kPer = 16 / sizeof(T);
+    const bool vec = n % 8 == 0 && aligned16(dc) && lddc % kPer == 0 && (act == SWC_HIP_ACT_NONE || (aligned16(z) && ldz % kPer == 0)) &&
+                     (!dz || (aligned16(dz) && ld % kPer == 0));
+    return with_act(act, [&]<int ACT>() {
+        if (vec) act_grad<T, ACT, true><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        else act_grad<T, ACT, false><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        SWC_LAUNCH_CHECK();
+        return (int)SWC_HIP_OK;
+    });
+}
+
+struct GradSpace {
+    uint16_t *dz, *a, *b;
+    float *part, *sums;
+    size_t bytes;
+};
+GradSpace grad_space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool pack_b, size_t partials, bool bias) {
+    Carver c{base};
+    GradSpace s{};
+    s.dz = own_dz ? c.take<uint16_t>((size_t)m * round8(n)) : nullptr;
+    s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
+    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
+    s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
+    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
+    s.bytes = c.used;
+    return s;
+}
+
+// one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
+template <Layout LA, Layout LB>
+int grad_product(const char *who, const Plan &p, const Shape &s, uint16_t *out, long ld, float *part) {
+    if (p.splits == 1) return run_product<LA, LB>(p, s, StoreBf16{out, ld, aligned_rows(out, ld)}, who);
+    if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
+    return join_parts(out, ld, part, p.splits, s.m, s.n);
+}
+
+size_t max2(size_t a, size_t b) { return a > b ? a : b; }
+
+int grad_bf16(const char *who, int m, int n, int k, const uint16_t *dc, long lddc, const uint16_t *a, long lda,
+              const uint16_t *b, long ldb, const uint16_t *preact, long ldp, int act, uint16_t *da, long ldda, uint16_t *db,
+              long lddb, uint16_t *dbias) {
+    const Plan pa = plan_product(m, k, n), pb = plan_product(k, n, m);
+    // dZ is dC itself without an activation; a copy when its rows do not start on 16-byte boundaries, or when dA would
+    // read past the end of a row
+    const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || (da && n % 8));
+    const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || n % 8);
+    const size_t partials = max2(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
+    const size_t need = grad_space(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
+    GradSpace w{};
+    if (need) {
+        char *base = static_cast<char *>(workspace(need, who));
+        if (!base) return fail_code();
+        w = grad_space(base, m, n, k, own_dz, pack_a, pack_b, partials, dbias);
+    }
+    if (own_dz || dbias) {
+        if (int rc = launch_act_grad<uint16_t>(w.dz, round8(n), dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
+        if (dbias)
+            if (int rc = sum_parts(dbias, nullptr, w.sums, sum_blocks(m), n)) return rc;
+    }
+    const uint16_t *dz = own_dz ? w.dz : dc;
+    const long lddz = own_dz ? round8(n) : lddc;
+    if (pack_b) {
+        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = round8(n);
+    }
+    if (pack_a) {
+        if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, nullptr, nullptr)) return rc;
+        a = w.a, lda = round8(k);
+    }
+    if (da)
+        if (int rc = grad_product<kAlongK, kAlongK>(who, pa, Shape{dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
+    if (db)
+        if (int rc = grad_product<kAcross, kAcross>(who, pb, Shape{a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
+    return SWC_HIP_OK;
+}
+
+struct GradSpaceF {
+    float *dz, *at, *bt, *part, *sums;
+    size_t bytes;
+};
+GradSpaceF grad_space_f(char *base, int m, int n, int k, bool own_dz, bool da, bool db, size_t partials, bool bias) {
+    Carver c{base};
+    GradSpaceF s{};
+    s.dz = own_dz ? c.take<float>((size_t)m * n) : nullptr;
+    s.at = db ? c.take<float>((size_t)m * k) : nullptr;
+    s.bt = da ? c.take<float>((size_t)k * n) : nullptr;
+    s.part = c.take<float>(partials / sizeof(float) + 1);
+    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
+    s.bytes = c.used;
+    return s;
+}
+
+int grad_f32(const char *who, int m, int n, int k, const float *dc, int lddc, const float *a, int lda, const float *b, int ldb,
+             const float *preact, int ldp, int act, float *da, int ldda, float *db, int lddb, float *dbias) {
+    const bool own_dz = (da || db) && act != SWC_HIP_ACT_NONE;
+    const size_t partials = max2(da ? swc_hip_gemm_workspace_bytes(m, k, n) : 0, db ? swc_hip_gemm_workspace_bytes(k, n, m) : 0);
+    const size_t need = grad_space_f(nullptr, m, n, k, own_dz, da, db, partials, dbias).bytes;
+    char *base = static_cast<char *>(workspace(need, who));
+    if (!base) return fail_code();
+    const GradSpaceF w = grad_space_f(base, m, n, k, own_dz, da, db, partials, dbias);
+    if (own_dz || dbias) {
+        if (int rc = launch_act_grad<float>(w.dz, n, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
+        if (dbias)
+            if (int rc = sum_parts(nullptr, dbias, w.sums, sum_blocks(m), n)) return rc;
+    }
+    const float *dz = own_dz ? w.dz : dc;
+    const int lddz = own_dz ? n : lddc;
+    if (da) {
+        if (int rc = swc_hip_matrixTrans_f(k, n, b, ldb, w.bt, k)) return rc;
+        if (int rc = gemm_f32(who, m, k, n, dz, lddz, w.bt, k, nullptr, da, ldda, 0, w.part, partials)) return rc;
+    }
+    if (db) {
+        if (int rc = swc_hip_matrixTrans_f(m, k, a, lda, w.at, m)) return rc;
+        if (int rc = gemm_f32(who, k, n, m, w.at, m, dz, lddz, nullptr, db, lddb, 0, w.part, partials)) return rc;
+    }
+    return SWC_HIP_OK;
+}
+
+// what every form of the gradient call answers with when there is nothing to sum over
+template <class T>
+int grad_of_nothing(int m, int n, int k, T *da, int ldda, T *db, int lddb, T *dbias) {
+    if (int rc = zero_rows(da, ldda, m, k)) return rc;
+    if (int rc = zero_rows(db, lddb, k, n)) return rc;
+    return zero_rows(dbias, n, 1, n);
+}
+
+} // namespace
+
+extern "C" {
+
+int swc_hip_matrixMatrixFCActAddGrad_f(int m, int n, int k, const float *cGrad, int ldcg, const float *a, int lda, const float *b,
+                                       int ldb, const float *preact, int ldp, int act, float *aGrad, int ldag, float *bGrad,
+                                       int ldbg, float *biasGrad) {
+    const char *who = "swc_hip_matrixMatrixFCActAddGrad_f";
+    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
+    if (k == 0) aGrad = bGrad = nullptr;
+    return grad_f32(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+}
+
+int swc_hip_matrixMatrixFCActAddGrad_bf(int m, int n, int k, const swc_hip_bf16 *cGrad, int ldcg, const swc_hip_bf16 *a, int lda,
+                                        const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *preact, int ldp, int act,
+                                        swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad, int ldbg, swc_hip_bf16 *biasGrad) {
+    const char *who = "swc_hip_matrixMatrixFCActAddGrad_bf";
+    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
+    SWC_REQUIRE_INIT();
+    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
+    if (k == 0) aGrad = bGrad = nullptr;
+    return grad_bf16(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+}
+
+size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int bf) {
+    if (!ready() || m <= 0 || n <= 0) return 0;
+    if (bf) {
+        const size_t partials = k > 0 ? max2(plan_product(m, k, n).partial_bytes(m, k), plan_product(k, n, m).partial_bytes(k, n)) : 0;
+        return grad_space(nullptr, m, n, k, true, true, true, partials, true).bytes;
+    }
+    const size_t partials = max2(swc_hip_gemm_workspace_bytes(m, k, n), swc_hip_gemm_workspace_bytes(k, n, m));
+    return grad_space_f(nullptr, m, n, k, true, true, true, partials, true).bytes;
+}
+
+} // extern "C"

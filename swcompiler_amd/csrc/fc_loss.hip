@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_rows(const int *selected, i
 
 // ---------------------------------------------------------------- bf16 forward
 struct RowStats {
-    static constexpr bool kHeavy = true, kTall = false;
+    static constexpr bool kHeavy = true, kThinToo = true;
     float2 *part;     // [row][block]: maximum, sum of exp(z - maximum)
     int blocks;
     float *picked;    // [row]: z of the row's class
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(1024) void mean_loss(const float *row_loss, Rows ro
 // ---------------------------------------------------------------- bf16 gradients
 // dz of a piece of the vocabulary whose first class is `first`, zeros in the columns that pad it to whole 16 bytes
 struct StoreDz {
-    static constexpr bool kHeavy = true, kTall = false;
+    static constexpr bool kHeavy = true, kThinToo = true;
     uint16_t *dz;
     long ld;
     int first;
@@ -219,19 +219,39 @@ __global__ __launch_bounds__(256) void gather_row_values(const float *lse, const
     grad_out[i] = grad ? grad[r] : 1.f;
 }
 
-// out[r] = sum of `parts` buffers' dense row of r, zeros for a row left out
-template <class T>
+// out[r] = sum of `parts` buffers' dense row of r, zeros for a row left out; four columns a thread where cols allow
+template <class T, bool VEC>
 __global__ __launch_bounds__(256) void spread_rows(T *out, long ld, const float *part, int parts, long stride, int m, int cols,
                                                    const int *place) {
+    constexpr int kPer = VEC ? 4 : 1;
+    const int j = (blockIdx.x * 256 + threadIdx.x) * kPer;
+    if (j >= cols) return;
     for (int r = blockIdx.y; r < m; r += gridDim.y) {
         const int at = place[r];
-        for (int j = blockIdx.x * 256 + threadIdx.x; j < cols; j += gridDim.x * 256) {
-            float s = 0.f;
-            if (at >= 0)
-                for (int p = 0; p < parts; ++p) s += part[p * stride + (size_t)at * cols + j];
-            store_any(out + r * ld + j, s);
-        }
+        float s[kPer] = {};
+        if (at >= 0)
+#pragma unroll 4
+            for (int p = 0; p < parts; ++p) {
+                const float *q = part + p * stride + (size_t)at * cols + j;
+                if constexpr (VEC) {
+                    const float4 d = *reinterpret_cast<const float4 *>(q);
+                    s[0] += d.x, s[1] += d.y, s[2] += d.z, s[3] += d.w;
+                } else {
+                    s[0] += *q;
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) store_any(out + r * ld + j + e, s[e]);
     }
+}
+template <class T>
+int launch_spread(T *out, long ld, const float *part, int parts, long stride, int m, int cols, const int *place) {
+    const bool vec = cols % 4 == 0;
+    const dim3 grid(ceil_div(vec ? cols / 4 : cols, 256), m < 32768 ? m : 32768);
+    if (vec) spread_rows<T, true><<<grid, 256, 0, stream()>>>(out, ld, part, parts, stride, m, cols, place);
+    else spread_rows<T, false><<<grid, 256, 0, stream()>>>(out, ld, part, parts, stride, m, cols, place);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
 }
 
 // sums over blocks of kSumRows dense rows of a piece's columns
@@ -325,14 +345,9 @@ Rows take_rows(Carver &c, int m) {
 }
 
 // Whole rows of the contraction: the epilogues of this file need finished sums.
-Plan whole_plan(int m, int n, int k) {
-    Plan p = plan_product(m, n, k);
-    p.splits = 1;
-    p.k_per_split = ((k + 63) / 64 ? (k + 63) / 64 : 1) * 64;
-    return p;
-}
-int block_columns(const Plan &p) { return p.kind == kThin ? Thin::TN * 32 : 64; }
-static_assert(Big::TN == 2 && Mid::TN == 2 && Low::TN == 2, "64 columns a wavefront");
+Plan whole_plan(int m, int n, int k) { return plan_product(m, n, k, true); }
+int block_columns(const Plan &p) { return p.kind == kThin || p.kind == kSmall ? 32 : 64; }
+static_assert(Big::TN == 2 && Mid::TN == 2 && Low::TN == 2 && Small::TN == 1 && Thin::TN == 1, "columns of a wavefront");
 
 // ---------------------------------------------------------------- spaces
 struct ForwardSpace {
@@ -527,11 +542,7 @@ int grad_bf16(const char *who, int m, int n, int k, const uint16_t *a, long lda,
             if (int rc = sum_parts(dbias + first, nullptr, w.sums, parts, cols)) return rc;
         }
     }
-    if (da) {
-        spread_rows<uint16_t><<<rows_grid(m, k), 256, 0, stream()>>>(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place);
-        SWC_LAUNCH_CHECK();
-    }
-    return SWC_HIP_OK;
+    return da ? launch_spread(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place) : (int)SWC_HIP_OK;
 }
 
 int grad_f32(const char *who, int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
@@ -571,11 +582,7 @@ int grad_f32(const char *who, int m, int n, int k, const float *a, int lda, cons
             if (int rc = sum_parts(nullptr, dbias + first, w.sums, parts, cols)) return rc;
         }
     }
-    if (da) {
-        spread_rows<float><<<rows_grid(m, k), 256, 0, stream()>>>(da, ldda, w.da, 1, 0, m, k, w.rows.place);
-        SWC_LAUNCH_CHECK();
-    }
-    return SWC_HIP_OK;
+    return da ? launch_spread(da, ldda, w.da, 1, 0, m, k, w.rows.place) : (int)SWC_HIP_OK;
 }
 
 constexpr int kMaxRows = 65535 * kSumRows;

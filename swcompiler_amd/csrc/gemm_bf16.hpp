@@ -431,7 +431,7 @@ __device__ __forceinline__ float column_value(const v2u (&c)[4], int v) {
 
 // A bf16 matrix of the product, rows 16-byte aligned or not.
 struct StoreBf16 {
-    static constexpr bool kHeavy = false, kTall = false;
+    static constexpr bool kHeavy = false, kThinToo = true;
     uint16_t *out;
     long ld;
     bool vec;
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(C::kThreads) void gemm_bf16(Shape s, Ep ep) {
 
 // fp32 partial sums of split blockIdx.y (or the whole product when there is one): out[split][m][n], ld = n
 struct StorePartial {
-    static constexpr bool kHeavy = false, kTall = false;
+    static constexpr bool kHeavy = false, kThinToo = true;
     float *out;
     long split_stride;   // elements between the splits' matrices
     long ld;

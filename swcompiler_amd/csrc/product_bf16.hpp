@@ -6,14 +6,14 @@
 namespace swc_hip {
 namespace mfma16 {
 
-using Big = Cfg<4, 2, 2, 4, 64, 3, 2>;      // 256 x 256, eight wavefronts, one workgroup per CU
-using Mid = Cfg<2, 2, 2, 2, 64, 3, 2>;      // 128 x 128, four wavefronts, two workgroups per CU
-using Low = Cfg<1, 2, 2, 2, 64, 3, 3>;      // 64 x 128
-using Thin = Cfg<1, 1, 1, 4, 64, 4, 4>;     // 32 x 128: few rows, the other operand streams
+using Big = Cfg<4, 2, 2, 4, 64, 3, 2>;    // 256 x 256, eight wavefronts, one workgroup per CU
+using Deep = Cfg<4, 4, 2, 2, 64, 3, 2>;   // 256 x 256, four wavefronts of 128 x 128: a third less LDS traffic, a longer end
+using Mid = Cfg<2, 2, 2, 2, 64, 3, 2>;    // 128 x 128, four wavefronts, two workgroups per CU
+using Low = Cfg<1, 2, 2, 2, 64, 3, 3>;    // 64 x 128, two
+using Small = Cfg<1, 1, 2, 2, 64, 3, 3>;  // 64 x 64, three
+using Thin = Cfg<1, 1, 1, 4, 64, 4, 4>;   // 32 x 128, two: few rows, the other operand streams
 
-using Deep = Cfg<4, 4, 2, 2, 64, 3, 2>;  // 256 x 256, four wavefronts of 128 x 128: a third less LDS traffic, a longer end
-
-enum Kind { kBig, kDeep, kMid, kLow, kThin };
+enum Kind { kBig, kDeep, kMid, kLow, kSmall, kThin };
 struct Plan {
     Kind kind;
     int splits, k_per_split;
@@ -23,45 +23,66 @@ struct Plan {
 // most memory the partial sums of one product may take
 constexpr size_t kMaxPartials = (size_t)256 << 20;
 
-inline Plan plan_product(int m, int n, int k) {
+// The tile and the number of ranges of the contraction with the least estimated time (microseconds):
+//     start and end of a workgroup, f, for each round of the chip
+//   + slices * max(the time of a slice alone on a CU, workgroups per CU * its share of a busy CU)
+//   + the output at 4.5 TB/s, and for a cut contraction the joining kernel: 4 us and the partial sums again.
+// The constants are fits to 10 shapes of 128-2048 x 1024-4096 x 512-50264 at 1 to 32 ranges.  What the model leaves on
+// the table there against the best of all measured: 333 x 1411 x 1003 7.0 us (64 x 64 whole; 128 x 128 in four ranges
+// 8.3 and the joining), 512 x 4096 x 4096 24.4 (64 x 128 whole; 128 x 128 in two 23.0 and the joining),
+// 2048 x 4096 x 4096 63.5 (128 x 128; 256 x 256 83.2), 1400 x 1024 x 50264 175 (256 x 256 in eight; 128 x 128 in four 250).
+// one: only whole contractions.
+inline Plan plan_product(int m, int n, int k, bool one = false) {
+    struct Tile {
+        Kind kind;
+        int bm, bn, per_cu;
+        double f, alone, busy;
+    };
+    static constexpr Tile kTiles[] = {{kBig, 256, 256, 1, 10.8, 0.89, 1.2}, {kMid, 128, 128, 2, 4.3, 0.43, 0.46},
+                                      {kLow, 64, 128, 2, 4.3, 0.275, 0.32}, {kSmall, 64, 64, 3, 3.3, 0.225, 0.2},
+                                      {kThin, 32, 128, 2, 3.0, 0.2, 0.16}};
     const int cus = num_cus();
-    auto tiles = [&](int bm, int bn) { return (long)((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-    Plan p{kBig, 1, 0};
-    long have;
-    int per_cu;
-    if (m <= 32) p.kind = kThin, have = tiles(32, 128), per_cu = 2;
-    else if (m <= 64) p.kind = kLow, have = tiles(64, 128), per_cu = 2;
-    else if (tiles(256, 256) * 4 >= 3L * cus) p.kind = k >= 6144 ? kDeep : kBig, have = tiles(256, 256), per_cu = 1;
-    else p.kind = kMid, have = tiles(128, 128), per_cu = 2;
-    // too few tiles: ranges of the contraction, at least four slices each
-    const int slices = (k + 63) / 64;
-    long splits = 1;
-    if (have < (long)per_cu * cus && slices >= 8) {
-        splits = ((long)per_cu * cus + have - 1) / have;
-        if (splits > slices / 4) splits = slices / 4;
-        while (splits > 1 && (size_t)splits * m * n * sizeof(float) > kMaxPartials) --splits;
-        if (splits > 64) splits = 64;
+    const int slices = k > 0 ? (k + 63) / 64 : 1;
+    const double operands = 2.0 * ((double)m * k + (double)n * k) / 5e6;
+    Plan best{kMid, 1, slices * 64};
+    double least = 1e30;
+    for (const Tile &t : kTiles) {
+        if ((t.kind == kThin) != (m <= 32)) continue;
+        const long tiles = (long)((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+        for (int splits = 1; splits <= 64 && splits <= slices; splits += splits < 4 ? 1 : splits < 16 ? 2 : 8) {
+            const int each = (slices + splits - 1) / splits, s = (slices + each - 1) / each;
+            if (s > 1 && (one || each < 4 || (size_t)s * m * n * sizeof(float) > kMaxPartials)) break;
+            const double groups = (double)tiles * s;
+            const double q = groups <= cus ? 1 : groups >= 4.0 * t.per_cu * cus ? groups / cus : (double)((long)((groups + cus - 1) / cus));
+            const double rounds = q <= t.per_cu ? 1 : q / t.per_cu;
+            double work = each * (t.alone > q * t.busy ? t.alone : q * t.busy);
+            work = work > operands ? work : operands;
+            const double mn = (double)m * n;
+            const double cost = rounds * t.f + work + (s > 1 ? 4 + 8 * s * mn / 4.5e6 : 2 * mn / 4.5e6);
+            if (cost < least) least = cost, best = Plan{t.kind, s, each * 64};
+        }
     }
-    const int each = (int)((slices + splits - 1) / splits);
-    p.splits = slices ? (slices + each - 1) / each : 1;
-    p.k_per_split = (each ? each : 1) * 64;
-    return p;
+    // one wavefront per SIMD pays where the end of a tile is a small part of it: 8192^3 785 -> 757 us, K = 4096 412 -> 417
+    if (best.kind == kBig && best.k_per_split >= 6144) best.kind = kDeep;
+    return best;
 }
 
 // The epilogues with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
-// wavefront per SIMD has nothing beside it while they run; those with kTall exist for the large and middle tiles only.
+// wavefront per SIMD has nothing beside it while they run; those without kThinToo never run on 32-row tiles.
 template <Layout LA, Layout LB, class Ep>
 int run_product(const Plan &p, const Shape &s, const Ep &ep, const char *who) {
     Shape t = s;
     t.k_per_split = p.k_per_split;
     if constexpr (!Ep::kHeavy)
         if (p.kind == kDeep) return launch_gemm_bf16<Deep, LA, LB>(t, p.splits, ep, who);
-    if constexpr (!Ep::kTall) {
-        if (p.kind == kLow) return launch_gemm_bf16<Low, LA, LB>(t, p.splits, ep, who);
+    if constexpr (Ep::kThinToo)
         if (p.kind == kThin) return launch_gemm_bf16<Thin, LA, LB>(t, p.splits, ep, who);
+    switch (p.kind) {
+    case kMid: return launch_gemm_bf16<Mid, LA, LB>(t, p.splits, ep, who);
+    case kLow: return launch_gemm_bf16<Low, LA, LB>(t, p.splits, ep, who);
+    case kSmall: return launch_gemm_bf16<Small, LA, LB>(t, p.splits, ep, who);
+    default: return launch_gemm_bf16<Big, LA, LB>(t, p.splits, ep, who);
     }
-    if (p.kind == kMid) return launch_gemm_bf16<Mid, LA, LB>(t, p.splits, ep, who);
-    return launch_gemm_bf16<Big, LA, LB>(t, p.splits, ep, who);
 }
 
 inline bool aligned_rows(const void *p, long ld) { return aligned16(p) && ld % 8 == 0; }
@@ -107,7 +128,9 @@ template <class T> int zero_rows(T *p, long ld, int rows, int cols) {
 // dst[r][0..ld) = src[rows ? rows[r] : r][0..cols) and zeros; rows at or beyond *count (when given) become zeros
 int copy_rows_bf16(uint16_t *dst, long ld, const uint16_t *src, long lds, int rows, int cols, const int *index, const int *count);
 int copy_rows_f32(float *dst, long ld, const float *src, long lds, int rows, int cols, const int *index, const int *count);
-// out[j] = sum over parts p of part[p][j], in that order
+// out[m][n] (rows of ld) = the sum of `parts` matrices, in order
+int join_parts(uint16_t *out, long ld, const float *part, int parts, int m, int n);
+// out[j] = sum over parts p of part[p][j], in a fixed order
 int sum_parts(uint16_t *out_bf, float *out_f, const float *part, int parts, int n);
 
 } // namespace mfma16

@@ -189,32 +189,37 @@ class _Arg:
     __slots__ = ("ptr", "shape", "type", "ld", "size")
 
     def __init__(self, rt, x, what):
-        self.shape = tuple(x.shape)
-        self.size = 1
-        for n in self.shape:
-            self.size *= n
+        self.shape = shape = tuple(x.shape)
         if isinstance(x, DeviceArray):
-            self.ptr, self.type = x.ptr, _NUMPY_TYPES.get(x.dtype.name)
-            self.ld = self.shape[-1] if self.shape else 1
+            self.ptr, self.type, self.size = x.ptr, _NUMPY_TYPES.get(x.dtype.name), x.size
+            self.ld = shape[-1] if shape else 1
             return
-        if not hasattr(x, "data_ptr"):
-            raise SwcHipError(f"{what}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
-        if x.device.type != "cuda" or x.device.index != rt.device:
-            raise SwcHipError(f"{what}: the tensor is on {x.device}, the runtime on device {rt.device}")
-        self.ptr, self.type = x.data_ptr() or None, _TORCH_TYPES.get(str(x.dtype))
+        self.ptr, self.type, self.size = _torch_operand(rt, x, what)
+        self.ld = shape[-1] if shape else 1
+        if x.is_contiguous():
+            return
         stride = x.stride()
-        for n, st in zip(self.shape[-1:], stride[-1:]):
-            if n > 1 and st != 1:
-                raise SwcHipError(f"{what}: the elements of a row are not contiguous (stride {st})")
-        self.ld = self.shape[-1] if self.shape else 1
-        if len(self.shape) == 2 and self.shape[0] > 1:
+        if len(shape) > 2 or (shape[-1] > 1 and stride[-1] != 1):
+            raise SwcHipError(f"{what}: the elements of a row are not contiguous (strides {stride})")
+        if len(shape) == 2 and shape[0] > 1:
             self.ld = stride[0]
-            if self.ld < self.shape[1]:
-                raise SwcHipError(f"{what}: rows overlap (stride {self.ld}, {self.shape[1]} columns)")
-        elif len(self.shape) > 2 and not x.is_contiguous():
-            raise SwcHipError(f"{what}: the tensor is not contiguous")
+            if self.ld < shape[1]:
+                raise SwcHipError(f"{what}: rows overlap (stride {self.ld}, {shape[1]} columns)")
 
 
+def _torch_operand(rt, x, what):
+    """-> (address, element type, elements) of a torch tensor on the runtime's device"""
+    if not hasattr(x, "data_ptr"):
+        raise SwcHipError(f"{what}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
+    if x.get_device() != rt.device:
+        raise SwcHipError(f"{what}: the tensor is on {x.device}, the runtime on device {rt.device}")
+    kind = _TORCH_KINDS.get(x.dtype)
+    if kind is None:
+        kind = _TORCH_KINDS[x.dtype] = _TORCH_TYPES.get(str(x.dtype), "?")
+    return x.data_ptr() or None, kind, x.numel()
+
+
+_TORCH_KINDS = {}     # torch.dtype -> element type, filled as they are met (this module does not import torch)
 _NUMPY_TYPES = {"float32": "f32", "int32": "i32", "uint16": "bf16", "uint8": "u8"}   # bfloat16 travels as its bits
 _TORCH_TYPES = {"torch.float32": "f32", "torch.int32": "i32", "torch.bfloat16": "bf16", "torch.uint16": "bf16",
                 "torch.uint8": "u8", "torch.float8_e4m3fn": "u8"}
@@ -787,34 +792,45 @@ class SwcHip:
 
     def _adamw(self, what, w, dw, states, scales, copies, state, lr, beta1, beta2, eps, decay, lr_factor, grad_factor):
         count = len(w)
-        sizes, dtype = (C.c_size_t * count)(), None
-        lists = [w, dw] + states + scales + ([copies] if copies is not None else [])
-        if any(len(x) != count for x in lists):
-            raise SwcHipError(f"{what}: lists of different lengths")
-        pointers = [(C.c_void_p * count)() for _ in lists]
-        state_type = ("u8",) if scales else ("f32",)
-        types = [("f32",), ("f32", "bf16")] + [state_type] * 2 + [("f32",)] * len(scales) + [("bf16",)]
-        for i in range(count):
-            for j, values in enumerate(lists):
-                if values[i] is None and copies is not None and j == len(lists) - 1:
+
+        def addresses(values, types, sizes, name):
+            """-> (array of addresses, element counts, the type of all)"""
+            if len(values) != count:
+                raise SwcHipError(f"{what}: lists of different lengths")
+            out, found, kind = [], [], types[0]
+            for i, x in enumerate(values):
+                if x is None and name == "copies":
+                    out.append(None)
                     continue
-                x = self._arg(values[i], f"{what}: tensor {i}", types[j])
-                if len(x.shape) == 2 and x.ld != x.shape[1]:
-                    raise SwcHipError(f"{what}: tensor {i} is not contiguous")
-                if j == 0:
-                    sizes[i] = x.size
-                want = -(-sizes[i] // ADAMW_BLOCK) if 4 <= j < 4 + len(scales) else sizes[i]
-                if x.size != want:
-                    raise SwcHipError(f"{what}: tensor {i}: {x.size} elements, expected {want}")
-                if j == 1:
-                    if dtype not in (None, x.type):
-                        raise SwcHipError(f"{what}: gradients of different types")
-                    dtype = x.type
-                pointers[j][i] = x.ptr
-        if scales:   # w, dw, mom8, momScale, var8, varScale
-            pointers[3], pointers[4] = pointers[4], pointers[3]
-        if copies is None:
-            pointers.append(None)
+                if isinstance(x, DeviceArray):
+                    ptr, t, n = x.ptr, _NUMPY_TYPES.get(x.dtype.name), x.size
+                else:
+                    ptr, t, n = _torch_operand(self, x, f"{what}: {name} of tensor {i}")
+                    if not x.is_contiguous():
+                        raise SwcHipError(f"{what}: {name} of tensor {i} is not contiguous")
+                if t not in types:
+                    raise SwcHipError(f"{what}: {name} of tensor {i}: element type {t} is not one of {', '.join(types)}")
+                if sizes is not None and n != sizes[i]:
+                    raise SwcHipError(f"{what}: {name} of tensor {i}: {n} elements, expected {sizes[i]}")
+                if i and t != kind:
+                    raise SwcHipError(f"{what}: {name} of different types")
+                kind = t
+                out.append(ptr)
+                found.append(n)
+            return (C.c_void_p * count)(*out), found, kind
+
+        pw, sizes, _ = addresses(w, ("f32",), None, "w")
+        pg, _, dtype = addresses(dw, ("f32", "bf16"), sizes, "dw")
+        held = ("u8",) if scales else ("f32",)
+        pm, pv = addresses(states[0], held, sizes, "mom")[0], addresses(states[1], held, sizes, "var")[0]
+        if scales:
+            blocks = [-(-n // ADAMW_BLOCK) for n in sizes]
+            pms, pvs = (addresses(x, ("f32",), blocks, name)[0] for x, name in zip(scales, ("mom_scale", "var_scale")))
+            pointers = [pw, pg, pm, pms, pv, pvs]
+        else:
+            pointers = [pw, pg, pm, pv]
+        pointers.append(None if copies is None else addresses(copies, ("bf16",), sizes, "copies")[0])
+        sizes = (C.c_size_t * count)(*sizes)
         one = [self._p(self._arg(x, f"{what}: factor", ("f32",))) for x in (lr_factor, grad_factor)]
         fn = getattr(self.lib, f"swc_hip_{what}" + ("_bf" if dtype == "bf16" else "_f"))
         self._check(fn(count, *pointers, sizes, self._state(state, what), lr, beta1, beta2, eps, decay, *one), what)
