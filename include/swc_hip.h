@@ -428,7 +428,7 @@ size_t swc_hip_conv2dFusedMaxpool_workspace_bytes(const size_t *cdims, const siz
 /* ---- operators of language models.  No counterparts in the reference: each
  * stands next to an op above whose work it does in the form that such models
  * need.  Matrices are row-major with leading dimensions in elements (at most
- * 4194240 for the _bf forms); outputs must not overlap inputs except where it
+ * 4194240 for the _bf forms, 2097088 for the _f ones); outputs must not overlap inputs except where it
  * is said.  Workspace: the size queries below, which answer for every alignment
  * of the operands. ---- */
 

@@ -31,10 +31,6 @@ void *workspace(size_t bytes, const char *who);
 // Looks up, for `device` (which must be current), the address of the fixed scratch array of the entry point
 // that allocates nothing (gemm.hip); called once per device by swc_hip_init.
 int gemm_noalloc_setup(int device);
-// C = A * B (+ bias, ReLU) on the fp32 kernels of gemm.hip with the partial sums of a product cut along K in `part`
-// (swc_hip_gemm_workspace_bytes of them, not null): for ops that keep other things in the workspace.
-int gemm_f32(const char *who, int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
-             float *c, int ldc, int relu, float *part, size_t part_bytes);
 
 // Test and tuning switches (the SWC_HIP_* environment variables; none is part of the contract).  swc_hip_init reads
 // them ONCE into this record (swc_hip_reload_switches reads them again, for a test process that changes them): no

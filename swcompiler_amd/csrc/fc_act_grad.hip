@@ -1,14 +1,15 @@
-// The gradients of the fully connected layer with its activation (matrixMatrixFCActAddGrad_f/_bf).
+// The gradients of the fully connected layer with its activation (matrixMatrixFCActAddGrad_f/_bf):
 //
 //     dZ = dC act'(Z), dA = dZ B^T, dB = A^T dZ, dbias = column sums of dZ
 //
-// bf16: the two products on the core of gemm_bf16.hpp, no matrix transposed in memory; dZ is rounded to bf16 once, for
-// both.  fp32: the kernels of gemm.hip take row-major operands, so A and B are transposed into the workspace first.
+// The two products on the core of product_tile.hpp, no matrix transposed in memory; dZ in one pass (three times its size
+// at the memory's rate), rounded to the matrices' type once for both products, its column sums before that rounding.
+// Without an activation dZ is dC itself.  4096 x 16384 x 4096 bf16 with tanh gelu: 872 us, 1260 TFLOP/s.
 #include "act.hpp"
-#include "product_bf16.hpp"
+#include "product.hpp"
 
 using namespace swc_hip;
-using namespace swc_hip::mfma16;
+using namespace swc_hip::product;
 
 namespace {
 
@@ -16,7 +17,7 @@ namespace {
 // values.  32 threads side by side hold eight columns each, eight rows at a time; VEC: 16 bytes of a row at once.
 constexpr int kSumRows = 32;
 template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int j, int n, float (&x)[8]) {
-    if constexpr (VEC && sizeof(T) == 2) {
+    if constexpr (VEC && kIsBf16<T>) {
         const uint4 d = *reinterpret_cast<const uint4 *>(p + j);
         const unsigned w[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
@@ -31,7 +32,7 @@ template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, i
 }
 template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int j, int n, const float (&x)[8]) {
 #if __HIP_DEVICE_COMPILE__
-    if constexpr (VEC && sizeof(T) == 2) {
+    if constexpr (VEC && kIsBf16<T>) {
         *reinterpret_cast<uint4 *>(p + j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
     } else if constexpr (VEC) {
         *reinterpret_cast<float4 *>(p + j) = make_float4(x[0], x[1], x[2], x[3]);
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, lon
                 float y[8];
                 load8<T, VEC>(z + r * ldz, j, n, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, sizeof(T) == 2>(y[e]);
+                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, kIsBf16<T>>(y[e]);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += j + e < n ? g[e] : 0.f;
@@ -93,8 +94,8 @@ int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, cons
     const void *in[4] = {dc, a, b, preact};
     for (const void *p : in)
         if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
-    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd || lddc > kMaxLd))
-        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
+    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || lddc > kMaxLd<T>)
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
     return SWC_HIP_OK;
 }
 
@@ -116,119 +117,86 @@ int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz
     });
 }
 
-struct GradSpace {
-    uint16_t *dz, *a, *b;
+template <class T> struct Space {
+    T *dz, *a, *b;
     float *part, *sums;
     size_t bytes;
 };
-GradSpace grad_space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool pack_b, size_t partials, bool bias) {
+template <class T>
+Space<T> space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool pack_b, size_t partials, bool bias) {
     Carver c{base};
-    GradSpace s{};
-    s.dz = own_dz ? c.take<uint16_t>((size_t)m * round8(n)) : nullptr;
-    s.a = pack_a ? c.take<uint16_t>((size_t)m * round8(k)) : nullptr;
-    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
+    Space<T> s{};
+    s.dz = own_dz ? c.take<T>((size_t)m * row_length<T>(n)) : nullptr;
+    s.a = pack_a ? c.take<T>((size_t)m * row_length<T>(k)) : nullptr;
+    s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
     s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
     s.bytes = c.used;
     return s;
 }
 
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+
 // one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
-template <Layout LA, Layout LB>
-int grad_product(const char *who, const Plan &p, const Shape &s, uint16_t *out, long ld, float *part) {
-    if (p.splits == 1) return run_product<LA, LB>(p, s, StoreBf16{out, ld, aligned_rows(out, ld)}, who);
+template <Layout LA, Layout LB, class T>
+int grad_product(const char *who, const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
+    if (p.splits == 1) return run_product<LA, LB>(p, s, Store<T>{out, ld, aligned_rows(out, ld)}, who);
     if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
-    return join_parts(out, ld, part, p.splits, s.m, s.n);
+    return join_parts<T>(out, ld, part, p.splits, s.m, s.n);
 }
 
-size_t max2(size_t a, size_t b) { return a > b ? a : b; }
-
-int grad_bf16(const char *who, int m, int n, int k, const uint16_t *dc, long lddc, const uint16_t *a, long lda,
-              const uint16_t *b, long ldb, const uint16_t *preact, long ldp, int act, uint16_t *da, long ldda, uint16_t *db,
-              long lddb, uint16_t *dbias) {
-    const Plan pa = plan_product(m, k, n), pb = plan_product(k, n, m);
+template <class T>
+int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda_, const T *b, int ldb_, const T *preact,
+              int ldp, int act, T *da, int ldda, T *db, int lddb, T *dbias) {
+    if (int rc = check_grad(who, m, n, k, dc, lddc, a, lda_, b, ldb_, preact, ldp, act, da, ldda, db, lddb, dbias)) return rc;
+    if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
+    if (m == 0 || n == 0) {   // sums of nothing
+        if (int rc = zero_rows(da, ldda, m, k)) return rc;
+        if (int rc = zero_rows(db, lddb, k, n)) return rc;
+        return zero_rows(dbias, n, 1, n);
+    }
+    if (k == 0) da = db = nullptr;
+    long lda = lda_, ldb = ldb_;
+    const Plan pa = plan_product<T>(m, k, n), pb = plan_product<T>(k, n, m);
     // dZ is dC itself without an activation; a copy when its rows do not start on 16-byte boundaries, or when dA would
     // read past the end of a row
-    const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || (da && n % 8));
-    const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || n % 8);
-    const size_t partials = max2(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
-    const size_t need = grad_space(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
-    GradSpace w{};
+    const bool tail = da && n % kChunk<T>;
+    const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || tail);
+    const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || tail);
+    const size_t partials = larger(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
+    const size_t need = space<T>(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
+    Space<T> w{};
     if (need) {
         char *base = static_cast<char *>(workspace(need, who));
         if (!base) return fail_code();
-        w = grad_space(base, m, n, k, own_dz, pack_a, pack_b, partials, dbias);
+        w = space<T>(base, m, n, k, own_dz, pack_a, pack_b, partials, dbias);
     }
+    const long padded = row_length<T>(n);
     if (own_dz || dbias) {
-        if (int rc = launch_act_grad<uint16_t>(w.dz, round8(n), dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
+        if (int rc = launch_act_grad<T>(w.dz, padded, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
         if (dbias)
-            if (int rc = sum_parts(dbias, nullptr, w.sums, sum_blocks(m), n)) return rc;
+            if (int rc = sum_parts<T>(dbias, w.sums, sum_blocks(m), n)) return rc;
     }
-    const uint16_t *dz = own_dz ? w.dz : dc;
-    const long lddz = own_dz ? round8(n) : lddc;
+    const T *dz = own_dz ? w.dz : dc;
+    const long lddz = own_dz ? padded : lddc;
     if (pack_b) {
-        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = round8(n);
+        if (int rc = copy_rows<T>(w.b, padded, b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = padded;
     }
     if (pack_a) {
-        if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, nullptr, nullptr)) return rc;
-        a = w.a, lda = round8(k);
+        if (int rc = copy_rows<T>(w.a, row_length<T>(k), a, lda, m, k, nullptr, nullptr)) return rc;
+        a = w.a, lda = row_length<T>(k);
     }
     if (da)
-        if (int rc = grad_product<kAlongK, kAlongK>(who, pa, Shape{dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
+        if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, {dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
     if (db)
-        if (int rc = grad_product<kAcross, kAcross>(who, pb, Shape{a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
+        if (int rc = grad_product<kAcross, kAcross, T>(who, pb, {a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
     return SWC_HIP_OK;
 }
 
-struct GradSpaceF {
-    float *dz, *at, *bt, *part, *sums;
-    size_t bytes;
-};
-GradSpaceF grad_space_f(char *base, int m, int n, int k, bool own_dz, bool da, bool db, size_t partials, bool bias) {
-    Carver c{base};
-    GradSpaceF s{};
-    s.dz = own_dz ? c.take<float>((size_t)m * n) : nullptr;
-    s.at = db ? c.take<float>((size_t)m * k) : nullptr;
-    s.bt = da ? c.take<float>((size_t)k * n) : nullptr;
-    s.part = c.take<float>(partials / sizeof(float) + 1);
-    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
-    s.bytes = c.used;
-    return s;
-}
-
-int grad_f32(const char *who, int m, int n, int k, const float *dc, int lddc, const float *a, int lda, const float *b, int ldb,
-             const float *preact, int ldp, int act, float *da, int ldda, float *db, int lddb, float *dbias) {
-    const bool own_dz = (da || db) && act != SWC_HIP_ACT_NONE;
-    const size_t partials = max2(da ? swc_hip_gemm_workspace_bytes(m, k, n) : 0, db ? swc_hip_gemm_workspace_bytes(k, n, m) : 0);
-    const size_t need = grad_space_f(nullptr, m, n, k, own_dz, da, db, partials, dbias).bytes;
-    char *base = static_cast<char *>(workspace(need, who));
-    if (!base) return fail_code();
-    const GradSpaceF w = grad_space_f(base, m, n, k, own_dz, da, db, partials, dbias);
-    if (own_dz || dbias) {
-        if (int rc = launch_act_grad<float>(w.dz, n, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
-        if (dbias)
-            if (int rc = sum_parts(nullptr, dbias, w.sums, sum_blocks(m), n)) return rc;
-    }
-    const float *dz = own_dz ? w.dz : dc;
-    const int lddz = own_dz ? n : lddc;
-    if (da) {
-        if (int rc = swc_hip_matrixTrans_f(k, n, b, ldb, w.bt, k)) return rc;
-        if (int rc = gemm_f32(who, m, k, n, dz, lddz, w.bt, k, nullptr, da, ldda, 0, w.part, partials)) return rc;
-    }
-    if (db) {
-        if (int rc = swc_hip_matrixTrans_f(m, k, a, lda, w.at, m)) return rc;
-        if (int rc = gemm_f32(who, k, n, m, w.at, m, dz, lddz, nullptr, db, lddb, 0, w.part, partials)) return rc;
-    }
-    return SWC_HIP_OK;
-}
-
-// what every form of the gradient call answers with when there is nothing to sum over
-template <class T>
-int grad_of_nothing(int m, int n, int k, T *da, int ldda, T *db, int lddb, T *dbias) {
-    if (int rc = zero_rows(da, ldda, m, k)) return rc;
-    if (int rc = zero_rows(db, lddb, k, n)) return rc;
-    return zero_rows(dbias, n, 1, n);
+template <class T> size_t most(int m, int n, int k) {
+    const size_t partials = k > 0 ? larger(plan_product<T>(m, k, n).partial_bytes(m, k), plan_product<T>(k, n, m).partial_bytes(k, n)) : 0;
+    return space<T>(nullptr, m, n, k > 0 ? k : 0, true, true, true, partials, true).bytes;
 }
 
 } // namespace
@@ -238,33 +206,20 @@ extern "C" {
 int swc_hip_matrixMatrixFCActAddGrad_f(int m, int n, int k, const float *cGrad, int ldcg, const float *a, int lda, const float *b,
                                        int ldb, const float *preact, int ldp, int act, float *aGrad, int ldag, float *bGrad,
                                        int ldbg, float *biasGrad) {
-    const char *who = "swc_hip_matrixMatrixFCActAddGrad_f";
-    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
-    SWC_REQUIRE_INIT();
-    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
-    if (k == 0) aGrad = bGrad = nullptr;
-    return grad_f32(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+    return gradients<float>("swc_hip_matrixMatrixFCActAddGrad_f", m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag,
+                            bGrad, ldbg, biasGrad);
 }
 
 int swc_hip_matrixMatrixFCActAddGrad_bf(int m, int n, int k, const swc_hip_bf16 *cGrad, int ldcg, const swc_hip_bf16 *a, int lda,
                                         const swc_hip_bf16 *b, int ldb, const swc_hip_bf16 *preact, int ldp, int act,
                                         swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad, int ldbg, swc_hip_bf16 *biasGrad) {
-    const char *who = "swc_hip_matrixMatrixFCActAddGrad_bf";
-    if (int rc = check_grad(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad)) return rc;
-    SWC_REQUIRE_INIT();
-    if (m == 0 || n == 0) return grad_of_nothing(m, n, k, aGrad, ldag, bGrad, ldbg, biasGrad);
-    if (k == 0) aGrad = bGrad = nullptr;
-    return grad_bf16(who, m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag, bGrad, ldbg, biasGrad);
+    return gradients<bf16>("swc_hip_matrixMatrixFCActAddGrad_bf", m, n, k, cGrad, ldcg, a, lda, b, ldb, preact, ldp, act, aGrad, ldag,
+                           bGrad, ldbg, biasGrad);
 }
 
 size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int bf) {
     if (!ready() || m <= 0 || n <= 0) return 0;
-    if (bf) {
-        const size_t partials = k > 0 ? max2(plan_product(m, k, n).partial_bytes(m, k), plan_product(k, n, m).partial_bytes(k, n)) : 0;
-        return grad_space(nullptr, m, n, k, true, true, true, partials, true).bytes;
-    }
-    const size_t partials = max2(swc_hip_gemm_workspace_bytes(m, k, n), swc_hip_gemm_workspace_bytes(k, n, m));
-    return grad_space_f(nullptr, m, n, k, true, true, true, partials, true).bytes;
+    return bf ? most<bf16>(m, n, k) : most<float>(m, n, k);
 }
 
 } // extern "C"

@@ -4,20 +4,21 @@
 //     z = A B + bias,  lse_r = log sum_j exp z_rj,  loss_r = lse_r - z[r, sel_r]
 //     dz_rj = g_r (exp(z_rj - lse_r) - [j = sel_r]),  dA = dz B^T,  dB = A^T dz,  dbias = column sums of dz
 //
-// bf16 forward: the product's accumulators never leave the registers; a wavefront reduces its 64 (32) columns of each
-// row to a maximum and a sum of exponentials, 8 bytes per row and block, which a second kernel joins — sums relative to
-// different maxima m_i join as sum_i s_i exp(m_i - max).  Gradients: piece by piece of the vocabulary the logits are
-// computed again, become dz in the epilogue (bf16, in the workspace) and feed the two products; dA is summed over the
-// pieces in fp32, each range of the contraction in a buffer of its own, and joined in a fixed order at the end: no
-// atomics, the same bits every time.  8 mnk flops for loss and gradients instead of 6 with the logits kept.
+// Forward: the product's accumulators never leave the registers; a wavefront reduces its 64 (32) columns of each row to a
+// maximum and a sum of exponentials, 8 bytes per row and block, which a second kernel joins — sums relative to different
+// maxima m_i join as sum_i s_i exp(m_i - max).  Gradients: piece by piece of the vocabulary the logits are computed
+// again, become dz in the epilogue (in the matrices' type, in the workspace) and feed the two products; dA is summed
+// over the pieces in fp32, each range of the contraction in a buffer of its own, and joined in a fixed order at the end:
+// no atomics, the same bits every time.  8 mnk flops for loss and gradients instead of 6 with the logits kept: 8192 x
+// 128256 x 4096 bf16 25.4 ms, 1355 TFLOP/s of them.
 //
 // Rows left out (their class outside the vocabulary) are dropped first: the rows that count are gathered into a dense
 // copy of A, so the products skip the others' work and nothing in them can reach a sum (0 * NaN is NaN).  Their number
 // is known on the device only; the kernels read it there.
-#include "product_bf16.hpp"
+#include "product.hpp"
 
 using namespace swc_hip;
-using namespace swc_hip::mfma16;
+using namespace swc_hip::product;
 
 namespace {
 
@@ -58,58 +59,56 @@ __global__ __launch_bounds__(kPickThreads) void pick_rows(const int *selected, i
     if (threadIdx.x == 0) *out.count = base;
 }
 
-// ---------------------------------------------------------------- bf16 forward
-struct RowStats {
+// bf16: the exponential instruction (relative error |x| 2^-24 and a little); fp32: the library function
+template <class T> __device__ __forceinline__ float exponential(float x) { return kIsBf16<T> ? fast_exp(x) : expf(x); }
+
+// ---------------------------------------------------------------- forward
+template <class T> struct RowStats {
     static constexpr bool kHeavy = true, kThinToo = true;
     float2 *part;     // [row][block]: maximum, sum of exp(z - maximum)
     int blocks;
     float *picked;    // [row]: z of the row's class
     const int *sel;
-    const uint16_t *bias;
+    const T *bias;
 #if __HIP_DEVICE_COMPILE__
-    template <bool WHOLE, int TM, int TN>
+    template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void reduce(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
-        v2u b[TN][4];
-        if (bias)
-#pragma unroll
-            for (int tn = 0; tn < TN; ++tn) load_columns<WHOLE>(bias, col0 + tn * 32, n, h, b[tn]);
+        ColumnData<T, P> b;
+        if (bias) b.template load<WHOLE>(bias, col0, n, h);
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int row = row0 + tm * 32 + l32;
+            const int row = row0 + P::row(tm, l32);
             const int want = (row < m ? sel[row] : -1) - col0;
-            float z[TN * 16];
+            float z[P::kValues];
             float top = -__builtin_inff();
 #pragma unroll
-            for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    float x = acc[tm][tn][v];
-                    if (bias) x += column_value(b[tn], v);
-                    if (!WHOLE && col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4 >= n) x = -__builtin_inff();
-                    z[tn * 16 + v] = x;
-                    top = fmaxf(top, x);
-                }
+            for (int u = 0; u < P::kValues; ++u) {
+                float x = P::value(acc[tm], u);
+                if (bias) x += b.value(u);
+                if (!WHOLE && col0 + P::column(u, h) >= n) x = -__builtin_inff();
+                z[u] = x;
+                top = fmaxf(top, x);
+            }
             if (__any(want >= 0 && want < 32 * TN)) {   // a row of these 32 has its class here
 #pragma unroll
-                for (int v = 0; v < TN * 16; ++v)
-                    if (v / 16 * 32 + 8 * (v % 16 / 4) + 4 * h + v % 4 == want) picked[row] = z[v];
+                for (int u = 0; u < P::kValues; ++u)
+                    if (P::column(u, h) == want) picked[row] = z[u];
             }
             top = fmaxf(top, __shfl_xor(top, 32));
             const float from = top == -__builtin_inff() ? 0.f : top;   // a block of impossible classes only
             float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < TN * 16; ++v) sum += fast_exp(z[v] - from);
+            for (int u = 0; u < P::kValues; ++u) sum += exponential<T>(z[u] - from);
             sum += __shfl_xor(sum, 32);
             if (h == 0 && row < m) part[(size_t)row * blocks + col0 / (32 * TN)] = make_float2(top, sum);
         }
     }
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
+    template <class P, int TM, int TN>
+    __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
         if (col0 >= n) return;
-        if (col0 + 32 * TN <= n && (reinterpret_cast<uintptr_t>(bias) & 7) == 0) reduce<true>(acc, row0, col0, m, n, lane);
-        else reduce<false>(acc, row0, col0, m, n, lane);
+        if (col0 + 32 * TN <= n && reinterpret_cast<uintptr_t>(bias) % (4 * sizeof(T)) == 0) reduce<P, true>(acc, row0, col0, m, n, lane);
+        else reduce<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
@@ -152,60 +151,53 @@ __global__ __launch_bounds__(1024) void mean_loss(const float *row_loss, Rows ro
     if (threadIdx.x == 0) *loss = count ? (float)(sums[0] / count) : 0.f;
 }
 
-// ---------------------------------------------------------------- bf16 gradients
+// ---------------------------------------------------------------- gradients
 // dz of a piece of the vocabulary whose first class is `first`, zeros in the columns that pad it to whole 16 bytes
-struct StoreDz {
+template <class T> struct StoreDz {
     static constexpr bool kHeavy = true, kThinToo = true;
-    uint16_t *dz;
+    T *dz;
     long ld;
     int first;
     const int *sel;
     const float *lse, *grad;
-    const uint16_t *bias;   // of the piece
+    const T *bias;   // of the piece
 #if __HIP_DEVICE_COMPILE__
-    template <bool WHOLE, int TM, int TN>
+    template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
         const int l32 = lane & 31, h = lane >> 5;
-        v2u b[TN][4];
-        if (bias)
-#pragma unroll
-            for (int tn = 0; tn < TN; ++tn) load_columns<WHOLE>(bias, col0 + tn * 32, n, h, b[tn]);
+        ColumnData<T, P> b;
+        if (bias) b.template load<WHOLE>(bias, col0, n, h);
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int row = row0 + tm * 32 + l32;
+            const int row = row0 + P::row(tm, l32);
             const bool ok = WHOLE || row < m;
             const int want = (ok ? sel[row] : -1) - first - col0;
             const float l = ok ? lse[row] : 0.f, g = ok ? grad[row] : 0.f;
-            const bool here = __any(ok && want >= 0 && want < 32 * TN);   // a row of these 32 has its class here
+            float x[P::kValues];
 #pragma unroll
-            for (int tn = 0; tn < TN; ++tn) {
-                float x[16];
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    float z = acc[tm][tn][v];
-                    if (bias) z += column_value(b[tn], v);
-                    x[v] = fast_exp(z - l);
-                }
-                if (here) {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (tn * 32 + 8 * (v / 4) + 4 * h + v % 4 == want) x[v] -= 1.f;
-                }
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    x[v] *= g;
-                    if (!WHOLE && col0 + tn * 32 + 8 * (v / 4) + 4 * h + v % 4 >= n) x[v] = 0.f;
-                }
-                store_block<WHOLE>(dz + row * ld, ok, col0 + tn * 32, (int)ld, true, h, x);
+            for (int u = 0; u < P::kValues; ++u) {
+                float z = P::value(acc[tm], u);
+                if (bias) z += b.value(u);
+                x[u] = exponential<T>(z - l);
             }
+            if (__any(ok && want >= 0 && want < 32 * TN)) {   // a row of these 32 has its class here
+#pragma unroll
+                for (int u = 0; u < P::kValues; ++u)
+                    if (P::column(u, h) == want) x[u] -= 1.f;
+            }
+#pragma unroll
+            for (int u = 0; u < P::kValues; ++u) {
+                x[u] *= g;
+                if (!WHOLE && col0 + P::column(u, h) >= n) x[u] = 0.f;
+            }
+            store_row<P, WHOLE>(dz + row * ld, ok, col0, (int)ld, true, h, x);
         }
     }
-    template <int TM, int TN>
-    __device__ __forceinline__ void operator()(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane,
-                                               int) const {
-        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n && (reinterpret_cast<uintptr_t>(bias) & 7) == 0)
-            store<true>(acc, row0, col0, m, n, lane);
-        else store<false>(acc, row0, col0, m, n, lane);
+    template <class P, int TM, int TN>
+    __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
+        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n && reinterpret_cast<uintptr_t>(bias) % (4 * sizeof(T)) == 0)
+            store<P, true>(acc, row0, col0, m, n, lane);
+        else store<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
@@ -267,71 +259,18 @@ __global__ __launch_bounds__(256) void column_sums(const T *dz, long ld, int col
     sums[(size_t)blockIdx.y * cols + j] = s;
 }
 
-__global__ __launch_bounds__(256) void to_bf16_rows(uint16_t *out, long ld, const float *part, int parts, long stride, int rows, int cols) {
-    for (int r = blockIdx.y; r < rows; r += gridDim.y)
-        for (int j = blockIdx.x * 256 + threadIdx.x; j < cols; j += gridDim.x * 256) {
-            float s = 0.f;
-            for (int p = 0; p < parts; ++p) s += part[p * stride + (size_t)r * cols + j];
-            store_any(out + r * ld + j, s);
-        }
-}
-
-// ---------------------------------------------------------------- fp32: pieces of logits in the workspace
-// A workgroup per dense row folds a piece into the row's running maximum and sum.
-__global__ __launch_bounds__(256) void fold_piece(const float *z, long ld, int cols, int first, Rows rows, float2 *run, float *picked) {
-    __shared__ float2 waves[4];
-    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (row >= *rows.count) return;
-    const float *p = z + row * ld;
-    float top = -__builtin_inff();
-    for (int j = threadIdx.x; j < cols; j += 256) top = fmaxf(top, p[j]);
-    const float from = top == -__builtin_inff() ? 0.f : top;
-    float sum = 0.f;
-    for (int j = threadIdx.x; j < cols; j += 256) sum += expf(p[j] - from);
-    float2 s = make_float2(top, sum);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s = join(s, make_float2(__shfl_xor(s.x, off), __shfl_xor(s.y, off)));
-    if (lane == 0) waves[wave] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s = join(join(waves[0], waves[1]), join(waves[2], waves[3]));
-        run[row] = first ? join(run[row], s) : s;
-        const int want = rows.sel[row] - first;
-        if (want >= 0 && want < cols) picked[row] = p[want];
-    }
-}
-
-// z -> dz in place, zeros for the rows behind the dense ones
-__global__ __launch_bounds__(256) void dz_piece(float *z, long ld, int cols, int first, int m, Rows rows, const float *lse, const float *grad) {
-    const int count = *rows.count;
-    for (int r = blockIdx.y; r < m; r += gridDim.y) {
-        const bool in = r < count;
-        const float l = in ? lse[r] : 0.f, g = in ? grad[r] : 0.f;
-        const int want = in ? rows.sel[r] - first : -1;
-        for (int j = blockIdx.x * 256 + threadIdx.x; j < cols; j += gridDim.x * 256) {
-            const float p = in ? expf(z[r * ld + j] - l) : 0.f;
-            z[r * ld + j] = in ? g * (j == want ? p - 1.f : p) : 0.f;
-        }
-    }
-}
-
-__global__ __launch_bounds__(256) void add_into(float *acc, const float *x, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) acc[i] += x[i];
-}
-
-dim3 rows_grid(int rows, long cols) {
-    const unsigned x = ceil_div(cols, 256);
-    return dim3(x > 64 ? 64 : x, rows < 32768 ? rows : 32768);
-}
-
+// ---------------------------------------------------------------- the calls
 template <class T>
 int check(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb, const int *selected) {
     if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
     if (m && !selected) return fail(SWC_HIP_EINVAL, "%s: selected is null", who);
     if (m && n && k && (!a || !b)) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
     if (m && n && k && (lda < k || ldb < n)) return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
-    if (sizeof(T) == 2 && (lda > kMaxLd || ldb > kMaxLd || round8(k) > kMaxLd || round8(n) > kMaxLd))
-        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd);
+    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || row_length<T>(k) > kMaxLd<T> || row_length<T>(n) > kMaxLd<T>)
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
+    if (m && n && k == 0) return fail(SWC_HIP_EINVAL, "%s: k is 0", who);
+    constexpr int kMaxRows = 65535 * kSumRows;
+    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
     return SWC_HIP_OK;
 }
 
@@ -345,55 +284,55 @@ Rows take_rows(Carver &c, int m) {
 }
 
 // Whole rows of the contraction: the epilogues of this file need finished sums.
-Plan whole_plan(int m, int n, int k) { return plan_product(m, n, k, true); }
+template <class T> Plan whole_plan(int m, int n, int k) { return plan_product<T>(m, n, k, true); }
 int block_columns(const Plan &p) { return p.kind == kThin || p.kind == kSmall ? 32 : 64; }
 static_assert(Big::TN == 2 && Mid::TN == 2 && Low::TN == 2 && Small::TN == 1 && Thin::TN == 1, "columns of a wavefront");
 
-// ---------------------------------------------------------------- spaces
-struct ForwardSpace {
+template <class T> struct ForwardSpace {
     Rows rows;
-    uint16_t *a, *b;
+    T *a, *b;
     float2 *part;
     float *picked;
     size_t bytes;
 };
-ForwardSpace forward_space(char *base, const Plan &p, int m, int n, int k, bool pack_b) {
+template <class T> ForwardSpace<T> forward_space(char *base, const Plan &p, int m, int n, int k, bool pack_b) {
     Carver c{base};
-    ForwardSpace s{};
+    ForwardSpace<T> s{};
     s.rows = take_rows(c, m);
-    s.a = c.take<uint16_t>((size_t)m * round8(k));
-    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
+    s.a = c.take<T>((size_t)m * row_length<T>(k));
+    s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.part = c.take<float2>((size_t)m * ((n + block_columns(p) - 1) / block_columns(p)));
     s.picked = c.take<float>(m);
     s.bytes = c.used;
     return s;
 }
 
-// Classes per piece of the gradients' dz: 256 MiB of it.
+// Classes per piece of the gradients' dz: 256 MiB of it.  Fewer would make dA's sums travel more often (at 8192 x 4096 the
+// 268 MB of them cost a twelfth of a piece of 4096 classes), more gain nothing.
 int piece_columns(int m, int n, size_t bytes) {
     size_t p = ((size_t)256 << 20) / bytes / m / 256 * 256;
     if (p < 256) p = 256;
     return p < (size_t)n ? (int)p : n;
 }
 
-struct GradSpace {
+template <class T> struct GradSpace {
     Rows rows;
-    uint16_t *a, *b, *dz;
+    T *a, *b, *dz;
     float *lse, *grad, *da, *part, *sums;
     int piece;
     Plan pa, pb;
     size_t bytes;
 };
-GradSpace grad_space(char *base, int m, int n, int k, bool pack_b, bool da, bool db, bool dbias) {
+template <class T> GradSpace<T> grad_space(char *base, int m, int n, int k, bool pack_b, bool da, bool db, bool dbias) {
     Carver c{base};
-    GradSpace s{};
-    s.piece = piece_columns(m, n, 2);
-    s.pa = plan_product(m, k, s.piece);
-    s.pb = plan_product(k, s.piece, m);
+    GradSpace<T> s{};
+    s.piece = piece_columns(m, n, sizeof(T));
+    s.pa = plan_product<T>(m, k, s.piece);
+    s.pb = plan_product<T>(k, s.piece, m);
     s.rows = take_rows(c, m);
-    s.a = c.take<uint16_t>((size_t)m * round8(k));
-    s.b = pack_b ? c.take<uint16_t>((size_t)k * round8(n)) : nullptr;
-    s.dz = c.take<uint16_t>((size_t)m * round8(s.piece));
+    s.a = c.take<T>((size_t)m * row_length<T>(k));
+    s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
+    s.dz = c.take<T>((size_t)m * row_length<T>(s.piece));
     s.lse = c.take<float>(m);
     s.grad = c.take<float>(m);
     s.da = da ? c.take<float>((size_t)s.pa.splits * m * k) : nullptr;
@@ -403,63 +342,33 @@ GradSpace grad_space(char *base, int m, int n, int k, bool pack_b, bool da, bool
     return s;
 }
 
-struct SpaceF {
-    Rows rows;
-    float *a, *z, *picked, *lse, *grad, *da, *tmp, *at, *bt, *part, *sums;
-    float2 *run;
-    int piece;
-    size_t partials, bytes;
-};
-SpaceF space_f(char *base, int m, int n, int k, bool gradients, bool da, bool db, bool dbias) {
-    Carver c{base};
-    SpaceF s{};
-    s.piece = piece_columns(m, n, 4);
-    const int tail = n % s.piece;   // the last piece has a plan of its own
-    s.partials = 0;
-    for (int p : {s.piece, tail}) {
-        if (!p) continue;
-        const size_t need[3] = {swc_hip_gemm_workspace_bytes(m, p, k), da ? swc_hip_gemm_workspace_bytes(m, k, p) : 0,
-                                db ? swc_hip_gemm_workspace_bytes(k, p, m) : 0};
-        for (size_t x : need) s.partials = x > s.partials ? x : s.partials;
+template <class T>
+int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb_, const T *bias, const int *selected,
+            float *row_loss, float *lse, float *loss) {
+    if (int rc = check(who, m, n, k, a, lda, b, ldb_, selected)) return rc;
+    if (!loss || (m && (!row_loss || !lse))) return fail(SWC_HIP_EINVAL, "%s: null output", who);
+    if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
+    if (m == 0 || n == 0) {   // no rows, or no classes: every row is left out
+        if (int rc = zero_rows(row_loss, m, m ? 1 : 0, m)) return rc;
+        if (int rc = zero_rows(lse, m, m ? 1 : 0, m)) return rc;
+        return zero_rows(loss, 1, 1, 1);
     }
-    s.rows = take_rows(c, m);
-    s.a = c.take<float>((size_t)m * k);
-    s.z = c.take<float>((size_t)m * s.piece);
-    s.part = c.take<float>(s.partials / sizeof(float) + 1);
-    if (!gradients) {
-        s.run = c.take<float2>(m);
-        s.picked = c.take<float>(m);
-    } else {
-        s.lse = c.take<float>(m);
-        s.grad = c.take<float>(m);
-        s.da = da ? c.take<float>((size_t)m * k) : nullptr;
-        s.tmp = da && s.piece < n ? c.take<float>((size_t)m * k) : nullptr;
-        s.bt = da ? c.take<float>((size_t)k * s.piece) : nullptr;
-        s.at = db ? c.take<float>((size_t)m * k) : nullptr;
-        s.sums = dbias ? c.take<float>((size_t)((m + kSumRows - 1) / kSumRows) * s.piece) : nullptr;
-    }
-    s.bytes = c.used;
-    return s;
-}
-
-// ---------------------------------------------------------------- the calls
-int forward_bf16(const char *who, int m, int n, int k, const uint16_t *a, long lda, const uint16_t *b, long ldb,
-                 const uint16_t *bias, const int *selected, float *row_loss, float *lse, float *loss) {
-    const Plan p = whole_plan(m, n, k);
+    long ldb = ldb_;
+    const Plan p = whole_plan<T>(m, n, k);
     const bool pack_b = !aligned_rows(b, ldb);
-    char *base = static_cast<char *>(workspace(forward_space(nullptr, p, m, n, k, pack_b).bytes, who));
+    char *base = static_cast<char *>(workspace(forward_space<T>(nullptr, p, m, n, k, pack_b).bytes, who));
     if (!base) return fail_code();
-    const ForwardSpace w = forward_space(base, p, m, n, k, pack_b);
+    const ForwardSpace<T> w = forward_space<T>(base, p, m, n, k, pack_b);
     pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, row_loss, lse);
     SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, w.rows.index, w.rows.count)) return rc;
+    if (int rc = copy_rows<T>(w.a, row_length<T>(k), a, lda, m, k, w.rows.index, w.rows.count)) return rc;
     if (pack_b) {
-        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = round8(n);
+        if (int rc = copy_rows<T>(w.b, row_length<T>(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = row_length<T>(n);
     }
     const int blocks = (n + block_columns(p) - 1) / block_columns(p);
-    const Shape s{w.a, b, round8(k), ldb, m, n, k, 0, w.rows.count};
-    if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats{w.part, blocks, w.picked, w.rows.sel, bias}, who)) return rc;
+    const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, w.rows.count};
+    if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias}, who)) return rc;
     join_rows<<<ceil_div(m, 4), 256, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse);
     SWC_LAUNCH_CHECK();
     mean_loss<<<1, 1024, 0, stream()>>>(row_loss, w.rows, loss);
@@ -467,154 +376,15 @@ int forward_bf16(const char *who, int m, int n, int k, const uint16_t *a, long l
     return SWC_HIP_OK;
 }
 
-__global__ __launch_bounds__(256) void finish_run(const float2 *run, const float *picked, Rows rows, float *row_loss, float *lse) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= *rows.count) return;
-    const float2 s = run[i];
-    const float l = (s.x == -__builtin_inff() ? 0.f : s.x) + logf(s.y);
-    lse[rows.index[i]] = l;
-    row_loss[rows.index[i]] = l - picked[i];
-}
-
-int forward_f32(const char *who, int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
-                const int *selected, float *row_loss, float *lse, float *loss) {
-    char *base = static_cast<char *>(workspace(space_f(nullptr, m, n, k, false, false, false, false).bytes, who));
-    if (!base) return fail_code();
-    const SpaceF w = space_f(base, m, n, k, false, false, false, false);
-    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, row_loss, lse);
-    SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows_f32(w.a, k, a, lda, m, k, w.rows.index, w.rows.count)) return rc;
-    for (int first = 0; first < n; first += w.piece) {
-        const int cols = n - first < w.piece ? n - first : w.piece;
-        if (int rc = gemm_f32(who, m, cols, k, w.a, k, b + first, ldb, bias ? bias + first : nullptr, w.z, cols, 0, w.part, w.partials))
-            return rc;
-        fold_piece<<<m, 256, 0, stream()>>>(w.z, cols, cols, first, w.rows, w.run, w.picked);
-        SWC_LAUNCH_CHECK();
-    }
-    finish_run<<<ceil_div(m, 256), 256, 0, stream()>>>(w.run, w.picked, w.rows, row_loss, lse);
-    SWC_LAUNCH_CHECK();
-    mean_loss<<<1, 1024, 0, stream()>>>(row_loss, w.rows, loss);
-    SWC_LAUNCH_CHECK();
-    return SWC_HIP_OK;
-}
-
-int grad_bf16(const char *who, int m, int n, int k, const uint16_t *a, long lda, const uint16_t *b, long ldb, const uint16_t *bias,
-              const int *selected, const float *lse, const float *row_grad, uint16_t *da, long ldda, uint16_t *db, long lddb,
-              uint16_t *dbias) {
-    const bool pack_b = !aligned_rows(b, ldb) || (da && n % 8);
-    char *base = static_cast<char *>(workspace(grad_space(nullptr, m, n, k, pack_b, da, db, dbias).bytes, who));
-    if (!base) return fail_code();
-    const GradSpace w = grad_space(base, m, n, k, pack_b, da, db, dbias);
-    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, nullptr, nullptr);
-    SWC_LAUNCH_CHECK();
-    gather_row_values<<<ceil_div(m, 256), 256, 0, stream()>>>(lse, row_grad, w.rows, w.lse, w.grad);
-    SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows_bf16(w.a, round8(k), a, lda, m, k, w.rows.index, w.rows.count)) return rc;
-    if (pack_b) {
-        if (int rc = copy_rows_bf16(w.b, round8(n), b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = round8(n);
-    }
-    for (int first = 0; first < n; first += w.piece) {
-        const int cols = n - first < w.piece ? n - first : w.piece;
-        const long ld = round8(cols);
-        const Shape z{w.a, b + first, round8(k), ldb, m, cols, k, 0, w.rows.count};
-        const StoreDz ep{w.dz, ld, first, w.rows.sel, w.lse, w.grad, bias ? bias + first : nullptr};
-        if (int rc = run_product<kAlongK, kAcross>(whole_plan(m, cols, k), z, ep, who)) return rc;
-        if (da) {
-            const Shape s{w.dz, b + first, ld, ldb, m, k, cols, 0, w.rows.count};
-            if (int rc = run_product<kAlongK, kAlongK>(w.pa, s, StorePartial{w.da, (long)m * k, k, first > 0}, who)) return rc;
-        }
-        if (db) {
-            const Shape s{w.a, w.dz, round8(k), ld, k, cols, m, 0, w.rows.count};
-            if (w.pb.splits == 1) {
-                const StoreBf16 out{db + first, lddb, aligned_rows(db + first, lddb)};
-                if (int rc = run_product<kAcross, kAcross>(w.pb, s, out, who)) return rc;
-            } else {
-                if (int rc = run_product<kAcross, kAcross>(w.pb, s, StorePartial{w.part, (long)k * cols, cols, false}, who)) return rc;
-                to_bf16_rows<<<rows_grid(k, cols), 256, 0, stream()>>>(db + first, lddb, w.part, w.pb.splits, (long)k * cols, k, cols);
-                SWC_LAUNCH_CHECK();
-            }
-        }
-        if (dbias) {
-            const int parts = (m + kSumRows - 1) / kSumRows;
-            column_sums<uint16_t><<<dim3(ceil_div(cols, 256), parts), 256, 0, stream()>>>(w.dz, ld, cols, w.rows, w.sums);
-            SWC_LAUNCH_CHECK();
-            if (int rc = sum_parts(dbias + first, nullptr, w.sums, parts, cols)) return rc;
-        }
-    }
-    return da ? launch_spread(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place) : (int)SWC_HIP_OK;
-}
-
-int grad_f32(const char *who, int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
-             const int *selected, const float *lse, const float *row_grad, float *da, int ldda, float *db, int lddb, float *dbias) {
-    char *base = static_cast<char *>(workspace(space_f(nullptr, m, n, k, true, da, db, dbias).bytes, who));
-    if (!base) return fail_code();
-    const SpaceF w = space_f(base, m, n, k, true, da, db, dbias);
-    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, nullptr, nullptr);
-    SWC_LAUNCH_CHECK();
-    gather_row_values<<<ceil_div(m, 256), 256, 0, stream()>>>(lse, row_grad, w.rows, w.lse, w.grad);
-    SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows_f32(w.a, k, a, lda, m, k, w.rows.index, w.rows.count)) return rc;
-    if (db)
-        if (int rc = swc_hip_matrixTrans_f(m, k, w.a, k, w.at, m)) return rc;
-    for (int first = 0; first < n; first += w.piece) {
-        const int cols = n - first < w.piece ? n - first : w.piece;
-        if (int rc = gemm_f32(who, m, cols, k, w.a, k, b + first, ldb, bias ? bias + first : nullptr, w.z, cols, 0, w.part, w.partials))
-            return rc;
-        dz_piece<<<rows_grid(m, cols), 256, 0, stream()>>>(w.z, cols, cols, first, m, w.rows, w.lse, w.grad);
-        SWC_LAUNCH_CHECK();
-        if (da) {
-            float *to = first ? w.tmp : w.da;
-            if (int rc = swc_hip_matrixTrans_f(k, cols, b + first, ldb, w.bt, k)) return rc;
-            if (int rc = gemm_f32(who, m, k, cols, w.z, cols, w.bt, k, nullptr, to, k, 0, w.part, w.partials)) return rc;
-            if (first) {
-                const unsigned blocks = ceil_div((size_t)m * k, 256);
-                add_into<<<blocks > 8192 ? 8192 : blocks, 256, 0, stream()>>>(w.da, w.tmp, (size_t)m * k);
-                SWC_LAUNCH_CHECK();
-            }
-        }
-        if (db)
-            if (int rc = gemm_f32(who, k, cols, m, w.at, m, w.z, cols, nullptr, db + first, lddb, 0, w.part, w.partials)) return rc;
-        if (dbias) {
-            const int parts = (m + kSumRows - 1) / kSumRows;
-            column_sums<float><<<dim3(ceil_div(cols, 256), parts), 256, 0, stream()>>>(w.z, cols, cols, w.rows, w.sums);
-            SWC_LAUNCH_CHECK();
-            if (int rc = sum_parts(nullptr, dbias + first, w.sums, parts, cols)) return rc;
-        }
-    }
-    return da ? launch_spread(da, ldda, w.da, 1, 0, m, k, w.rows.place) : (int)SWC_HIP_OK;
-}
-
-constexpr int kMaxRows = 65535 * kSumRows;
-
-template <class T, class F>
-int forward(const char *who, F call, int m, int n, int k, const T *a, int lda, const T *b, int ldb, const T *bias,
-            const int *selected, float *row_loss, float *lse, float *loss) {
-    if (int rc = check(who, m, n, k, a, lda, b, ldb, selected)) return rc;
-    if (!loss || (m && (!row_loss || !lse))) return fail(SWC_HIP_EINVAL, "%s: null output", who);
-    if (m && k == 0 && n) return fail(SWC_HIP_EINVAL, "%s: k is 0", who);
-    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
-    if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
-    if (m == 0) return swc_hip_fill_f(loss, 0.f, 1);
-    if (n == 0) {   // no classes: every row is left out
-        if (int rc = swc_hip_fill_f(row_loss, 0.f, m)) return rc;
-        if (int rc = swc_hip_fill_f(lse, 0.f, m)) return rc;
-        return swc_hip_fill_f(loss, 0.f, 1);
-    }
-    return call(who, m, n, k, a, lda, b, ldb, bias, selected, row_loss, lse, loss);
-}
-
-template <class T, class F>
-int gradients(const char *who, F call, int m, int n, int k, const T *a, int lda, const T *b, int ldb, const T *bias,
-              const int *selected, const float *lse, const float *row_grad, T *da, int ldda, T *db, int lddb, T *dbias) {
-    if (int rc = check(who, m, n, k, a, lda, b, ldb, selected)) return rc;
+template <class T>
+int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb_, const T *bias, const int *selected,
+              const float *lse, const float *row_grad, T *da, int ldda, T *db, int lddb, T *dbias) {
+    if (int rc = check(who, m, n, k, a, lda, b, ldb_, selected)) return rc;
     if (m && !lse) return fail(SWC_HIP_EINVAL, "%s: lse is null", who);
     if ((da && ldda < k) || (db && lddb < n)) return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
     const void *in[3] = {a, b, bias};
     for (const void *p : in)
         if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
-    if (m && n && k == 0) return fail(SWC_HIP_EINVAL, "%s: k is 0", who);
-    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
     if (!da && !db && !dbias) return SWC_HIP_OK;
     if (m == 0 || n == 0) {
@@ -622,7 +392,49 @@ int gradients(const char *who, F call, int m, int n, int k, const T *a, int lda,
         if (int rc = zero_rows(db, lddb, k, n)) return rc;
         return zero_rows(dbias, n, 1, n);
     }
-    return call(who, m, n, k, a, lda, b, ldb, bias, selected, lse, row_grad, da, ldda, db, lddb, dbias);
+    long ldb = ldb_;
+    const bool pack_b = !aligned_rows(b, ldb) || (da && n % kChunk<T>);
+    char *base = static_cast<char *>(workspace(grad_space<T>(nullptr, m, n, k, pack_b, da, db, dbias).bytes, who));
+    if (!base) return fail_code();
+    const GradSpace<T> w = grad_space<T>(base, m, n, k, pack_b, da, db, dbias);
+    const long ldw = row_length<T>(k);
+    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, nullptr, nullptr);
+    SWC_LAUNCH_CHECK();
+    gather_row_values<<<ceil_div(m, 256), 256, 0, stream()>>>(lse, row_grad, w.rows, w.lse, w.grad);
+    SWC_LAUNCH_CHECK();
+    if (int rc = copy_rows<T>(w.a, ldw, a, lda, m, k, w.rows.index, w.rows.count)) return rc;
+    if (pack_b) {
+        if (int rc = copy_rows<T>(w.b, row_length<T>(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        b = w.b, ldb = row_length<T>(n);
+    }
+    for (int first = 0; first < n; first += w.piece) {
+        const int cols = n - first < w.piece ? n - first : w.piece;
+        const long ld = row_length<T>(cols);
+        const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, w.rows.count};
+        const StoreDz<T> ep{w.dz, ld, first, w.rows.sel, w.lse, w.grad, bias ? bias + first : nullptr};
+        if (int rc = run_product<kAlongK, kAcross>(whole_plan<T>(m, cols, k), z, ep, who)) return rc;
+        if (da) {
+            const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, w.rows.count};
+            if (int rc = run_product<kAlongK, kAlongK>(w.pa, s, StorePartial{w.da, (long)m * k, k, first > 0}, who)) return rc;
+        }
+        if (db) {
+            const Shape<T> s{w.a, w.dz, ldw, ld, k, cols, m, 0, w.rows.count};
+            if (w.pb.splits == 1) {
+                const Store<T> out{db + first, lddb, aligned_rows(db + first, lddb)};
+                if (int rc = run_product<kAcross, kAcross>(w.pb, s, out, who)) return rc;
+            } else {
+                if (int rc = run_product<kAcross, kAcross>(w.pb, s, StorePartial{w.part, (long)k * cols, cols, false}, who)) return rc;
+                if (int rc = join_parts<T>(db + first, lddb, w.part, w.pb.splits, k, cols)) return rc;
+            }
+        }
+        if (dbias) {
+            const int parts = (m + kSumRows - 1) / kSumRows;
+            column_sums<T><<<dim3(ceil_div(cols, 256), parts), 256, 0, stream()>>>(w.dz, ld, cols, w.rows, w.sums);
+            SWC_LAUNCH_CHECK();
+            if (int rc = sum_parts<T>(dbias + first, w.sums, parts, cols)) return rc;
+        }
+    }
+    return da ? launch_spread(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place) : (int)SWC_HIP_OK;
 }
 
 } // namespace
@@ -631,36 +443,38 @@ extern "C" {
 
 int swc_hip_matrixFCSoftmaxWithLoss_f(int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
                                       const int *selected, float *rowLoss, float *lse, float *loss) {
-    return forward("swc_hip_matrixFCSoftmaxWithLoss_f", forward_f32, m, n, k, a, lda, b, ldb, bias, selected, rowLoss, lse, loss);
+    return forward<float>("swc_hip_matrixFCSoftmaxWithLoss_f", m, n, k, a, lda, b, ldb, bias, selected, rowLoss, lse, loss);
 }
 
 int swc_hip_matrixFCSoftmaxWithLoss_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda, const swc_hip_bf16 *b, int ldb,
                                        const swc_hip_bf16 *bias, const int *selected, float *rowLoss, float *lse, float *loss) {
-    return forward("swc_hip_matrixFCSoftmaxWithLoss_bf", forward_bf16, m, n, k, a, lda, b, ldb, bias, selected, rowLoss, lse, loss);
+    return forward<bf16>("swc_hip_matrixFCSoftmaxWithLoss_bf", m, n, k, a, lda, b, ldb, bias, selected, rowLoss, lse, loss);
 }
 
 size_t swc_hip_matrixFCSoftmaxWithLoss_workspace_bytes(int m, int n, int k, int bf) {
     if (!ready() || m <= 0 || n <= 0 || k <= 0) return 0;
-    return bf ? forward_space(nullptr, whole_plan(m, n, k), m, n, k, true).bytes : space_f(nullptr, m, n, k, false, false, false, false).bytes;
+    return bf ? forward_space<bf16>(nullptr, whole_plan<bf16>(m, n, k), m, n, k, true).bytes
+              : forward_space<float>(nullptr, whole_plan<float>(m, n, k), m, n, k, true).bytes;
 }
 
 int swc_hip_matrixFCSoftmaxWithLossGrad_f(int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
                                           const int *selected, const float *lse, const float *rowGrad, float *aGrad, int ldag,
                                           float *bGrad, int ldbg, float *biasGrad) {
-    return gradients("swc_hip_matrixFCSoftmaxWithLossGrad_f", grad_f32, m, n, k, a, lda, b, ldb, bias, selected, lse, rowGrad, aGrad,
-                     ldag, bGrad, ldbg, biasGrad);
+    return gradients<float>("swc_hip_matrixFCSoftmaxWithLossGrad_f", m, n, k, a, lda, b, ldb, bias, selected, lse, rowGrad, aGrad,
+                            ldag, bGrad, ldbg, biasGrad);
 }
 
 int swc_hip_matrixFCSoftmaxWithLossGrad_bf(int m, int n, int k, const swc_hip_bf16 *a, int lda, const swc_hip_bf16 *b, int ldb,
                                            const swc_hip_bf16 *bias, const int *selected, const float *lse, const float *rowGrad,
                                            swc_hip_bf16 *aGrad, int ldag, swc_hip_bf16 *bGrad, int ldbg, swc_hip_bf16 *biasGrad) {
-    return gradients("swc_hip_matrixFCSoftmaxWithLossGrad_bf", grad_bf16, m, n, k, a, lda, b, ldb, bias, selected, lse, rowGrad,
-                     aGrad, ldag, bGrad, ldbg, biasGrad);
+    return gradients<bf16>("swc_hip_matrixFCSoftmaxWithLossGrad_bf", m, n, k, a, lda, b, ldb, bias, selected, lse, rowGrad, aGrad,
+                           ldag, bGrad, ldbg, biasGrad);
 }
 
 size_t swc_hip_matrixFCSoftmaxWithLossGrad_workspace_bytes(int m, int n, int k, int bf) {
     if (!ready() || m <= 0 || n <= 0 || k <= 0) return 0;
-    return bf ? grad_space(nullptr, m, n, k, true, true, true, true).bytes : space_f(nullptr, m, n, k, true, true, true, true).bytes;
+    return bf ? grad_space<bf16>(nullptr, m, n, k, true, true, true, true).bytes
+              : grad_space<float>(nullptr, m, n, k, true, true, true, true).bytes;
 }
 
 } // extern "C"

@@ -883,11 +883,6 @@ int swc_hip::gemm_noalloc_setup(int device) {
     return SWC_HIP_OK;
 }
 
-int swc_hip::gemm_f32(const char *who, int m, int n, int k, const float *a, int lda, const float *b, int ldb, const float *bias,
-                      float *c, int ldc, int relu, float *part, size_t part_bytes) {
-    return gemm_dispatch(who, m, n, k, a, lda, b, ldb, bias, c, ldc, relu, 0, PartialStore{part, part_bytes});
-}
-
 extern "C" {
 
 int swc_hip_matrixMatrixMul_f(int m, int n, int k, const float *a, int lda, const float *b, int ldb, float *c,

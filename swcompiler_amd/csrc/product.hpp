@@ -1,0 +1,144 @@
+// Which tiles a product of the language-model operators takes, and what their callers share: padded copies of operands
+// whose rows do not start on 16-byte boundaries, and the joining of partial sums of a product cut along its contraction.
+#pragma once
+#include "product_tile.hpp"
+
+namespace swc_hip {
+namespace product {
+
+using Big = Cfg<4, 2, 2, 4, 3, 2>;    // 256 x 256, eight wavefronts, one workgroup per CU
+using Deep = Cfg<4, 4, 2, 2, 3, 2>;   // 256 x 256, four wavefronts of 128 x 128: a third less LDS traffic, a longer end
+using Mid = Cfg<2, 2, 2, 2, 3, 2>;    // 128 x 128, four wavefronts, two workgroups per CU
+using Low = Cfg<1, 2, 2, 2, 3, 3>;    // 64 x 128, two
+using Small = Cfg<1, 1, 2, 2, 3, 3>;  // 64 x 64, three
+using Thin = Cfg<1, 1, 1, 4, 4, 4>;   // 32 x 128, two: few rows, the other operand streams
+
+enum Kind { kBig, kDeep, kMid, kLow, kSmall, kThin };
+struct Plan {
+    Kind kind;
+    int splits, k_per_split;
+    size_t partial_bytes(int m, int n) const { return splits > 1 ? (size_t)splits * m * n * sizeof(float) : 0; }
+};
+
+// most memory the partial sums of one product may take
+constexpr size_t kMaxPartials = (size_t)256 << 20;
+
+// The tile and the number of ranges of the contraction with the least estimated time (microseconds):
+//     start and end of a workgroup, f, for each round of the chip
+//   + slices * max(the time of a slice alone on a CU, workgroups per CU * its share of a busy CU)
+//   + the output at 4.5 TB/s, and for a cut contraction the joining kernel: 4 us and the partial sums again.
+// The bf16 constants are fits to 10 shapes of 128-2048 x 1024-4096 x 512-50264 at 1 to 32 ranges.  What the model chooses
+// there, and the other side measured: 333 x 1411 x 1003 7.0 us (64 x 64 whole; 128 x 128 in four ranges 8.3 and the
+// joining), 512 x 4096 x 4096 24.4 (64 x 128 whole; 128 x 128 in two 23.0 and the joining), 2048 x 4096 x 4096 63.5 (128 x
+// 128; 256 x 256 83.2), 1400 x 1024 x 50264 175 (256 x 256 in eight; 128 x 128 in four 250).  An fp32 slice is half as many
+// products at a sixteenth of the rate: the matrix cores set its time.
+// one: only whole contractions.
+template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
+    struct Tile {
+        Kind kind;
+        int bm, bn, per_cu;
+        double f, alone, busy;
+    };
+    static constexpr Tile kBf16Tiles[] = {{kBig, 256, 256, 1, 10.8, 0.89, 1.2}, {kMid, 128, 128, 2, 4.3, 0.43, 0.46},
+                                          {kLow, 64, 128, 2, 4.3, 0.275, 0.32}, {kSmall, 64, 64, 3, 3.3, 0.225, 0.2},
+                                          {kThin, 32, 128, 2, 3.0, 0.2, 0.16}};
+    static constexpr Tile kFp32Tiles[] = {{kBig, 256, 256, 1, 12, 7.2, 7.2}, {kMid, 128, 128, 2, 5, 2.0, 1.83},
+                                          {kLow, 64, 128, 2, 4.5, 1.05, 0.95}, {kSmall, 64, 64, 3, 3.5, 0.55, 0.48},
+                                          {kThin, 32, 128, 2, 3.0, 0.55, 0.5}};
+    constexpr int kPer = kSlice<T>, E = sizeof(T);
+    const int cus = num_cus();
+    const int slices = k > 0 ? (k + kPer - 1) / kPer : 1;
+    const double operands = (double)E * ((double)m * k + (double)n * k) / 5e6;
+    Plan best{kMid, 1, slices * kPer};
+    double least = 1e30;
+    for (const Tile &t : kIsBf16<T> ? kBf16Tiles : kFp32Tiles) {
+        if ((t.kind == kThin) != (m <= 32)) continue;
+        const long tiles = (long)((m + t.bm - 1) / t.bm) * ((n + t.bn - 1) / t.bn);
+        for (int splits = 1; splits <= 64 && splits <= slices; splits += splits < 4 ? 1 : splits < 16 ? 2 : 8) {
+            const int each = (slices + splits - 1) / splits, s = (slices + each - 1) / each;
+            if (s > 1 && (one || each < 4 || (size_t)s * m * n * sizeof(float) > kMaxPartials)) break;
+            const double groups = (double)tiles * s;
+            const double q = groups <= cus ? 1 : groups >= 4.0 * t.per_cu * cus ? groups / cus : (double)((long)((groups + cus - 1) / cus));
+            const double rounds = q <= t.per_cu ? 1 : q / t.per_cu;
+            double work = each * (t.alone > q * t.busy ? t.alone : q * t.busy);
+            work = work > operands ? work : operands;
+            const double mn = (double)m * n;
+            const double cost = rounds * t.f + work + (s > 1 ? 4 + 8 * s * mn / 4.5e6 : E * mn / 4.5e6);
+            if (cost < least) least = cost, best = Plan{t.kind, s, each * kPer};
+        }
+    }
+    // one wavefront per SIMD pays where the end of a tile is a small part of it: bf16 8192^3 785 -> 757 us, K = 4096 412 -> 417
+    if (best.kind == kBig && kIsBf16<T> && best.k_per_split >= 6144) best.kind = kDeep;
+    return best;
+}
+
+// The epilogues with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
+// wavefront per SIMD has nothing beside it while they run; those without kThinToo never run on 32-row tiles.
+template <Layout LA, Layout LB, class T, class Ep>
+int run_product(const Plan &p, const Shape<T> &s, const Ep &ep, const char *who) {
+    Shape<T> t = s;
+    t.k_per_split = p.k_per_split;
+    if constexpr (!Ep::kHeavy && kIsBf16<T>)
+        if (p.kind == kDeep) return launch_product<T, Deep, LA, LB>(t, p.splits, ep, who);
+    if constexpr (Ep::kThinToo)
+        if (p.kind == kThin) return launch_product<T, Thin, LA, LB>(t, p.splits, ep, who);
+    switch (p.kind) {
+    case kMid: return launch_product<T, Mid, LA, LB>(t, p.splits, ep, who);
+    case kLow: return launch_product<T, Low, LA, LB>(t, p.splits, ep, who);
+    case kSmall: return launch_product<T, Small, LA, LB>(t, p.splits, ep, who);
+    default: return launch_product<T, Big, LA, LB>(t, p.splits, ep, who);
+    }
+}
+
+// what the loads take: rows on 16-byte boundaries
+template <class T> bool aligned_rows(const T *p, long ld) { return aligned16(p) && ld % kChunk<T> == 0; }
+template <class T> long row_length(long cols) { return (cols + kChunk<T> - 1) / kChunk<T> * kChunk<T>; }
+
+// A workspace handed out in 256-byte steps; with a null base it only counts.
+struct Carver {
+    char *base;
+    size_t used = 0;
+    template <class T> T *take(size_t count) {
+        const size_t at = used;
+        used += (count * sizeof(T) + 255) & ~(size_t)255;
+        return base ? reinterpret_cast<T *>(base + at) : nullptr;
+    }
+};
+
+// an element in fp32, whichever the type
+__device__ __forceinline__ float load_any(const uint16_t *p) { return __builtin_bit_cast(float, (unsigned)*p << 16); }
+__device__ __forceinline__ float load_any(const float *p) { return *p; }
+__device__ __forceinline__ void store_any(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store_any(uint16_t *p, float x) {
+#if __HIP_DEVICE_COMPILE__
+    *p = __builtin_bit_cast(uint16_t, (__bf16)x);
+#endif
+}
+
+inline unsigned grid_of(size_t n) {
+    const size_t b = (n + 255) / 256;
+    return (unsigned)(b > 16384 ? 16384 : b);
+}
+
+template <class T> __global__ __launch_bounds__(256) void fill_rows(T *p, long ld, int rows, int cols) {
+    const size_t total = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) p[(i / cols) * ld + i % cols] = T(0);
+}
+template <class T> int zero_rows(T *p, long ld, int rows, int cols) {
+    if (!p || !rows || !cols) return SWC_HIP_OK;
+    fill_rows<T><<<grid_of((size_t)rows * cols), 256, 0, stream()>>>(p, ld, rows, cols);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+// dst[r][0..ld) = src[index ? index[r] : r][0..cols) and zeros behind; rows at or beyond *count (when given) become
+// zeros.  dst: rows on 16-byte boundaries.
+template <class T> int copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index, const int *count);
+// out[m][n] (rows of ld) = the sum of `parts` matrices, in order
+template <class T> int join_parts(T *out, long ld, const float *part, int parts, int m, int n);
+// out[j] = sum over parts p of part[p][j], in a fixed order
+template <class T> int sum_parts(T *out, const float *part, int parts, int n);
+
+} // namespace product
+
+} // namespace swc_hip
