@@ -19,7 +19,6 @@ template <class T, int ACT> struct FcEpilogue {
     const T *bias, *residual;
     T *preact, *c;
     long ldr, ldp, ldc;
-    bool vec;   // every matrix given has 16-byte aligned rows, and the bias can be read four elements at a time
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void end(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -32,112 +31,83 @@ template <class T, int ACT> struct FcEpilogue {
             const int row = row0 + P::row(tm, l32);
             const bool ok = row < m;
             // a row's second summand is requested together, before its first use
-            if (residual) r.template load<WHOLE>(residual + row * ldr, ok, col0, n, vec, h);
+            if (residual) r.template load<WHOLE>(residual + row * ldr, ok, col0, n, h);
             float z[P::kValues], x[P::kValues];
 #pragma unroll
             for (int u = 0; u < P::kValues; ++u) z[u] = P::value(acc[tm], u) + (bias ? b.value(u) : 0.f);
-            if (preact) store_row<P, WHOLE>(preact + row * ldp, ok, col0, n, vec, h, z);
+            if (preact) store_row<P, WHOLE>(preact + row * ldp, ok, col0, n, h, z);
             if (residual) r.get(x);
 #pragma unroll
             for (int u = 0; u < P::kValues; ++u) z[u] = act_value<ACT, kIsBf16<T>>(z[u]) + (residual ? x[u] : 0.f);
-            store_row<P, WHOLE>(c + row * ldc, ok, col0, n, vec, h, z);
+            store_row<P, WHOLE>(c + row * ldc, ok, col0, n, h, z);
         }
     }
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
-        if (vec && row0 + 32 * TM <= m && col0 + 32 * TN <= n) end<P, true>(acc, row0, col0, m, n, lane);
+        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n) end<P, true>(acc, row0, col0, m, n, lane);
         else end<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
 
 // The end of a layer from fp32 sums: `parts` matrices of m x n to be added in order, then bias, activation, residual.
-// Four columns of a row a thread; VEC: rows of sums on 16-byte boundaries.
-template <class T, int ACT, bool VEC>
-__global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long ldpart, long part_stride, const T *bias,
-                                                 const T *residual, long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
+// Four columns of a row a thread.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long part_stride, const T *bias, const T *residual,
+                                                 long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
 #if __HIP_DEVICE_COMPILE__
     const int j = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
     if (j >= n) return;
+    const int have = n - j < 4 ? n - j : 4;
     float b[4] = {};
-    if (bias)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = j + e < n ? load_any(bias + j + e) : 0.f;
+    if (bias) load4(bias + j, have, b);
     for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < m; r += gridDim.y * 4) {
         float z[4] = {}, x[4] = {};
-        const float *p = part + r * ldpart + j;
-        if (residual)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = j + e < n ? load_any(residual + r * ldr + j + e) : 0.f;
+        const float *p = part + (long)r * n + j;
+        if (residual) load4(residual + r * ldr + j, have, x);
 #pragma unroll 8
         for (int i = 0; i < parts; ++i) {
-            if (VEC) {
-                const float4 d = *reinterpret_cast<const float4 *>(p + i * part_stride);
-                z[0] += d.x, z[1] += d.y, z[2] += d.z, z[3] += d.w;
-            } else {
+            float d[4];
+            load4(p + i * part_stride, have, d);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] += j + e < n ? p[i * part_stride + e] : 0.f;
-            }
+            for (int e = 0; e < 4; ++e) z[e] += d[e];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (j + e >= n) continue;
-            z[e] += b[e];
-            if (preact) store_any(preact + r * ldp + j + e, z[e]);
-            store_any(c + r * ldc + j + e, act_value<ACT, kIsBf16<T>>(z[e]) + x[e]);
-        }
+        for (int e = 0; e < 4; ++e) z[e] += b[e];
+        if (preact) store4(preact + r * ldp + j, have, z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = act_value<ACT, kIsBf16<T>>(z[e]) + x[e];
+        store4(c + r * ldc + j, have, z);
     }
 #endif
 }
 template <class T>
-int launch_finish(int act, const float *part, int parts, long ldpart, long part_stride, const T *bias, const T *residual, long ldr,
-                  T *preact, long ldp, T *c, long ldc, int m, int n) {
+int launch_finish(int act, const float *part, int parts, const T *bias, const T *residual, long ldr, T *preact, long ldp, T *c, long ldc,
+                  int m, int n) {
     const unsigned rows = ceil_div(m, 4);
     const dim3 grid(ceil_div(n, 256), rows > 16384 ? 16384 : rows);
-    const bool vec = aligned16(part) && ldpart % 4 == 0 && part_stride % 4 == 0 && n % 4 == 0;
     return with_act(act, [&]<int ACT>() {
-        if (vec) fc_finish<T, ACT, true><<<grid, 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact, ldp, c, ldc, m, n);
-        else fc_finish<T, ACT, false><<<grid, 256, 0, stream()>>>(part, parts, ldpart, part_stride, bias, residual, ldr, preact, ldp, c, ldc, m, n);
+        fc_finish<T, ACT><<<grid, 256, 0, stream()>>>(part, parts, (long)m * n, bias, residual, ldr, preact, ldp, c, ldc, m, n);
         SWC_LAUNCH_CHECK();
         return (int)SWC_HIP_OK;
     });
 }
 
-// Rows into a copy whose rows start on 16-byte boundaries, zeros behind their end and in the rows that do not exist:
-// 16 bytes a thread.  A source at any alignment is read in the two aligned 16-byte pieces that hold the thread's eight
-// values (each of them holds at least one that exists, so neither leaves the allocation's pages), shifted together.
-__device__ __forceinline__ uint4 eight_at(const bf16 *p, int have) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    const uint4 *q = reinterpret_cast<const uint4 *>(at & ~(uintptr_t)15);
-    const int shift = (int)(at & 15) * 8;
-    const uint4 lo = q[0], hi = shift / 16 + have > 8 ? q[1] : make_uint4(0, 0, 0, 0);
-    typedef unsigned __int128 u128;
-    const u128 l = (u128)(((uint64_t)lo.y << 32) | lo.x) | ((u128)(((uint64_t)lo.w << 32) | lo.z) << 64);
-    const u128 h = (u128)(((uint64_t)hi.y << 32) | hi.x) | ((u128)(((uint64_t)hi.w << 32) | hi.z) << 64);
-    u128 v = shift ? (l >> shift) | (h << (128 - shift)) : l;
-    if (have < 8) v &= ((u128)1 << (16 * have)) - 1;
-    const uint64_t a = (uint64_t)v, b = (uint64_t)(v >> 64);
-    return make_uint4((unsigned)a, (unsigned)(a >> 32), (unsigned)b, (unsigned)(b >> 32));
+// Rows into copies whose rows start on 16-byte boundaries, zeros behind their end: 16 bytes a thread, both operands of a
+// product in one launch.
+template <class T> __device__ __forceinline__ void copy_chunk(const Copy<T> &c, long row, long j) {
+    *reinterpret_cast<v4u *>(c.dst + row * c.ld + j) = chunk_at(c.src + row * c.lds + j, c.cols - j);
 }
-__device__ __forceinline__ uint4 chunk_at(const bf16 *p, long have) { return eight_at(p, have < 8 ? (int)have : 8); }
-__device__ __forceinline__ uint4 chunk_at(const float *p, long have) {
-    if (have >= 4 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) return *reinterpret_cast<const uint4 *>(p);
-    unsigned v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = e < have ? __builtin_bit_cast(unsigned, p[e]) : 0u;
-    return make_uint4(v[0], v[1], v[2], v[3]);
-}
-template <class T>
-__global__ __launch_bounds__(256) void copy_chunks(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index,
-                                                   const int *count) {
-    const int have = count ? *count : rows;
-    const long j = ((long)blockIdx.x * 256 + threadIdx.x) * kChunk<T>;
-    if (j >= ld) return;
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < have && j < cols) v = chunk_at(src + (index ? index[r] : r) * lds + j, cols - j);
-        *reinterpret_cast<uint4 *>(dst + r * ld + j) = v;
+template <class T> __global__ __launch_bounds__(256) void copy_chunks(Copy<T> a, Copy<T> b, long chunks_a, long chunks) {
+#if __HIP_DEVICE_COMPILE__
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (long)gridDim.x * 256) {
+        const bool first = i < chunks_a;
+        const long per = (first ? a.ld : b.ld) / kChunk<T>, at = first ? i : i - chunks_a;
+        const long row = at / per, j = (at - row * per) * kChunk<T>;
+        if (first) copy_chunk(a, row, j);
+        else copy_chunk(b, row, j);
     }
+#endif
 }
 
 // 32 columns and eight ranges of the parts a workgroup: a range's parts are added in order, then the ranges in order.
@@ -197,7 +167,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda_, const T 
     if (int rc = check_forward(who, m, n, k, a, lda_, b, ldb_, act, residual, ldr, preact, ldp, c, ldc)) return rc;
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
     if (m == 0 || n == 0) return SWC_HIP_OK;
-    if (k == 0) return launch_finish<T>(act, nullptr, 0, 0, 0, bias, residual, ldr, preact, ldp, c, ldc, m, n);
+    if (k == 0) return launch_finish<T>(act, nullptr, 0, bias, residual, ldr, preact, ldp, c, ldc, m, n);
     long lda = lda_, ldb = ldb_;
     const Plan p = plan_product<T>(m, n, k);
     const bool pack_a = !aligned_rows(a, lda) || k % kChunk<T>, pack_b = !aligned_rows(b, ldb);
@@ -208,24 +178,18 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda_, const T 
         if (!base) return fail_code();
         w = space<T>(base, p, m, n, k, pack_a, pack_b);
     }
-    if (pack_a) {
-        if (int rc = copy_rows<T>(w.a, row_length<T>(k), a, lda, m, k, nullptr, nullptr)) return rc;
-        a = w.a, lda = row_length<T>(k);
-    }
-    if (pack_b) {
-        if (int rc = copy_rows<T>(w.b, row_length<T>(n), b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = row_length<T>(n);
-    }
+    if (int rc = copy_operands<T>({pack_a ? w.a : nullptr, a, row_length<T>(k), lda, m, k}, {pack_b ? w.b : nullptr, b, row_length<T>(n), ldb, k, n}))
+        return rc;
+    if (pack_a) a = w.a, lda = row_length<T>(k);
+    if (pack_b) b = w.b, ldb = row_length<T>(n);
     const Shape<T> s{a, b, lda, ldb, m, n, k, 0, nullptr};
     if (!partial_sums(p)) {
-        const bool vec = (!residual || aligned_rows(residual, ldr)) && (!preact || aligned_rows(preact, ldp)) && aligned_rows(c, ldc) &&
-                         reinterpret_cast<uintptr_t>(bias) % (4 * sizeof(T)) == 0;
         return with_act(act, [&]<int ACT>() {
-            return run_product<kAlongK, kAcross>(p, s, FcEpilogue<T, ACT>{bias, residual, preact, c, ldr, ldp, ldc, vec}, who);
+            return run_product<kAlongK, kAcross>(p, s, FcEpilogue<T, ACT>{bias, residual, preact, c, ldr, ldp, ldc}, who);
         });
     }
     if (int rc = run_product<kAlongK, kAcross>(p, s, StorePartial{w.part, (long)m * n, n, false}, who)) return rc;
-    return launch_finish<T>(act, w.part, p.splits, n, (long)m * n, bias, residual, ldr, preact, ldp, c, ldc, m, n);
+    return launch_finish<T>(act, w.part, p.splits, bias, residual, ldr, preact, ldp, c, ldc, m, n);
 }
 
 } // namespace
@@ -233,15 +197,15 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda_, const T 
 namespace swc_hip {
 namespace product {
 
-template <class T> int copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index, const int *count) {
-    if (!rows || !ld) return SWC_HIP_OK;
-    copy_chunks<T><<<dim3(ceil_div(ld / kChunk<T>, 256), rows < 32768 ? rows : 32768), 256, 0, stream()>>>(dst, ld, src, lds, rows, cols,
-                                                                                                          index, count);
+template <class T> int copy_operands(const Copy<T> &a, const Copy<T> &b) {
+    const long na = a.dst ? a.rows * (a.ld / kChunk<T>) : 0, nb = b.dst ? b.rows * (b.ld / kChunk<T>) : 0;
+    if (!(na + nb)) return SWC_HIP_OK;
+    copy_chunks<T><<<grid_of(na + nb), 256, 0, stream()>>>(a, b, na, na + nb);
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
 template <class T> int join_parts(T *out, long ld, const float *part, int parts, int m, int n) {
-    return launch_finish<T>(SWC_HIP_ACT_NONE, part, parts, n, (long)m * n, nullptr, nullptr, 0, nullptr, 0, out, ld, m, n);
+    return launch_finish<T>(SWC_HIP_ACT_NONE, part, parts, nullptr, nullptr, 0, nullptr, 0, out, ld, m, n);
 }
 template <class T> int sum_parts(T *out, const float *part, int parts, int n) {
     if (!n) return SWC_HIP_OK;
@@ -249,8 +213,8 @@ template <class T> int sum_parts(T *out, const float *part, int parts, int n) {
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
-template int copy_rows<bf16>(bf16 *, long, const bf16 *, long, int, int, const int *, const int *);
-template int copy_rows<float>(float *, long, const float *, long, int, int, const int *, const int *);
+template int copy_operands<bf16>(const Copy<bf16> &, const Copy<bf16> &);
+template int copy_operands<float>(const Copy<float> &, const Copy<float> &);
 template int join_parts<bf16>(bf16 *, long, const float *, int, int, int);
 template int join_parts<float>(float *, long, const float *, int, int, int);
 template int sum_parts<bf16>(bf16 *, const float *, int, int);

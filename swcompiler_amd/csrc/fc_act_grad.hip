@@ -14,69 +14,48 @@ using namespace swc_hip::product;
 namespace {
 
 // dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of kSumRows rows' column sums of the unrounded
-// values.  32 threads side by side hold eight columns each, eight rows at a time; VEC: 16 bytes of a row at once.
+// values.  64 threads side by side hold four columns each, four rows at a time.
 constexpr int kSumRows = 32;
-template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int j, int n, float (&x)[8]) {
-    if constexpr (VEC && kIsBf16<T>) {
-        const uint4 d = *reinterpret_cast<const uint4 *>(p + j);
-        const unsigned w[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-    } else if constexpr (VEC) {
-        const float4 a = *reinterpret_cast<const float4 *>(p + j), b = *reinterpret_cast<const float4 *>(p + j + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = j + e < n ? load_any(p + j + e) : 0.f;
-    }
-}
-template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int j, int n, const float (&x)[8]) {
-#if __HIP_DEVICE_COMPILE__
-    if constexpr (VEC && kIsBf16<T>) {
-        *reinterpret_cast<uint4 *>(p + j) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-    } else if constexpr (VEC) {
-        *reinterpret_cast<float4 *>(p + j) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(p + j + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (j + e < n) store_any(p + j + e, x[e]);
-    }
-#endif
-}
-
-template <class T, int ACT, bool VEC>
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums) {
 #if __HIP_DEVICE_COMPILE__
-    __shared__ float part[8][257];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int j = (blockIdx.x * 32 + tx) * 8;
+    __shared__ float part[4][256];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int j = (blockIdx.x * 64 + tx) * 4;
     const int r0 = blockIdx.y * kSumRows;
     const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
-    float sum[8] = {};
-    if (j < (n > ld ? n : ld))
-#pragma unroll 2
-        for (int r = r0 + ty; r < r1; r += 8) {
-            float g[8];
-            load8<T, VEC>(dc + r * ldc, j, n, g);
+    const int have = n - j;
+    float sum[4] = {};
+    if (have > 0) {
+#pragma unroll 4
+        for (int r = r0 + ty; r < r1; r += 4) {
+            float g[4];
+            load4(dc + r * ldc + j, have, g);
             if constexpr (ACT != SWC_HIP_ACT_NONE) {
-                float y[8];
-                load8<T, VEC>(z + r * ldz, j, n, y);
+                float y[4];
+                load4(z + r * ldz + j, have, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT, kIsBf16<T>>(y[e]);
+                for (int e = 0; e < 4; ++e) g[e] *= act_slope<ACT, kIsBf16<T>>(y[e]);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += j + e < n ? g[e] : 0.f;
-            if (dz) store8<T, VEC>(dz + r * ld, j, (int)ld, g);
+            for (int e = 0; e < 4; ++e) {
+                if (e >= have) g[e] = 0.f;
+                sum[e] += g[e];
+            }
+            if (dz) store4(dz + r * ld + j, (int)ld - j, g);
         }
+    } else if (dz && j < ld) {   // the rest of the padding
+        const float none[4] = {};
+        for (int r = r0 + ty; r < r1; r += 4) store4(dz + r * ld + j, (int)ld - j, none);
+    }
     if (!sums) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
+    for (int e = 0; e < 4; ++e) part[ty][tx * 4 + e] = sum[e];
     __syncthreads();
     const int col = blockIdx.x * 256 + threadIdx.x;
     float s = 0.f;
 #pragma unroll
-    for (int y = 0; y < 8; ++y) s += part[y][threadIdx.x];
+    for (int y = 0; y < 4; ++y) s += part[y][threadIdx.x];
     if (col < n) sums[(size_t)blockIdx.y * n + col] = s;
 #endif
 }
@@ -106,12 +85,8 @@ int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz
     if (!dz) ld = 0;
     const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m));
     if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
-    constexpr int kPer = 16 / sizeof(T);
-    const bool vec = n % 8 == 0 && aligned16(dc) && lddc % kPer == 0 && (act == SWC_HIP_ACT_NONE || (aligned16(z) && ldz % kPer == 0)) &&
-                     (!dz || (aligned16(dz) && ld % kPer == 0));
     return with_act(act, [&]<int ACT>() {
-        if (vec) act_grad<T, ACT, true><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
-        else act_grad<T, ACT, false><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
         SWC_LAUNCH_CHECK();
         return (int)SWC_HIP_OK;
     });
@@ -140,7 +115,7 @@ size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 // one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
 template <Layout LA, Layout LB, class T>
 int grad_product(const char *who, const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
-    if (p.splits == 1) return run_product<LA, LB>(p, s, Store<T>{out, ld, aligned_rows(out, ld)}, who);
+    if (p.splits == 1) return run_product<LA, LB>(p, s, Store<T>{out, ld}, who);
     if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
     return join_parts<T>(out, ld, part, p.splits, s.m, s.n);
 }
@@ -179,14 +154,10 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
     }
     const T *dz = own_dz ? w.dz : dc;
     const long lddz = own_dz ? padded : lddc;
-    if (pack_b) {
-        if (int rc = copy_rows<T>(w.b, padded, b, ldb, k, n, nullptr, nullptr)) return rc;
-        b = w.b, ldb = padded;
-    }
-    if (pack_a) {
-        if (int rc = copy_rows<T>(w.a, row_length<T>(k), a, lda, m, k, nullptr, nullptr)) return rc;
-        a = w.a, lda = row_length<T>(k);
-    }
+    if (int rc = copy_operands<T>({pack_a ? w.a : nullptr, a, row_length<T>(k), lda, m, k}, {pack_b ? w.b : nullptr, b, padded, ldb, k, n}))
+        return rc;
+    if (pack_a) a = w.a, lda = row_length<T>(k);
+    if (pack_b) b = w.b, ldb = padded;
     if (da)
         if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, {dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
     if (db)

@@ -22,23 +22,42 @@ using namespace swc_hip::product;
 
 namespace {
 
-// The rows that count, in order.
+// The rows that count, in order, with what the gradients need of each.
 struct Rows {
     int *index;    // dense row -> row
     int *place;    // row -> dense row, -1 if left out
     int *sel;      // class of a dense row
     int *count;
+    float *lse, *grad;   // of a dense row (gradients only)
 };
+// What the rows come with: lse and row_grad (may be null) are read for the gradients, row_loss and lse_out of the rows left
+// out are set to 0 for the forward call.
+struct RowsFrom {
+    const int *selected;
+    int m, n;
+    const float *lse, *row_grad;
+    float *row_loss, *lse_out;
+};
+__device__ __forceinline__ void take_row(const RowsFrom &from, const Rows &to, int r, bool in, int at, int sel) {
+    to.place[r] = in ? at : -1;
+    if (in) {
+        to.index[at] = r, to.sel[at] = sel;
+        if (from.lse) to.lse[at] = from.lse[r], to.grad[at] = from.row_grad ? from.row_grad[r] : 1.f;
+    } else if (from.row_loss) {
+        from.row_loss[r] = 0.f, from.lse_out[r] = 0.f;
+    }
+}
 
+// Many rows: one workgroup numbers them, then copy_dense.
 constexpr int kPickThreads = 1024;
-__global__ __launch_bounds__(kPickThreads) void pick_rows(const int *selected, int m, int n, Rows out, float *row_loss, float *lse) {
+__global__ __launch_bounds__(kPickThreads) void pick_rows(RowsFrom from, Rows to) {
     __shared__ int waves[kPickThreads / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int base = 0;
-    for (int r0 = 0; r0 < m; r0 += kPickThreads) {
+    for (int r0 = 0; r0 < from.m; r0 += kPickThreads) {
         const int r = r0 + threadIdx.x;
-        const int sel = r < m ? selected[r] : -1;
-        const bool in = sel >= 0 && sel < n;
+        const int sel = r < from.m ? from.selected[r] : -1;
+        const bool in = sel >= 0 && sel < from.n;
         const unsigned long long mask = __ballot(in);
         if (lane == 0) waves[wave] = __popcll(mask);
         __syncthreads();
@@ -47,16 +66,62 @@ __global__ __launch_bounds__(kPickThreads) void pick_rows(const int *selected, i
             before += w < wave ? waves[w] : 0;
             all += waves[w];
         }
-        if (r < m) {
-            const int at = before + __popcll(mask & ((1ull << lane) - 1));
-            out.place[r] = in ? at : -1;
-            if (in) out.index[at] = r, out.sel[at] = sel;
-            else if (row_loss) row_loss[r] = 0.f, lse[r] = 0.f;
-        }
+        if (r < from.m) take_row(from, to, r, in, before + __popcll(mask & ((1ull << lane) - 1)), sel);
         base = all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) *out.count = base;
+    if (threadIdx.x == 0) *to.count = base;
+}
+template <class T>
+__global__ __launch_bounds__(256) void copy_dense(const T *a, long lda, int k, T *dense, long ld, Rows rows) {
+#if __HIP_DEVICE_COMPILE__
+    const int count = *rows.count;
+    const long j = ((long)blockIdx.x * 256 + threadIdx.x) * kChunk<T>;
+    if (j >= ld) return;
+    for (int r = blockIdx.y; r < count; r += gridDim.y)
+        *reinterpret_cast<v4u *>(dense + r * ld + j) = chunk_at(a + rows.index[r] * lda + j, k - j);
+#endif
+}
+// Few rows: a workgroup per row counts the rows before its own and copies it, one launch instead of two.
+constexpr int kCountRows = 4096;
+template <class T>
+__global__ __launch_bounds__(256) void count_and_copy(RowsFrom from, Rows to, const T *a, long lda, int k, T *dense, long ld) {
+#if __HIP_DEVICE_COMPILE__
+    __shared__ int sums[2][4];
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0, all = 0;
+    for (int r0 = 0; r0 < from.m; r0 += 256) {
+        const int r = r0 + threadIdx.x;
+        const int sel = r < from.m ? from.selected[r] : -1;
+        const bool in = sel >= 0 && sel < from.n;
+        all += __popcll(__ballot(in));
+        before += __popcll(__ballot(in && r < row));
+    }
+    if (lane == 0) sums[0][wave] = before, sums[1][wave] = all;
+    __syncthreads();
+    const int at = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+    const int sel = from.selected[row];
+    const bool in = sel >= 0 && sel < from.n;
+    if (threadIdx.x == 0) {
+        take_row(from, to, row, in, at, sel);
+        if (row == 0) *to.count = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+    }
+    if (!in) return;
+    for (long j = threadIdx.x * kChunk<T>; j < ld; j += 256 * kChunk<T>)
+        *reinterpret_cast<v4u *>(dense + at * ld + j) = chunk_at(a + row * lda + j, k - j);
+#endif
+}
+template <class T> int gather_rows(const RowsFrom &from, const Rows &to, const T *a, long lda, int k, T *dense) {
+    const long ld = row_length<T>(k);
+    if (from.m <= kCountRows) {
+        count_and_copy<T><<<from.m, 256, 0, stream()>>>(from, to, a, lda, k, dense, ld);
+    } else {
+        pick_rows<<<1, kPickThreads, 0, stream()>>>(from, to);
+        SWC_LAUNCH_CHECK();
+        copy_dense<T><<<dim3(ceil_div(ld / kChunk<T>, 256), from.m < 32768 ? from.m : 32768), 256, 0, stream()>>>(a, lda, k, dense, ld, to);
+    }
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
 }
 
 // bf16: the exponential instruction (relative error |x| 2^-24 and a little); fp32: the library function
@@ -107,7 +172,7 @@ template <class T> struct RowStats {
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
         if (col0 >= n) return;
-        if (col0 + 32 * TN <= n && reinterpret_cast<uintptr_t>(bias) % (4 * sizeof(T)) == 0) reduce<P, true>(acc, row0, col0, m, n, lane);
+        if (col0 + 32 * TN <= n) reduce<P, true>(acc, row0, col0, m, n, lane);
         else reduce<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
@@ -118,30 +183,44 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
     return make_float2(top, a.y * expf(a.x - from) + b.y * expf(b.x - from));
 }
 
-// One wavefront per dense row joins its blocks.
-__global__ __launch_bounds__(256) void join_rows(const float2 *part, int blocks, const float *picked, Rows rows, float *row_loss,
-                                                 float *lse) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= *rows.count) return;
+// A wavefront joins a dense row's blocks -> the row's loss (in lane 0)
+__device__ __forceinline__ float join_row(int row, int lane, const float2 *part, int blocks, const float *picked, const Rows &rows,
+                                          float *row_loss, float *lse) {
     const float2 *p = part + (size_t)row * blocks;
     float2 s = make_float2(-__builtin_inff(), 0.f);
     for (int b = lane; b < blocks; b += 64) s = join(s, p[b]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s = join(s, make_float2(__shfl_xor(s.x, off), __shfl_xor(s.y, off)));
+    const float l = (s.x == -__builtin_inff() ? 0.f : s.x) + logf(s.y), loss = l - picked[row];
     if (lane == 0) {
-        const float l = (s.x == -__builtin_inff() ? 0.f : s.x) + logf(s.y);
         const int r = rows.index[row];
         lse[r] = l;
-        row_loss[r] = l - picked[row];
+        row_loss[r] = loss;
     }
+    return loss;
+}
+__global__ __launch_bounds__(256) void join_rows(const float2 *part, int blocks, const float *picked, Rows rows, float *row_loss,
+                                                 float *lse) {
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row < *rows.count) join_row(row, threadIdx.x & 63, part, blocks, picked, rows, row_loss, lse);
 }
 
-// *loss = mean over the dense rows, summed in double in a fixed order
-__global__ __launch_bounds__(1024) void mean_loss(const float *row_loss, Rows rows, float *loss) {
+// *loss = mean over the dense rows, summed in double in a fixed order; JOIN: joins the rows first (few rows: one launch)
+template <bool JOIN>
+__global__ __launch_bounds__(1024) void mean_loss(const float2 *part, int blocks, const float *picked, Rows rows, float *row_loss,
+                                                  float *lse, float *loss) {
     __shared__ double sums[1024];
     const int count = *rows.count;
     double s = 0;
-    for (int i = threadIdx.x; i < count; i += 1024) s += row_loss[rows.index[i]];
+    if (JOIN) {
+        const int lane = threadIdx.x & 63;
+        for (int i = threadIdx.x >> 6; i < count; i += 16) {
+            const float l = join_row(i, lane, part, blocks, picked, rows, row_loss, lse);
+            if (lane == 0) s += l;
+        }
+    } else {
+        for (int i = threadIdx.x; i < count; i += 1024) s += row_loss[rows.index[i]];
+    }
     sums[threadIdx.x] = s;
     __syncthreads();
     for (int off = 512; off > 0; off >>= 1) {
@@ -190,26 +269,17 @@ template <class T> struct StoreDz {
                 x[u] *= g;
                 if (!WHOLE && col0 + P::column(u, h) >= n) x[u] = 0.f;
             }
-            store_row<P, WHOLE>(dz + row * ld, ok, col0, (int)ld, true, h, x);
+            store_row<P, WHOLE>(dz + row * ld, ok, col0, (int)ld, h, x);
         }
     }
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
-        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n && reinterpret_cast<uintptr_t>(bias) % (4 * sizeof(T)) == 0)
+        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n)
             store<P, true>(acc, row0, col0, m, n, lane);
         else store<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
 };
-
-// lse and the upstream gradient of the dense rows
-__global__ __launch_bounds__(256) void gather_row_values(const float *lse, const float *grad, Rows rows, float *lse_out, float *grad_out) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= *rows.count) return;
-    const int r = rows.index[i];
-    lse_out[i] = lse[r];
-    grad_out[i] = grad ? grad[r] : 1.f;
-}
 
 // out[r] = sum of `parts` buffers' dense row of r, zeros for a row left out; four columns a thread where cols allow
 template <class T, bool VEC>
@@ -274,12 +344,13 @@ int check(const char *who, int m, int n, int k, const T *a, int lda, const T *b,
     return SWC_HIP_OK;
 }
 
-Rows take_rows(Carver &c, int m) {
-    Rows r;
+Rows take_rows(Carver &c, int m, bool gradients) {
+    Rows r{};
     r.index = c.take<int>(m);
     r.place = c.take<int>(m);
     r.sel = c.take<int>(m);
     r.count = c.take<int>(1);
+    if (gradients) r.lse = c.take<float>(m), r.grad = c.take<float>(m);
     return r;
 }
 
@@ -298,7 +369,7 @@ template <class T> struct ForwardSpace {
 template <class T> ForwardSpace<T> forward_space(char *base, const Plan &p, int m, int n, int k, bool pack_b) {
     Carver c{base};
     ForwardSpace<T> s{};
-    s.rows = take_rows(c, m);
+    s.rows = take_rows(c, m, false);
     s.a = c.take<T>((size_t)m * row_length<T>(k));
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.part = c.take<float2>((size_t)m * ((n + block_columns(p) - 1) / block_columns(p)));
@@ -318,7 +389,7 @@ int piece_columns(int m, int n, size_t bytes) {
 template <class T> struct GradSpace {
     Rows rows;
     T *a, *b, *dz;
-    float *lse, *grad, *da, *part, *sums;
+    float *da, *part, *sums;
     int piece;
     Plan pa, pb;
     size_t bytes;
@@ -329,12 +400,10 @@ template <class T> GradSpace<T> grad_space(char *base, int m, int n, int k, bool
     s.piece = piece_columns(m, n, sizeof(T));
     s.pa = plan_product<T>(m, k, s.piece);
     s.pb = plan_product<T>(k, s.piece, m);
-    s.rows = take_rows(c, m);
+    s.rows = take_rows(c, m, true);
     s.a = c.take<T>((size_t)m * row_length<T>(k));
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.dz = c.take<T>((size_t)m * row_length<T>(s.piece));
-    s.lse = c.take<float>(m);
-    s.grad = c.take<float>(m);
     s.da = da ? c.take<float>((size_t)s.pa.splits * m * k) : nullptr;
     s.part = db && s.pb.splits > 1 ? c.take<float>((size_t)s.pb.splits * k * s.piece) : nullptr;
     s.sums = dbias ? c.take<float>((size_t)((m + kSumRows - 1) / kSumRows) * s.piece) : nullptr;
@@ -359,19 +428,21 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
     char *base = static_cast<char *>(workspace(forward_space<T>(nullptr, p, m, n, k, pack_b).bytes, who));
     if (!base) return fail_code();
     const ForwardSpace<T> w = forward_space<T>(base, p, m, n, k, pack_b);
-    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, row_loss, lse);
-    SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows<T>(w.a, row_length<T>(k), a, lda, m, k, w.rows.index, w.rows.count)) return rc;
+    if (int rc = gather_rows<T>({selected, m, n, nullptr, nullptr, row_loss, lse}, w.rows, a, lda, k, w.a)) return rc;
     if (pack_b) {
-        if (int rc = copy_rows<T>(w.b, row_length<T>(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        if (int rc = copy_operands<T>({}, {w.b, b, row_length<T>(n), ldb, k, n})) return rc;
         b = w.b, ldb = row_length<T>(n);
     }
     const int blocks = (n + block_columns(p) - 1) / block_columns(p);
     const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, w.rows.count};
     if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias}, who)) return rc;
-    join_rows<<<ceil_div(m, 4), 256, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse);
-    SWC_LAUNCH_CHECK();
-    mean_loss<<<1, 1024, 0, stream()>>>(row_loss, w.rows, loss);
+    if (m <= 128) {
+        mean_loss<true><<<1, 1024, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse, loss);
+    } else {
+        join_rows<<<ceil_div(m, 4), 256, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse);
+        SWC_LAUNCH_CHECK();
+        mean_loss<false><<<1, 1024, 0, stream()>>>(nullptr, 0, nullptr, w.rows, row_loss, lse, loss);
+    }
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
@@ -398,20 +469,16 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
     if (!base) return fail_code();
     const GradSpace<T> w = grad_space<T>(base, m, n, k, pack_b, da, db, dbias);
     const long ldw = row_length<T>(k);
-    pick_rows<<<1, kPickThreads, 0, stream()>>>(selected, m, n, w.rows, nullptr, nullptr);
-    SWC_LAUNCH_CHECK();
-    gather_row_values<<<ceil_div(m, 256), 256, 0, stream()>>>(lse, row_grad, w.rows, w.lse, w.grad);
-    SWC_LAUNCH_CHECK();
-    if (int rc = copy_rows<T>(w.a, ldw, a, lda, m, k, w.rows.index, w.rows.count)) return rc;
+    if (int rc = gather_rows<T>({selected, m, n, lse, row_grad, nullptr, nullptr}, w.rows, a, lda, k, w.a)) return rc;
     if (pack_b) {
-        if (int rc = copy_rows<T>(w.b, row_length<T>(n), b, ldb, k, n, nullptr, nullptr)) return rc;
+        if (int rc = copy_operands<T>({}, {w.b, b, row_length<T>(n), ldb, k, n})) return rc;
         b = w.b, ldb = row_length<T>(n);
     }
     for (int first = 0; first < n; first += w.piece) {
         const int cols = n - first < w.piece ? n - first : w.piece;
         const long ld = row_length<T>(cols);
         const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, w.rows.count};
-        const StoreDz<T> ep{w.dz, ld, first, w.rows.sel, w.lse, w.grad, bias ? bias + first : nullptr};
+        const StoreDz<T> ep{w.dz, ld, first, w.rows.sel, w.rows.lse, w.rows.grad, bias ? bias + first : nullptr};
         if (int rc = run_product<kAlongK, kAcross>(whole_plan<T>(m, cols, k), z, ep, who)) return rc;
         if (da) {
             const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, w.rows.count};
@@ -420,7 +487,7 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
         if (db) {
             const Shape<T> s{w.a, w.dz, ldw, ld, k, cols, m, 0, w.rows.count};
             if (w.pb.splits == 1) {
-                const Store<T> out{db + first, lddb, aligned_rows(db + first, lddb)};
+                const Store<T> out{db + first, lddb};
                 if (int rc = run_product<kAcross, kAcross>(w.pb, s, out, who)) return rc;
             } else {
                 if (int rc = run_product<kAcross, kAcross>(w.pb, s, StorePartial{w.part, (long)k * cols, cols, false}, who)) return rc;

@@ -41,14 +41,14 @@ template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
     };
     static constexpr Tile kBf16Tiles[] = {{kBig, 256, 256, 1, 10.8, 0.89, 1.2}, {kMid, 128, 128, 2, 4.3, 0.43, 0.46},
                                           {kLow, 64, 128, 2, 4.3, 0.275, 0.32}, {kSmall, 64, 64, 3, 3.3, 0.225, 0.2},
-                                          {kThin, 32, 128, 2, 3.0, 0.2, 0.16}};
+                                          {kThin, 32, 128, 2, 3.0, 0.23, 0.16}};
     static constexpr Tile kFp32Tiles[] = {{kBig, 256, 256, 1, 12, 7.2, 7.2}, {kMid, 128, 128, 2, 5, 2.0, 1.83},
                                           {kLow, 64, 128, 2, 4.5, 1.05, 0.95}, {kSmall, 64, 64, 3, 3.5, 0.55, 0.48},
                                           {kThin, 32, 128, 2, 3.0, 0.55, 0.5}};
     constexpr int kPer = kSlice<T>, E = sizeof(T);
     const int cus = num_cus();
     const int slices = k > 0 ? (k + kPer - 1) / kPer : 1;
-    const double operands = (double)E * ((double)m * k + (double)n * k) / 5e6;
+    const double operands = (double)E * ((double)m * k + (double)n * k) / 9e6;   // (from the last-level cache)
     Plan best{kMid, 1, slices * kPer};
     double least = 1e30;
     for (const Tile &t : kIsBf16<T> ? kBf16Tiles : kFp32Tiles) {
@@ -131,9 +131,69 @@ template <class T> int zero_rows(T *p, long ld, int rows, int cols) {
     return SWC_HIP_OK;
 }
 
-// dst[r][0..ld) = src[index ? index[r] : r][0..cols) and zeros behind; rows at or beyond *count (when given) become
-// zeros.  dst: rows on 16-byte boundaries.
-template <class T> int copy_rows(T *dst, long ld, const T *src, long lds, int rows, int cols, const int *index, const int *count);
+#if __HIP_DEVICE_COMPILE__
+// `have` (at least one) elements from any address, zeros behind them: four in fp32, or 16 bytes as they are
+__device__ __forceinline__ void load4(const bf16 *p, int have, float (&x)[4]) {
+    if (have >= 4) {
+        const v2u d = *reinterpret_cast<const At<bf16>::four *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? d[e / 2] & 0xffff0000u : d[e / 2] << 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = e < have ? load_any(p + e) : 0.f;
+    }
+}
+__device__ __forceinline__ void load4(const float *p, int have, float (&x)[4]) {
+    if (have >= 4) {
+        const v4f d = *reinterpret_cast<const At<float>::four *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = d[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = e < have ? p[e] : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(bf16 *p, int have, const float (&x)[4]) {
+    if (have >= 4) {
+        *reinterpret_cast<At<bf16>::four *>(p) = v2u{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < have) store_any(p + e, x[e]);
+    }
+}
+__device__ __forceinline__ void store4(float *p, int have, const float (&x)[4]) {
+    if (have >= 4) {
+        *reinterpret_cast<At<float>::four *>(p) = v4f{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < have) p[e] = x[e];
+    }
+}
+template <class T> __device__ __forceinline__ v4u chunk_at(const T *p, long have) {
+    if (have >= kChunk<T>) return __builtin_bit_cast(v4u, *reinterpret_cast<const typename At<T>::chunk *>(p));
+    v4u d = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e)
+        if (e < have) {
+            if constexpr (kIsBf16<T>) d[e / 2] |= (unsigned)p[e] << (16 * (e & 1));
+            else d[e] = __builtin_bit_cast(unsigned, p[e]);
+        }
+    return d;
+}
+#endif
+
+// dst[r][0..ld) = src[r][0..cols) and zeros behind; dst null: nothing to copy.  dst: rows on 16-byte boundaries, ld =
+// row_length(cols).
+template <class T> struct Copy {
+    T *dst;
+    const T *src;
+    long ld, lds;
+    int rows, cols;
+};
+// both operands of a product, in one launch
+template <class T> int copy_operands(const Copy<T> &a, const Copy<T> &b);
 // out[m][n] (rows of ld) = the sum of `parts` matrices, in order
 template <class T> int join_parts(T *out, long ld, const float *part, int parts, int m, int n);
 // out[j] = sum over parts p of part[p][j], in a fixed order

@@ -385,10 +385,21 @@ __device__ __forceinline__ unsigned pack_bf16(float x, float y) {
     return __builtin_bit_cast(unsigned, v);
 }
 
+// Vectors at any element's address: one memory instruction (the target takes unaligned global accesses).
+template <class T> struct At;
+template <> struct At<bf16> {
+    typedef v4u chunk __attribute__((aligned(2)));
+    typedef v2u four __attribute__((aligned(2)));
+};
+template <> struct At<float> {
+    typedef v4f chunk __attribute__((aligned(4)));
+    typedef v4f four __attribute__((aligned(4)));
+};
+
 // A lane's part of a row of C (or of a matrix of its shape) to and from memory, `row` the address of the row's first
-// column and col0 the wavefront's first.  Every lane of the wavefront calls these; ok: its row exists; vec: rows start on
-// 16-byte boundaries.  WHOLE: the row exists with all the wavefront's columns, and vec (the path without control flow: a
-// branch per row makes the compiler wait for every store before it).
+// column and col0 the wavefront's first.  Every lane of the wavefront calls these; ok: its row exists.  WHOLE: the row
+// exists with all the wavefront's columns (the path without control flow: a branch per row makes the compiler wait for
+// every store before it).
 //
 // bf16: the sixteen values of a 32-column block are dealt out again between the half-waves, so that lane h holds columns
 // 16 q + 8 h .. + 7 of it: 16-byte accesses.
@@ -398,7 +409,7 @@ __device__ __forceinline__ void half_waves_swap(unsigned &lo, unsigned &hi) {   
 }
 
 template <class P, bool WHOLE>
-__device__ __forceinline__ void store_row(bf16 *row, bool ok, int col0, int n, bool vec, int h, const float (&x)[P::kValues]) {
+__device__ __forceinline__ void store_row(bf16 *row, bool ok, int col0, int n, int h, const float (&x)[P::kValues]) {
 #pragma unroll
     for (int b = 0; b < P::kValues / 16; ++b)
 #pragma unroll
@@ -408,8 +419,8 @@ __device__ __forceinline__ void store_row(bf16 *row, bool ok, int col0, int n, b
             half_waves_swap(d[0], d[2]);
             half_waves_swap(d[1], d[3]);
             const int c = col0 + 32 * b + 16 * q + 8 * h;
-            if (WHOLE || (ok && vec && c + 8 <= n)) {
-                *reinterpret_cast<v4u *>(row + c) = v4u{d[0], d[1], d[2], d[3]};
+            if (WHOLE || (ok && c + 8 <= n)) {
+                *reinterpret_cast<At<bf16>::chunk *>(row + c) = v4u{d[0], d[1], d[2], d[3]};
             } else if (ok) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -418,12 +429,12 @@ __device__ __forceinline__ void store_row(bf16 *row, bool ok, int col0, int n, b
         }
 }
 template <class P, bool WHOLE>
-__device__ __forceinline__ void store_row(float *row, bool ok, int col0, int n, bool vec, int h, const float (&x)[P::kValues]) {
+__device__ __forceinline__ void store_row(float *row, bool ok, int col0, int n, int h, const float (&x)[P::kValues]) {
 #pragma unroll
     for (int q = 0; q < P::kGroups; ++q) {
         const int c = col0 + P::col(q, h);
-        if (WHOLE || (ok && vec && c + 4 <= n)) {
-            *reinterpret_cast<v4f *>(row + c) = v4f{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        if (WHOLE || (ok && c + 4 <= n)) {
+            *reinterpret_cast<At<float>::chunk *>(row + c) = v4f{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
         } else if (ok) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -436,21 +447,17 @@ __device__ __forceinline__ void store_row(float *row, bool ok, int col0, int n, 
 template <class T, class P> struct RowData;
 template <class P> struct RowData<bf16, P> {
     v4u d[P::kValues / 8];
-    template <bool WHOLE> __device__ __forceinline__ void load(const bf16 *row, bool ok, int col0, int n, bool vec, int h) {
+    template <bool WHOLE> __device__ __forceinline__ void load(const bf16 *row, bool ok, int col0, int n, int h) {
 #pragma unroll
         for (int i = 0; i < P::kValues / 8; ++i) {
             const int c = col0 + 16 * i + 8 * h;
-            if constexpr (WHOLE) {
-                d[i] = *reinterpret_cast<const v4u *>(row + c);
+            if (WHOLE || (ok && c + 8 <= n)) {
+                d[i] = *reinterpret_cast<const At<bf16>::chunk *>(row + c);
             } else {
                 d[i] = v4u{0, 0, 0, 0};
-                if (ok && vec && c + 8 <= n) {
-                    d[i] = *reinterpret_cast<const v4u *>(row + c);
-                } else if (ok) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < n) d[i][e / 2] |= (unsigned)row[c + e] << (16 * (e & 1));
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (ok && c + e < n) d[i][e / 2] |= (unsigned)row[c + e] << (16 * (e & 1));
             }
         }
     }
@@ -467,12 +474,12 @@ template <class P> struct RowData<bf16, P> {
 };
 template <class P> struct RowData<float, P> {
     v4f d[P::kGroups];
-    template <bool WHOLE> __device__ __forceinline__ void load(const float *row, bool ok, int col0, int n, bool vec, int h) {
+    template <bool WHOLE> __device__ __forceinline__ void load(const float *row, bool ok, int col0, int n, int h) {
 #pragma unroll
         for (int q = 0; q < P::kGroups; ++q) {
             const int c = col0 + P::col(q, h);
-            if constexpr (WHOLE) {
-                d[q] = *reinterpret_cast<const v4f *>(row + c);
+            if (WHOLE || (ok && c + 4 <= n)) {
+                d[q] = *reinterpret_cast<const At<float>::chunk *>(row + c);
             } else {
                 d[q] = v4f{0, 0, 0, 0};
 #pragma unroll
@@ -487,8 +494,7 @@ template <class P> struct RowData<float, P> {
     }
 };
 
-// The values a lane needs of a vector over the columns (bias), as loaded.  WHOLE: all columns exist and the vector's start
-// allows loads of four elements.
+// The values a lane needs of a vector over the columns (bias), as loaded.  WHOLE: all columns exist.
 template <class T, class P> struct ColumnData {
     typedef std::conditional_t<kIsBf16<T>, v2u, v4f> four;
     four d[P::kGroups];
@@ -496,8 +502,8 @@ template <class T, class P> struct ColumnData {
 #pragma unroll
         for (int q = 0; q < P::kGroups; ++q) {
             const int c = col0 + P::col(q, h);
-            if constexpr (WHOLE) {
-                d[q] = *reinterpret_cast<const four *>(v + c);
+            if (WHOLE || c + 4 <= n) {
+                d[q] = *reinterpret_cast<const typename At<T>::four *>(v + c);
             } else {
                 d[q] = four{};
 #pragma unroll
@@ -556,12 +562,11 @@ __global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) 
 #endif
 }
 
-// The matrix of the product in its type, rows 16-byte aligned or not.
+// The matrix of the product in its type.
 template <class T> struct Store {
     static constexpr bool kHeavy = false, kThinToo = true;
     T *out;
     long ld;
-    bool vec;
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -572,12 +577,12 @@ template <class T> struct Store {
             float x[P::kValues];
 #pragma unroll
             for (int u = 0; u < P::kValues; ++u) x[u] = P::value(acc[tm], u);
-            store_row<P, WHOLE>(out + row * ld, row < m, col0, n, vec, h, x);
+            store_row<P, WHOLE>(out + row * ld, row < m, col0, n, h, x);
         }
     }
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int) const {
-        if (vec && row0 + 32 * TM <= m && col0 + 32 * TN <= n) store<P, true>(acc, row0, col0, m, n, lane);
+        if (row0 + 32 * TM <= m && col0 + 32 * TN <= n) store<P, true>(acc, row0, col0, m, n, lane);
         else store<P, false>(acc, row0, col0, m, n, lane);
     }
 #endif
@@ -594,7 +599,6 @@ struct StorePartial {
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int split) const {
         const int l32 = lane & 31, h = lane >> 5;
-        const bool vec = (ld & 3) == 0;   // (the buffer itself starts on a 256-byte boundary)
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int row = row0 + P::row(tm, l32);
@@ -604,8 +608,8 @@ struct StorePartial {
             for (int q = 0; q < P::kGroups; ++q) {
                 const int col = col0 + P::col(q, h);
                 v4f x = {P::value(acc[tm], 4 * q), P::value(acc[tm], 4 * q + 1), P::value(acc[tm], 4 * q + 2), P::value(acc[tm], 4 * q + 3)};
-                if (vec && col + 4 <= n) {
-                    v4f *o = reinterpret_cast<v4f *>(p + col);
+                if (col + 4 <= n) {
+                    auto *o = reinterpret_cast<At<float>::chunk *>(p + col);
                     *o = add ? *o + x : x;
                 } else {
 #pragma unroll
