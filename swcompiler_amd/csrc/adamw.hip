@@ -47,7 +47,6 @@ struct Tensor {
 };
 struct Tensor8 : Tensor {
     float *mom_scale, *var_scale;
-    bool aligned;   // every pointer on the boundary of four of its elements
 };
 // (the tables fill the 4 KiB that kernel arguments may take)
 template <class T, int N> struct Table {
@@ -55,7 +54,7 @@ template <class T, int N> struct Table {
     unsigned first[N + 1];   // first chunk of each tensor
     int count, number0;      // number0: the first tensor's number in the call
 };
-constexpr int kTensors = 64, kTensors8 = 44;
+constexpr int kTensors = 64, kTensors8 = 48;
 static_assert(sizeof(Table<Tensor, kTensors>) + sizeof(Step) <= 4000 && sizeof(Table<Tensor8, kTensors8>) + sizeof(Step) <= 4000, "");
 
 template <class T, int N> __device__ __forceinline__ int tensor_of(const Table<T, N> &tab, unsigned chunk) {
@@ -102,21 +101,58 @@ __device__ __forceinline__ void step_one(float &w, float g, float &mom, float &v
     w = w * k.shrink - k.c1 * mom / (sqrtf(var * k.c2) + s.eps);
 }
 
-// A chunk is four elements a thread.
+// Four consecutive elements, from any address; NT: past the caches (a model's states do not fit them).
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef f4 f4_any __attribute__((aligned(4)));
+typedef u2 u2_any __attribute__((aligned(2)));
+typedef unsigned u1_any __attribute__((aligned(1)));
+template <bool NT, class V, class P> __device__ __forceinline__ V fetch(const P *p) {
+    const V *q = reinterpret_cast<const V *>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool NT, class V, class P, class X> __device__ __forceinline__ void put(P *p, X x) {
+    V *q = reinterpret_cast<V *>(p);
+    if (NT) __builtin_nontemporal_store((V)x, q);
+    else *q = (V)x;
+}
+template <bool NT> __device__ __forceinline__ void fetch4(const float *p, float (&x)[4]) {
+    const f4 d = fetch<NT, f4_any>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = d[e];
+}
+template <bool NT> __device__ __forceinline__ void fetch4(const uint16_t *p, float (&x)[4]) {
+    const u2 d = fetch<NT, u2_any>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(float, e & 1 ? d[e / 2] & 0xffff0000u : d[e / 2] << 16);
+}
+template <bool NT> __device__ __forceinline__ void put4(float *p, const float (&x)[4]) { put<NT, f4_any>(p, f4{x[0], x[1], x[2], x[3]}); }
+// (the copy is read by the next step's products: it stays in the caches' reach)
+__device__ __forceinline__ void put4_bf16(uint16_t *p, const float (&x)[4]) {
+    put<false, u2_any>(p, u2{to_bf16(x[0]) | (unsigned)to_bf16(x[1]) << 16, to_bf16(x[2]) | (unsigned)to_bf16(x[3]) << 16});
+}
+
+// A chunk is four consecutive elements a thread.
 constexpr unsigned kChunk = 4 * kThreads;
 
-template <class G>
+template <class G, bool NT>
 __global__ __launch_bounds__(kThreads) void adamw_tensors(Table<Tensor, kTensors> tab, Step s) {
     const int which = tensor_of(tab, blockIdx.x);
     const Tensor &t = tab.t[which];
     const Scalars k = scalars(s);
-    const size_t i0 = (size_t)(blockIdx.x - tab.first[which]) * kChunk + threadIdx.x;
+    const size_t i0 = (size_t)(blockIdx.x - tab.first[which]) * kChunk + 4 * threadIdx.x;
     float *mom = static_cast<float *>(t.mom), *var = static_cast<float *>(t.var);
     const G *dw = static_cast<const G *>(t.dw);
+    if (i0 + 4 <= t.size) {
+        float w[4], g[4], m[4], v[4];
+        fetch4<NT>(t.w + i0, w), fetch4<NT>(dw + i0, g), fetch4<NT>(mom + i0, m), fetch4<NT>(var + i0, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const size_t i = i0 + e * kThreads;
-        if (i >= t.size) return;
+        for (int e = 0; e < 4; ++e) step_one(w[e], g[e], m[e], v[e], k, s);
+        put4<NT>(t.w + i0, w), put4<NT>(mom + i0, m), put4<NT>(var + i0, v);
+        if (t.copy) put4_bf16(t.copy + i0, w);
+        return;
+    }
+    for (size_t i = i0; i < t.size; ++i) {   // the last thread's one to three
         float w = t.w[i], m = mom[i], v = var[i];
         step_one(w, grad_of(dw, i), m, v, k, s);
         t.w[i] = w, mom[i] = m, var[i] = v;
@@ -167,38 +203,27 @@ __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
     return (unsigned)(8 * (e + 7) + q - 8);
 }
 
-// A wavefront owns a block of 256 elements, a lane four of them: consecutive ones (FULL: the block is whole and every
-// tensor starts on the boundary of four of its elements), or one of every 64.
-template <class G, bool FULL>
+// A wavefront owns a block of 256 elements, a lane four consecutive ones of them (FULL: the block is whole).
+template <class G, bool FULL, bool NT>
 __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int lane, unsigned number, const Scalars &k, const Step &s) {
     uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);
     const G *dw = static_cast<const G *>(t.dw);
     const float ms = t.mom_scale[block], vs = t.var_scale[block];
-    const size_t i0 = block * kBlock + (FULL ? lane * 4 : lane);
-    constexpr int kStep = FULL ? 1 : 64;
+    const size_t i0 = block * kBlock + lane * 4;
     float w[4], g[4], m[4], r[4], top = 0.f, peak = 0.f;
     unsigned mc[4], vc[4];
     bool in[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) in[e] = FULL || i0 + e * kStep < t.size;
+    for (int e = 0; e < 4; ++e) in[e] = FULL || i0 + e < t.size;
     if constexpr (FULL) {
-        const float4 x = *reinterpret_cast<const float4 *>(t.w + i0);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-        if constexpr (sizeof(G) == 4) {
-            const float4 y = *reinterpret_cast<const float4 *>(dw + i0);
-            g[0] = y.x, g[1] = y.y, g[2] = y.z, g[3] = y.w;
-        } else {
-            const uint2 y = *reinterpret_cast<const uint2 *>(dw + i0);
-            g[0] = __builtin_bit_cast(float, y.x << 16), g[1] = __builtin_bit_cast(float, y.x & 0xffff0000u);
-            g[2] = __builtin_bit_cast(float, y.y << 16), g[3] = __builtin_bit_cast(float, y.y & 0xffff0000u);
-        }
-        const unsigned a = *reinterpret_cast<const unsigned *>(mom8 + i0), b = *reinterpret_cast<const unsigned *>(var8 + i0);
+        fetch4<NT>(t.w + i0, w), fetch4<NT>(dw + i0, g);
+        const unsigned a = fetch<NT, u1_any>(mom8 + i0), b = fetch<NT, u1_any>(var8 + i0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) mc[e] = (a >> (8 * e)) & 0xffu, vc[e] = (b >> (8 * e)) & 0xffu;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const size_t i = i0 + e * kStep;
+            const size_t i = i0 + e;
             w[e] = in[e] ? t.w[i] : 0.f;
             g[e] = in[e] ? grad_of(dw, i) : 0.f;
             mc[e] = in[e] ? mom8[i] : 0u, vc[e] = in[e] ? var8[i] : 0u;
@@ -219,24 +244,21 @@ __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int
     const double im = mscale > 0.f ? 1.0 / (double)mscale : 0.0, iv = vscale > 0.f ? 1.0 / (double)vscale : 0.0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const size_t i = i0 + e * kStep;
         // (the quotients by a reciprocal in 64 bits: the fp32 quotient of mom correctly rounded)
         const float x = fminf(fmaxf((float)(m[e] * im), -kLargest), kLargest);
         const double y = fmin(r[e] * iv, (double)kLargest);
         mc[e] = fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8;
-        vc[e] = r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)i + number)) : kNan8;
+        vc[e] = r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)(i0 + e) + number)) : kNan8;
     }
     if constexpr (FULL) {
-        *reinterpret_cast<float4 *>(t.w + i0) = make_float4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<unsigned *>(mom8 + i0) = mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24;
-        *reinterpret_cast<unsigned *>(var8 + i0) = vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24;
-        if (t.copy)
-            *reinterpret_cast<uint2 *>(t.copy + i0) = make_uint2(to_bf16(w[0]) | (unsigned)to_bf16(w[1]) << 16,
-                                                                 to_bf16(w[2]) | (unsigned)to_bf16(w[3]) << 16);
+        put4<NT>(t.w + i0, w);
+        put<NT, u1_any>(mom8 + i0, mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24);
+        put<NT, u1_any>(var8 + i0, vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24);
+        if (t.copy) put4_bf16(t.copy + i0, w);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const size_t i = i0 + e * kStep;
+            const size_t i = i0 + e;
             if (!in[e]) continue;
             t.w[i] = w[e], mom8[i] = (uint8_t)mc[e], var8[i] = (uint8_t)vc[e];
             if (t.copy) t.copy[i] = to_bf16(w[e]);
@@ -248,7 +270,7 @@ __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int
     }
 }
 
-template <class G>
+template <class G, bool NT>
 __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTensors8> tab, Step s) {
     const int which = tensor_of(tab, blockIdx.x);
     const Tensor8 &t = tab.t[which];
@@ -256,8 +278,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTenso
     const size_t block = (size_t)(blockIdx.x - tab.first[which]) * 4 + (threadIdx.x >> 6);
     if (block * kBlock >= t.size) return;   // whole wavefronts leave together
     const unsigned number = (unsigned)(tab.number0 + which) * 0x9E3779B9u + (unsigned)s.state->steps * 0x85EBCA6Bu;
-    if (t.aligned && (block + 1) * kBlock <= t.size) adamw8_block<G, true>(t, block, threadIdx.x & 63, number, k, s);
-    else adamw8_block<G, false>(t, block, threadIdx.x & 63, number, k, s);
+    if ((block + 1) * kBlock <= t.size) adamw8_block<G, true, NT>(t, block, threadIdx.x & 63, number, k, s);
+    else adamw8_block<G, false, NT>(t, block, threadIdx.x & 63, number, k, s);
 }
 
 int check(const char *who, int count, const void *const *w, const void *const *dw, const void *const *mom,
@@ -301,6 +323,13 @@ int launch_tables(const char *who, int count, const size_t *sizes, Fill fill, La
     return SWC_HIP_OK;
 }
 
+// Whether the weights of a call are large enough to be streamed past the caches.
+bool streams(const size_t *sizes, int count, size_t bytes) {
+    size_t all = 0;
+    for (int i = 0; i < count; ++i) all += sizes[i];
+    return all * bytes >= kStreamingBytes;
+}
+
 template <class G>
 int adamw(const char *who, int count, float *const *w, const G *const *dw, float *const *mom, float *const *var,
           uint16_t *const *copies, const size_t *sizes, const void *state, float lr, double beta1, double beta2, float eps,
@@ -314,7 +343,8 @@ int adamw(const char *who, int count, float *const *w, const G *const *dw, float
         who, count, sizes,
         [&](Tensor &t, int i) { t = Tensor{w[i], dw[i], mom[i], var[i], copies ? copies[i] : nullptr, sizes[i]}; },
         [&](const Table<Tensor, kTensors> &tab, unsigned chunks) {
-            adamw_tensors<G><<<chunks, kThreads, 0, stream()>>>(tab, s);
+            auto kern = streams(sizes, count, sizeof(float)) ? adamw_tensors<G, true> : adamw_tensors<G, false>;
+            kern<<<chunks, kThreads, 0, stream()>>>(tab, s);
         });
 }
 
@@ -333,11 +363,10 @@ int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint
         [&](Tensor8 &t, int i) {
             t.w = w[i], t.dw = dw[i], t.mom = mom8[i], t.var = var8[i], t.copy = copies ? copies[i] : nullptr;
             t.size = sizes[i], t.mom_scale = mom_scale[i], t.var_scale = var_scale[i];
-            auto on = [](const void *p, size_t step) { return reinterpret_cast<uintptr_t>(p) % step == 0; };
-            t.aligned = on(t.w, 16) && on(t.dw, 4 * sizeof(G)) && on(t.mom, 4) && on(t.var, 4) && on(t.copy, 8);
         },
         [&](const Table<Tensor8, kTensors8> &tab, unsigned chunks) {
-            adamw8_tensors<G><<<chunks, kThreads, 0, stream()>>>(tab, s);
+            auto kern = streams(sizes, count, sizeof(float)) ? adamw8_tensors<G, true> : adamw8_tensors<G, false>;
+            kern<<<chunks, kThreads, 0, stream()>>>(tab, s);
         });
 }
 

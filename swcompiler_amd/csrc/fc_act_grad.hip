@@ -13,17 +13,16 @@ using namespace swc_hip::product;
 
 namespace {
 
-// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of kSumRows rows' column sums of the unrounded
-// values.  64 threads side by side hold four columns each, four rows at a time.
-constexpr int kSumRows = 32;
+// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.  64 threads side by side hold four columns each, four rows at a time.
 template <class T, int ACT>
-__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums) {
+__global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums,
+                                                int each) {
 #if __HIP_DEVICE_COMPILE__
     __shared__ float part[4][256];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int j = (blockIdx.x * 64 + tx) * 4;
-    const int r0 = blockIdx.y * kSumRows;
-    const int r1 = r0 + kSumRows < m ? r0 + kSumRows : m;
+    const int r0 = blockIdx.y * each;
+    const int r1 = r0 + each < m ? r0 + each : m;
     const int have = n - j;
     float sum[4] = {};
     if (have > 0) {
@@ -78,15 +77,17 @@ int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, cons
     return SWC_HIP_OK;
 }
 
-int sum_blocks(int m) { return (m + kSumRows - 1) / kSumRows; }
+// Rows a workgroup takes: 32, or 8 where that leaves the chip short of workgroups (512 x 1024: 10 us and 4).
+int sum_rows(int m, int n) { return (long)((m + 31) / 32) * ((n + 255) / 256) >= 4L * swc::devices::HipDevice::computeUnits ? 32 : 8; }
+int sum_blocks(int m, int n) { return (m + sum_rows(m, n) - 1) / sum_rows(m, n); }
 
 template <class T>
 int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
     if (!dz) ld = 0;
-    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m));
-    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * kSumRows);
+    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m, n));
+    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * sum_rows(m, n));
     return with_act(act, [&]<int ACT>() {
-        act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums);
+        act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums, sum_rows(m, n));
         SWC_LAUNCH_CHECK();
         return (int)SWC_HIP_OK;
     });
@@ -105,7 +106,7 @@ Space<T> space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool p
     s.a = pack_a ? c.take<T>((size_t)m * row_length<T>(k)) : nullptr;
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
-    s.sums = bias ? c.take<float>((size_t)sum_blocks(m) * n) : nullptr;
+    s.sums = bias ? c.take<float>((size_t)sum_blocks(m, n) * n) : nullptr;
     s.bytes = c.used;
     return s;
 }
@@ -150,7 +151,7 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
     if (own_dz || dbias) {
         if (int rc = launch_act_grad<T>(w.dz, padded, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
         if (dbias)
-            if (int rc = sum_parts<T>(dbias, w.sums, sum_blocks(m), n)) return rc;
+            if (int rc = sum_parts<T>(dbias, w.sums, sum_blocks(m, n), n)) return rc;
     }
     const T *dz = own_dz ? w.dz : dc;
     const long lddz = own_dz ? padded : lddc;

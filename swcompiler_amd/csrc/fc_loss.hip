@@ -178,22 +178,33 @@ template <class T> struct RowStats {
 #endif
 };
 
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
-    const float top = fmaxf(a.x, b.x), from = top == -__builtin_inff() ? 0.f : top;
-    return make_float2(top, a.y * expf(a.x - from) + b.y * expf(b.x - from));
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    return x;
 }
 
-// A wavefront joins a dense row's blocks -> the row's loss (in lane 0)
+// A wavefront joins a dense row's blocks -> the row's loss: their maxima first, then the sums relative to the largest.
 __device__ __forceinline__ float join_row(int row, int lane, const float2 *part, int blocks, const float *picked, const Rows &rows,
                                           float *row_loss, float *lse) {
     const float2 *p = part + (size_t)row * blocks;
-    float2 s = make_float2(-__builtin_inff(), 0.f);
-    for (int b = lane; b < blocks; b += 64) s = join(s, p[b]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s = join(s, make_float2(__shfl_xor(s.x, off), __shfl_xor(s.y, off)));
-    const float l = (s.x == -__builtin_inff() ? 0.f : s.x) + logf(s.y), loss = l - picked[row];
+    const float2 first = lane < blocks ? p[lane] : make_float2(-__builtin_inff(), 0.f);
+    const float z = picked[row];
+    const int r = rows.index[row];
+    float top = first.x;
+    for (int b = lane + 64; b < blocks; b += 64) top = fmaxf(top, p[b].x);
+    top = wave_max(top);
+    const float from = top == -__builtin_inff() ? 0.f : top;
+    float sum = first.y * expf(first.x - from);
+    for (int b = lane + 64; b < blocks; b += 64) sum += p[b].y * expf(p[b].x - from);
+    sum = wave_sum(sum);
+    const float l = from + logf(sum), loss = l - z;
     if (lane == 0) {
-        const int r = rows.index[row];
         lse[r] = l;
         row_loss[r] = loss;
     }
@@ -436,7 +447,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
     const int blocks = (n + block_columns(p) - 1) / block_columns(p);
     const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, w.rows.count};
     if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias}, who)) return rc;
-    if (m <= 128) {
+    if (m <= 64) {
         mean_loss<true><<<1, 1024, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse, loss);
     } else {
         join_rows<<<ceil_div(m, 4), 256, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse);

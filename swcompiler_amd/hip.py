@@ -190,12 +190,11 @@ class _Arg:
 
     def __init__(self, rt, x, what):
         self.shape = shape = tuple(x.shape)
+        self.ld = shape[-1] if shape else 1
         if isinstance(x, DeviceArray):
             self.ptr, self.type, self.size = x.ptr, _NUMPY_TYPES.get(x.dtype.name), x.size
-            self.ld = shape[-1] if shape else 1
             return
         self.ptr, self.type, self.size = _torch_operand(rt, x, what)
-        self.ld = shape[-1] if shape else 1
         if x.is_contiguous():
             return
         stride = x.stride()
@@ -690,8 +689,8 @@ class SwcHip:
         a = _Arg(self, x, what)
         if a.type not in types:
             raise SwcHipError(f"{what}: element type {a.type or x.dtype} is not one of {', '.join(types)}")
-        if shape is not None and a.shape != tuple(shape):
-            raise SwcHipError(f"{what}: shape {a.shape}, expected {tuple(shape)}")
+        if shape is not None and a.shape != shape:
+            raise SwcHipError(f"{what}: shape {a.shape}, expected {shape}")
         return a
 
     @staticmethod
@@ -797,6 +796,15 @@ class SwcHip:
             """-> (array of addresses, element counts, the type of all)"""
             if len(values) != count:
                 raise SwcHipError(f"{what}: lists of different lengths")
+            try:   # torch tensors of one known type that need no further word
+                kinds = {x.dtype for x in values}
+                kind = _TORCH_KINDS.get(kinds.pop()) if len(kinds) == 1 else None
+                if kind in types and all([x.is_contiguous() and x.get_device() == self.device for x in values]):
+                    found = [x.numel() for x in values]
+                    if sizes is None or found == sizes:
+                        return (C.c_void_p * count)(*[x.data_ptr() for x in values]), found, kind
+            except AttributeError:
+                pass
             out, found, kind = [], [], types[0]
             for i, x in enumerate(values):
                 if x is None and name == "copies":
