@@ -427,10 +427,13 @@ size_t swc_hip_conv2dFusedMaxpool_workspace_bytes(const size_t *cdims, const siz
 
 /* ---- operators of language models.  No counterparts in the reference: each
  * stands next to an op above whose work it does in the form that such models
- * need.  Matrices are row-major with leading dimensions in elements (at most
- * 4194240 for the _bf forms, 2097088 for the _f ones); outputs must not overlap inputs except where it
- * is said.  Workspace: the size queries below, which answer for every alignment
- * of the operands. ---- */
+ * need.  Matrices are row-major with leading dimensions in elements; those of
+ * inputs, n and k are at most 4194240 for the _bf forms and 2097088 for the _f
+ * ones, m at most 2^30 (4194240 for the softmax loss): beyond,
+ * SWC_HIP_EUNSUPPORTED.  Addresses need the alignment of an element only (16
+ * bytes, for rows too, save a copy).  Outputs must not overlap inputs or each
+ * other except where it is said.  Workspace: the size queries below, which
+ * answer for every alignment of the operands. ---- */
 
 /* the activations */
 enum {
@@ -445,7 +448,8 @@ enum {
  *     Z[m,n] = A[m,k] * B[k,n] + bias[n]      C = act(Z) + residual[m,n]
  * bias, residual and preact may be NULL.  preact receives Z (in the matrices'
  * type), which the gradient call needs unless act is SWC_HIP_ACT_NONE.
- * residual may be C itself.  k == 0 gives Z = bias. */
+ * residual may be C itself (with ldr == ldc).  k == 0 gives Z = bias.  No
+ * workspace for one row (bf16) or up to four (fp32). */
 int swc_hip_matrixMatrixFCActAdd_f(int m, int n, int k, const float *a, int lda,
                                    const float *b, int ldb, const float *bias, int act,
                                    const float *residual, int ldr, float *preact, int ldp,
@@ -482,7 +486,8 @@ size_t swc_hip_matrixMatrixFCActAddGrad_workspace_bytes(int m, int n, int k, int
  * A row whose selected[r] lies outside [0, n) is left out: its rowLoss and lse
  * are 0, it does not count in the mean, and nothing in its row of A (infinities
  * and NaN included) reaches any result.  With no row left *loss is 0.
- * rowLoss, lse and loss are fp32 device memory and must all be given. */
+ * rowLoss, lse and loss are fp32 device memory and must all be given; k must be
+ * positive. */
 int swc_hip_matrixFCSoftmaxWithLoss_f(int m, int n, int k, const float *a, int lda,
                                       const float *b, int ldb, const float *bias,
                                       const int *selected, float *rowLoss, float *lse, float *loss);
@@ -499,7 +504,8 @@ size_t swc_hip_matrixFCSoftmaxWithLoss_workspace_bytes(int m, int n, int k, int 
  * gradient of the SUM of the rows' losses, as matrixSoftmaxWithLossGrad_f gives
  * it.  Rows left out have a zero row in aGrad and no part in the others.  The
  * logits are computed again piece by piece.  Any of the three outputs may be
- * NULL; all are overwritten.  The _bf form holds dz in bfloat16 for the products. */
+ * NULL; all are overwritten.  The _bf form holds dz in bfloat16 for the products
+ * and the column sums. */
 int swc_hip_matrixFCSoftmaxWithLossGrad_f(int m, int n, int k, const float *a, int lda,
                                           const float *b, int ldb, const float *bias,
                                           const int *selected, const float *lse,
@@ -529,7 +535,8 @@ size_t swc_hip_matrixFCSoftmaxWithLossGrad_workspace_bytes(int m, int n, int k, 
  * before the call returns; a size of 0 skips its tensor.  w is fp32; dw is fp32
  * in the _f forms and bfloat16 in the _bf forms; copies (NULL, or `count`
  * pointers of which any may be NULL) receive w rounded to bfloat16.
- * No two tensors of a call may overlap.  (The betas are doubles: 1 - beta of a
+ * No two tensors of a call may overlap (a w given twice is refused); a tensor has
+ * at most 17179868160 elements.  (The betas are doubles: 1 - beta of a
  * float beta near 1 has lost a few digits.) */
 #define SWC_HIP_ADAMW_STATE_BYTES 32u
 int swc_hip_adamwAdvance(void *state, double beta1, double beta2);
@@ -548,12 +555,14 @@ int swc_hip_adamw_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, 
  * (e4m3: 8-bit floats of 4 exponent and 3 mantissa bits, bias 7, largest value
  * 448, no infinities).  A step decodes both, updates as above in fp32 and encodes
  * them again with scale = (largest finite magnitude of the block) * (1/448 as an
- * fp32): mom / scale, as an fp32, to the nearest value, ties to even; sqrt(var) up or down at random with the
- * probabilities that keep its expectation (a variance decays by less per step
- * than half the distance of two values, and would never move if it were rounded
- * to the nearest), but a positive one never to zero.  The random number of
- * element i of tensor t in step s is 20 bits of a hash of (i + t * 0x9E3779B9 +
- * s * 0x85EBCA6B): the same step gives the same bits.  A value that is not
+ * fp32), or 0, and the block as zeros, where that magnitude is at most 2^-100:
+ * mom / scale, as an fp32, to the nearest value, ties to even; sqrt(var) up or
+ * down at random with the probabilities that keep its expectation (a variance
+ * decays by less per step than half the distance of two values, and would never
+ * move if it were rounded to the nearest), but a positive one never to zero.  The
+ * random number of element i of tensor t in step s is 20 bits of a hash of
+ * (i + t * 0x9E3779B9 + s * 0x85EBCA6B) modulo 2^32: the same step gives the same
+ * bits.  A value that is not
  * finite is held as NaN.  w is updated from the unrounded states.  momScale and
  * varScale hold (size + SWC_HIP_ADAMW_BLOCK - 1) / SWC_HIP_ADAMW_BLOCK floats per tensor;
  * all zero is the state before the first step. */

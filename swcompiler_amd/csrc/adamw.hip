@@ -4,10 +4,12 @@
 // Bound by memory: per element w 8 bytes, the gradient 4 or 2, the states 16 or 4, the bfloat16 copy 2 — and some
 // twenty fp32 operations.  One launch covers up to kTensors tensors: their pointers travel by value in the kernel
 // arguments (nothing to upload, so a recorded graph needs no buffer of its own), and a workgroup finds its tensor by
-// bisecting the running count of chunks (an entry per tensor, in scalar registers).
+// comparing its number with each tensor's first, one a lane.
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <vector>
 
 using namespace swc_hip;
 
@@ -57,14 +59,12 @@ template <class T, int N> struct Table {
 constexpr int kTensors = 64, kTensors8 = 48;
 static_assert(sizeof(Table<Tensor, kTensors>) + sizeof(Step) <= 4000 && sizeof(Table<Tensor8, kTensors8>) + sizeof(Step) <= 4000, "");
 
+// The last tensor whose first chunk is not behind this one (one without elements shares its first chunk with the next).
 template <class T, int N> __device__ __forceinline__ int tensor_of(const Table<T, N> &tab, unsigned chunk) {
-    int lo = 0, hi = tab.count;   // first[lo] <= chunk < first[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (tab.first[mid] <= chunk) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+    static_assert(N <= 64, "a lane for each");
+    const int lane = threadIdx.x & 63;
+    const bool before = lane < tab.count && tab.first[lane < N ? lane : N] <= chunk;
+    return __popcll(__ballot(before)) - 1;
 }
 
 __device__ __forceinline__ float grad_of(const float *p, size_t i) { return p[i]; }
@@ -132,8 +132,10 @@ __device__ __forceinline__ void put4_bf16(uint16_t *p, const float (&x)[4]) {
     put<false, u2_any>(p, u2{to_bf16(x[0]) | (unsigned)to_bf16(x[1]) << 16, to_bf16(x[2]) | (unsigned)to_bf16(x[3]) << 16});
 }
 
-// A chunk is four consecutive elements a thread.
+// A chunk is four consecutive elements a thread: a workgroup's work.  (Four chunks a workgroup: 265M parameters 1341 us
+// against 1298, its registers halve the wavefronts.)  A launch has at most 2^32 - 1 threads.
 constexpr unsigned kChunk = 4 * kThreads;
+constexpr unsigned kMaxChunks = 0xffffffffu / kThreads;
 
 template <class G, bool NT>
 __global__ __launch_bounds__(kThreads) void adamw_tensors(Table<Tensor, kTensors> tab, Step s) {
@@ -192,9 +194,10 @@ __device__ __forceinline__ unsigned to_e4m3(float y) {
     return 0;
 #endif
 }
-// 0 <= y <= 448 up or down by 20 random bits, which side settled in 64 bits: with the exponent E of y (at least that of the least normal value) the
-// values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is 8 (E + 7) + q - 8 — also
-// where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the subnormal values).
+// 0 <= y <= 448 up or down by 20 random bits, which side settled in 64 bits: with the exponent E of y (at least that of the
+// least normal value) the values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is
+// 8 (E + 7) + q - 8 — also where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the
+// subnormal values).
 __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
     const int e = max((int)(__builtin_bit_cast(unsigned long long, y) >> 52) - 1023, -6);
     const double units = __builtin_bit_cast(double, (unsigned long long)(1023 + 3 - e) << 52);   // 2^(3 - E)
@@ -295,6 +298,15 @@ int check(const char *who, int count, const void *const *w, const void *const *d
     for (int i = 0; i < count; ++i)
         if (sizes[i] && (!w[i] || !dw[i] || !mom[i] || !var[i] || (eight && (!mom_scale[i] || !var_scale[i]))))
             return fail(SWC_HIP_EINVAL, "%s: null pointer for tensor %d", who, i);
+    for (int i = 0; i < count; ++i)
+        if (sizes[i] > (size_t)kMaxChunks * kChunk) return fail(SWC_HIP_EUNSUPPORTED, "%s: tensor %d has %zu elements", who, i, sizes[i]);
+    // one parameter given twice (tied weights) would be stepped by two workgroups at a time
+    std::vector<const void *> seen;
+    seen.reserve(count);
+    for (int i = 0; i < count; ++i)
+        if (sizes[i]) seen.push_back(w[i]);
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return fail(SWC_HIP_EINVAL, "%s: a tensor is given twice", who);
     return SWC_HIP_OK;
 }
 
@@ -308,9 +320,8 @@ int launch_tables(const char *who, int count, const size_t *sizes, Fill fill, La
         tab.count = 0;
         tab.number0 = next;
         for (; next < count && tab.count < N; ++next) {
-            const size_t need = (sizes[next] + kChunk - 1) / kChunk;
-            if (need > 0x7fffffffu) return fail(SWC_HIP_EUNSUPPORTED, "%s: tensor %d has %zu elements", who, next, sizes[next]);
-            if (chunks + need > 0x7fffffffu) break;
+            const size_t need = (sizes[next] + kChunk - 1) / kChunk;   // (at most kMaxChunks: check)
+            if (chunks + need > kMaxChunks) break;
             fill(tab.t[tab.count], next);
             tab.first[tab.count++] = chunks;
             chunks += (unsigned)need;
@@ -338,7 +349,8 @@ int adamw(const char *who, int count, float *const *w, const G *const *dw, float
                        (const void *const *)var, nullptr, nullptr, sizes, state, false, lr, beta1, beta2, eps, decay))
         return rc;
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
-    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1), (float)(1. - beta2), eps, decay};
+    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1),
+                 (float)(1. - beta2), eps, decay};
     return launch_tables<Tensor, kTensors>(
         who, count, sizes,
         [&](Tensor &t, int i) { t = Tensor{w[i], dw[i], mom[i], var[i], copies ? copies[i] : nullptr, sizes[i]}; },
@@ -357,7 +369,8 @@ int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint
                        state, true, lr, beta1, beta2, eps, decay))
         return rc;
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
-    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1), (float)(1. - beta2), eps, decay};
+    const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1),
+                 (float)(1. - beta2), eps, decay};
     return launch_tables<Tensor8, kTensors8>(
         who, count, sizes,
         [&](Tensor8 &t, int i) {

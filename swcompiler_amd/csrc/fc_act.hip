@@ -4,8 +4,9 @@
 //     Z = A B + bias, C = act(Z) + residual
 //
 // One product on the core of product_tile.hpp, with everything behind the sums in its epilogue; a product cut along k
-// (few tiles) leaves fp32 partial sums in the workspace and ends in fc_finish; few rows take fc_stream or fc_few.  4096 x 16384 x 4096 bf16 with bias, tanh
-// gelu and residual: 486 us (the product alone 412, the residual's 134 MB another 30).
+// (few tiles) leaves fp32 partial sums in the workspace and ends in fc_finish; few rows take fc_stream or fc_few.
+// 4096 x 16384 x 4096 bf16 with bias, tanh gelu and residual: 461 us, 1190 TFLOP/s (the product alone 412; the residual's 134
+// MB another 30).  2048 x 4096 x 4096 fp32 with gelu and residual 498 us, 138 TFLOP/s of the 152 that a large product reaches.
 #include "act.hpp"
 #include "product.hpp"
 
@@ -51,7 +52,8 @@ template <class T, int ACT> struct FcEpilogue {
 };
 
 // The end of a layer from fp32 sums: `parts` matrices of m x n to be added in order, then bias, activation, residual.
-// Four columns of a row a thread.
+// Four columns of a row a thread.  Bound by memory: parts + 1 to 3 passes over m x n; where it runs that is a few MB from
+// the caches, and its launch.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void fc_finish(const float *part, int parts, long part_stride, const T *bias, const T *residual,
                                                  long ldr, T *preact, long ldp, T *c, long ldc, int m, int n) {
@@ -222,9 +224,9 @@ int launch_stream(int, const float *, long, const float *, long, const float *, 
 
 // One to four rows in fp32, or one in bf16 where fc_stream does not take the operands: bound by one pass over B.  A
 // workgroup owns 64 bytes of B's columns; four lanes side by side read them, 256 rows of B at a time, each a chunk of 16
-// bytes from any address, eight rows ahead; the sums over the 256 lanes of a column are joined by lane exchange within a wavefront and through LDS between the
-// sixteen of them, and the first threads end the layer.  One launch, no workspace.  (Workgroups 2 j and 2 j + 1, which
-// share lines of B, are eight apart in launch order: on one XCD's L2.)
+// bytes from any address, eight rows ahead; the sums over the 256 lanes of a column are joined by lane exchange within a
+// wavefront and through LDS between the sixteen of them, and the first threads end the layer.  One launch, no workspace.
+// (Workgroups 2 j and 2 j + 1, which share lines of B, are eight apart in launch order: on one XCD's L2.)
 constexpr int kFewThreads = 1024;
 template <class T, int M, int ACT>
 __global__ __launch_bounds__(kFewThreads) void fc_few(const T *a, long lda, const T *b, long ldb, const T *bias, const T *residual,
@@ -336,17 +338,21 @@ template <class T> __global__ __launch_bounds__(256) void add_parts(T *out, cons
 }
 
 template <class T>
-int check_forward(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb, int act, const T *residual,
-                  int ldr, const T *preact, int ldp, const T *c, int ldc) {
+int check_forward(const char *who, int m, int n, int k, const T *a, int lda, const T *b, int ldb, const T *bias, int act,
+                  const T *residual, int ldr, const T *preact, int ldp, const T *c, int ldc) {
     if (m < 0 || n < 0 || k < 0) return fail(SWC_HIP_EINVAL, "%s: negative dimension", who);
     if (!known_act(act)) return fail(SWC_HIP_EINVAL, "%s: unknown activation %d", who, act);
     if (m == 0 || n == 0) return SWC_HIP_OK;
     if (!c || (k && (!a || !b))) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
     if ((k && (lda < k || ldb < n)) || ldc < n || (residual && ldr < n) || (preact && ldp < n))
         return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
-    if ((const void *)c == a || (const void *)c == b || (preact && (preact == a || preact == b || preact == c || preact == residual)))
-        return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
-    if (lda > kMaxLd<T> || ldb > kMaxLd<T>) return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
+    const bool c_in = c == a || c == b || c == bias;
+    if (c_in || (preact && (preact == a || preact == b || preact == bias || preact == c || preact == residual)))
+        return fail(SWC_HIP_EINVAL, "%s: an output is also an input or another output", who);
+    if (residual == c && ldr != ldc && m > 1) return fail(SWC_HIP_EINVAL, "%s: the residual is C in rows of another length", who);
+    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || n > kMaxLd<T>)
+        return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
+    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
     return SWC_HIP_OK;
 }
 
@@ -371,7 +377,7 @@ template <class T> Space<T> space(char *base, const Plan &p, int m, int n, int k
 template <class T>
 int forward(const char *who, int m, int n, int k, const T *a, int lda_, const T *b, int ldb_, const T *bias, int act, const T *residual,
             int ldr, T *preact, int ldp, T *c, int ldc) {
-    if (int rc = check_forward(who, m, n, k, a, lda_, b, ldb_, act, residual, ldr, preact, ldp, c, ldc)) return rc;
+    if (int rc = check_forward(who, m, n, k, a, lda_, b, ldb_, bias, act, residual, ldr, preact, ldp, c, ldc)) return rc;
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
     if (m == 0 || n == 0) return SWC_HIP_OK;
     if (k == 0) return launch_finish<T>(act, nullptr, 0, bias, residual, ldr, preact, ldp, c, ldc, m, n);

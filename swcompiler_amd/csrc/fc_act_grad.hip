@@ -13,7 +13,8 @@ using namespace swc_hip::product;
 
 namespace {
 
-// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.  64 threads side by side hold four columns each, four rows at a time.
+// dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.  64
+// threads side by side hold four columns each, four rows at a time.  Bound by memory: three passes over m x n.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums,
                                                 int each) {
@@ -72,20 +73,25 @@ int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, cons
     const void *in[4] = {dc, a, b, preact};
     for (const void *p : in)
         if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
-    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || lddc > kMaxLd<T>)
+    if ((da && (da == db || da == dbias)) || (db && db == dbias)) return fail(SWC_HIP_EINVAL, "%s: two outputs are the same", who);
+    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || lddc > kMaxLd<T> || n > kMaxLd<T> || k > kMaxLd<T>)
         return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
+    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
     return SWC_HIP_OK;
 }
 
-// Rows a workgroup takes: 32, or 8 where that leaves the chip short of workgroups (512 x 1024: 10 us and 4).
-int sum_rows(int m, int n) { return (long)((m + 31) / 32) * ((n + 255) / 256) >= 4L * swc::devices::HipDevice::computeUnits ? 32 : 8; }
+// Rows a workgroup takes: 32, or 8 where that leaves the chip short of workgroups (512 x 1024: 10 us and 4); more where a
+// grid's 65535 rows of workgroups would not cover them.
+int sum_rows(int m, int n) {
+    if ((m + 31) / 32 > 65535) return (m + 65534) / 65535;
+    return (long)((m + 31) / 32) * ((n + 255) / 256) >= 4L * swc::devices::HipDevice::computeUnits ? 32 : 8;
+}
 int sum_blocks(int m, int n) { return (m + sum_rows(m, n) - 1) / sum_rows(m, n); }
 
 template <class T>
 int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
     if (!dz) ld = 0;
     const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m, n));
-    if (grid.y > 65535) return fail(SWC_HIP_EUNSUPPORTED, "matrixMatrixFCActAddGrad: more than %d rows", 65535 * sum_rows(m, n));
     return with_act(act, [&]<int ACT>() {
         act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums, sum_rows(m, n));
         SWC_LAUNCH_CHECK();

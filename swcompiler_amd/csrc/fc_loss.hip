@@ -347,11 +347,11 @@ int check(const char *who, int m, int n, int k, const T *a, int lda, const T *b,
     if (m && !selected) return fail(SWC_HIP_EINVAL, "%s: selected is null", who);
     if (m && n && k && (!a || !b)) return fail(SWC_HIP_EINVAL, "%s: null pointer", who);
     if (m && n && k && (lda < k || ldb < n)) return fail(SWC_HIP_EINVAL, "%s: leading dimension smaller than row length", who);
-    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || row_length<T>(k) > kMaxLd<T> || row_length<T>(n) > kMaxLd<T>)
+    if (lda > kMaxLd<T> || ldb > kMaxLd<T> || k > kMaxLd<T> || n > kMaxLd<T>)
         return fail(SWC_HIP_EUNSUPPORTED, "%s: leading dimension beyond %ld", who, kMaxLd<T>);
     if (m && n && k == 0) return fail(SWC_HIP_EINVAL, "%s: k is 0", who);
-    constexpr int kMaxRows = 65535 * kSumRows;
-    if (m > kMaxRows) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMaxRows);
+    constexpr int kMost = 65535 * kSumRows;
+    if (m > kMost) return fail(SWC_HIP_EUNSUPPORTED, "%s: more than %d rows", who, kMost);
     return SWC_HIP_OK;
 }
 
@@ -427,6 +427,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
             float *row_loss, float *lse, float *loss) {
     if (int rc = check(who, m, n, k, a, lda, b, ldb_, selected)) return rc;
     if (!loss || (m && (!row_loss || !lse))) return fail(SWC_HIP_EINVAL, "%s: null output", who);
+    if (m && (row_loss == lse || row_loss == loss || lse == loss)) return fail(SWC_HIP_EINVAL, "%s: two outputs are the same", who);
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
     if (m == 0 || n == 0) {   // no rows, or no classes: every row is left out
         if (int rc = zero_rows(row_loss, m, m ? 1 : 0, m)) return rc;
@@ -467,6 +468,7 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
     const void *in[3] = {a, b, bias};
     for (const void *p : in)
         if (p && (p == da || p == db || p == dbias)) return fail(SWC_HIP_EINVAL, "%s: an output is also an input", who);
+    if ((da && (da == db || da == dbias)) || (db && db == dbias)) return fail(SWC_HIP_EINVAL, "%s: two outputs are the same", who);
     if (!ready()) return fail(SWC_HIP_ENOTINIT, "%s: swc_hip_init has not been called", who);
     if (!da && !db && !dbias) return SWC_HIP_OK;
     if (m == 0 || n == 0) {

@@ -71,8 +71,10 @@ constexpr int kSliceBytes = 128, kStepBytes = 32, kSteps = kSliceBytes / kStepBy
 template <class T> constexpr int kSlice = kSliceBytes / (int)sizeof(T);   // contraction indices of a slice
 template <class T> constexpr int kChunk = 16 / (int)sizeof(T);            // elements of a 16-byte chunk
 
-// largest leading dimension whose tile offsets stay inside 31 bits (256 rows of it)
+// largest leading dimension whose tile offsets stay inside 31 bits (256 rows of it), and most rows: indices of tiles, ranges
+// of a contraction and slices loaded past its end all stay inside 31 bits
 template <class T> constexpr long kMaxLd = (1L << 31) / (256 * (long)sizeof(T)) - 64;
+constexpr int kMaxRows = 1 << 30;
 
 template <class T> struct Shape {
     const T *a;
@@ -641,7 +643,8 @@ struct StorePartial {
 template <class T, class C, Layout LA, Layout LB, class Ep>
 int launch_product(const Shape<T> &s, int splits, const Ep &ep, const char *who) {
     const long tiles = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN);
-    if (tiles > 0x7fffffffL || splits > 65535) return fail(SWC_HIP_EINVAL, "%s: too many tiles", who);
+    // (a grid has at most 2^32 - 1 threads in each direction)
+    if (tiles > 0xffffffffL / C::kThreads || splits > 65535) return fail(SWC_HIP_EUNSUPPORTED, "%s: too many tiles", who);
     note_kernel("product<%s,%dx%d,%d,%d,%s%s> x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, C::SA, C::SB, LA == kAlongK ? "k" : "m",
                 LB == kAlongK ? "k" : "n", splits);
     auto kern = product_tiles<T, C, LA, LB, Ep>;

@@ -126,7 +126,7 @@ void *workspace(size_t bytes, const char *who) {
     if (!g.ws_auto) {
         fail(SWC_HIP_EINVAL, "%s: needs %zu bytes of scratch memory and no workspace is set: size one with "
              "swc_hip_gemm_workspace_bytes / swc_hip_conv2d_workspace_bytes / swc_hip_conv2dGrad_workspace_bytes / "
-             "swc_hip_matrixSoftmaxWithLoss_workspace_bytes and pass it to swc_hip_set_workspace (ops do not allocate; "
+             "swc_hip_matrixSoftmaxWithLoss_workspace_bytes / the entry point's own _workspace_bytes query and pass it to swc_hip_set_workspace (ops do not allocate; "
              "swc_hip_enable_auto_workspace lets the library keep a buffer of its own)", who, bytes);
         return nullptr;
     }

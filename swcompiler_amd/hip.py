@@ -4,7 +4,10 @@ Method names and argument order mirror the reference's CPU kernels
 (src/codegen/utils/kernels.h) — the same correspondence the C ABI keeps — so a
 parity test reads like a call sequence of the reference's generated program.
 Data lives in DeviceArray objects (device memory + shape); numpy arrays cross
-only through upload()/download().
+only through upload()/download().  The operators of language models take torch tensors too, as
+they are; a program that uses torch imports it before this library is loaded
+(torch brings a HIP runtime of its own, and a process has one), and shares its
+stream (use_default_stream) or synchronises between the two.
 
 No fallback: a missing library or device raises SwcHipError.
 """
@@ -182,6 +185,13 @@ def pool_out_dims(idims, kernels, strides, pads):
             (w + pads[1] + pads[3] - kernels[1]) // strides[1] + 1, c)
 
 
+def _int32(x, what):
+    """x where the library takes a 32-bit int (ctypes would cut a larger one off without a word)"""
+    if x > 0x7fffffff:
+        raise SwcHipError(f"{what}: {x} is beyond 2^31 - 1")
+    return x
+
+
 class _Arg:
     """What an op needs of an operand: its address, shape, element type and row stride.  Operands are DeviceArrays or
     torch tensors on the runtime's device (taken as they are: any row stride, columns contiguous)."""
@@ -204,6 +214,7 @@ class _Arg:
             self.ld = stride[0]
             if self.ld < shape[1]:
                 raise SwcHipError(f"{what}: rows overlap (stride {self.ld}, {shape[1]} columns)")
+            _int32(self.ld, what + ": row stride")
 
 
 def _torch_operand(rt, x, what):
@@ -708,7 +719,8 @@ class SwcHip:
         a, b = self._arg(a, what + ": a", ("f32", "bf16")), self._arg(b, what + ": b", ("f32", "bf16"))
         if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0] or a.type != b.type:
             raise SwcHipError(f"{what}: a {a.shape} {a.type} and b {b.shape} {b.type} do not multiply")
-        return a, b, a.shape[0], b.shape[1], a.shape[1], (a.type,), "_f" if a.type == "f32" else "_bf"
+        m, n, k = _int32(a.shape[0], what), _int32(b.shape[1], what), _int32(a.shape[1], what)
+        return a, b, m, n, k, (a.type,), "_f" if a.type == "f32" else "_bf"
 
     @staticmethod
     def _activation(act):
@@ -839,7 +851,10 @@ class SwcHip:
             pointers = [pw, pg, pm, pv]
         pointers.append(None if copies is None else addresses(copies, ("bf16",), sizes, "copies")[0])
         sizes = (C.c_size_t * count)(*sizes)
-        one = [self._p(self._arg(x, f"{what}: factor", ("f32",))) for x in (lr_factor, grad_factor)]
+        factors = [self._arg(x, f"{what}: factor", ("f32",)) for x in (lr_factor, grad_factor)]
+        if any(x is not None and x.size != 1 for x in factors):
+            raise SwcHipError(f"{what}: a factor is one value")
+        one = [self._p(x) for x in factors]
         fn = getattr(self.lib, f"swc_hip_{what}" + ("_bf" if dtype == "bf16" else "_f"))
         self._check(fn(count, *pointers, sizes, self._state(state, what), lr, beta1, beta2, eps, decay, *one), what)
 

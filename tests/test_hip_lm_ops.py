@@ -11,6 +11,8 @@ lost element at the edge of a tile.
 import ctypes as C
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -121,6 +123,7 @@ EINVAL, EUNSUPPORTED, ENOTINIT = 1, 2, 4
 P = C.c_void_p(1 << 20)   # an address that is never followed: every call below is refused before it starts work
 Q = C.c_void_p(2 << 20)
 R = C.c_void_p(3 << 20)
+S, T = C.c_void_p(4 << 20), C.c_void_p(5 << 20)
 
 
 def fc_args(m=4, n=8, k=8, a=P, lda=8, b=Q, ldb=8, bias=None, act=0, res=None, ldr=0, pre=None, ldp=0, c=R, ldc=8):
@@ -132,7 +135,7 @@ def fc_grad_args(m=4, n=8, k=8, dc=P, lddc=8, a=Q, lda=8, b=Q, ldb=8, pre=None, 
     return m, n, k, dc, lddc, a, lda, b, ldb, pre, ldp, act, da, ldda, db, lddb, dbias
 
 
-def loss_args(m=4, n=8, k=8, a=P, lda=8, b=Q, ldb=8, bias=None, sel=Q, row=R, lse=R, loss=R):
+def loss_args(m=4, n=8, k=8, a=P, lda=8, b=Q, ldb=8, bias=None, sel=Q, row=R, lse=S, loss=T):
     return m, n, k, a, lda, b, ldb, bias, sel, row, lse, loss
 
 
@@ -144,14 +147,18 @@ def loss_grad_args(m=4, n=8, k=8, a=P, lda=8, b=Q, ldb=8, bias=None, sel=Q, lse=
 REFUSED = [
     ("matrixMatrixFCActAdd", fc_args, [dict(m=-1), dict(act=5), dict(act=-1), dict(a=None), dict(c=None), dict(lda=7),
                                        dict(ldb=7), dict(ldc=7), dict(res=Q, ldr=7), dict(pre=Q, ldp=7), dict(c=P), dict(c=Q),
-                                       dict(pre=R, ldp=8)]),
+                                       dict(pre=R, ldp=8), dict(bias=R), dict(pre=P, ldp=8), dict(bias=P, pre=P, ldp=8),
+                                       dict(res=R, ldr=9), dict(res=P, pre=P, ldp=8, ldr=8)]),
     ("matrixMatrixFCActAddGrad", fc_grad_args, [dict(n=-1), dict(act=9), dict(dc=None), dict(act=2), dict(act=2, pre=P, ldp=7),
                                                 dict(b=None), dict(db=R, lddb=8, a=None), dict(lddc=7), dict(ldda=7),
-                                                dict(db=R, lddb=7), dict(da=P), dict(db=Q, lddb=8), dict(dbias=P)]),
+                                                dict(db=R, lddb=7), dict(da=P), dict(db=Q, lddb=8), dict(dbias=P),
+                                                dict(db=R, lddb=8), dict(dbias=R), dict(da=None, db=R, lddb=8, dbias=R)]),
     ("matrixFCSoftmaxWithLoss", loss_args, [dict(k=-1), dict(sel=None), dict(a=None), dict(b=None), dict(lda=7), dict(ldb=7),
-                                            dict(row=None), dict(lse=None), dict(loss=None), dict(k=0)]),
+                                            dict(row=None), dict(lse=None), dict(loss=None), dict(k=0),
+                                            dict(lse=R), dict(loss=R), dict(loss=S)]),
     ("matrixFCSoftmaxWithLossGrad", loss_grad_args, [dict(m=-1), dict(sel=None), dict(lse=None), dict(a=None), dict(ldda=7),
-                                                     dict(db=R, lddb=7), dict(da=P), dict(dbias=Q), dict(k=0)]),
+                                                     dict(db=R, lddb=7), dict(da=P), dict(dbias=Q), dict(k=0),
+                                                     dict(db=R, lddb=8), dict(dbias=R), dict(da=None, db=R, lddb=8, dbias=R)]),
 ]
 
 
@@ -171,6 +178,19 @@ def test_refused_sizes():
     assert lib().swc_hip_matrixFCSoftmaxWithLoss_bf(*loss_args(ldb=far)) == EUNSUPPORTED
     assert lib().swc_hip_matrixFCSoftmaxWithLoss_f(*loss_args(m=5_000_000)) == EUNSUPPORTED
     assert lib().swc_hip_matrixFCSoftmaxWithLossGrad_bf(*loss_grad_args(m=5_000_000)) == EUNSUPPORTED
+    assert lib().swc_hip_matrixMatrixFCActAdd_f(*fc_args(m=(1 << 30) + 1)) == EUNSUPPORTED
+    assert lib().swc_hip_matrixMatrixFCActAddGrad_f(*fc_grad_args(m=(1 << 30) + 1)) == EUNSUPPORTED
+    # (a matrix that is not needed has no row length to be refused for, the dimension has)
+    assert lib().swc_hip_matrixMatrixFCActAddGrad_bf(*fc_grad_args(k=far, a=None, lda=0, ldda=far)) == EUNSUPPORTED
+    assert lib().swc_hip_matrixMatrixFCActAdd_bf(*fc_args(n=far, k=0, ldc=far)) == EUNSUPPORTED
+
+
+def test_adamw_refuses_sizes_and_repeats():
+    for name in ("adamw_f", "adamw8_bf"):
+        assert adamw_call(name, sizes=(17179868161,)) == EUNSUPPORTED
+    two, sizes = (C.c_void_p * 2)(P.value, P.value), (C.c_size_t * 2)(5, 5)
+    call = lambda w, n: lib().swc_hip_adamw_f(2, w, two, two, two, None, n, P, 1e-3, 0.9, 0.99, 1e-8, 0.0, None, None)   # noqa: E731
+    assert call(two, sizes) == EINVAL and b"twice" in lib().swc_hip_last_error()
 
 
 def adamw_call(name, count=1, w=P, dw=P, mom=P, var=P, scale=P, sizes=(5,), state=P, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8,
@@ -250,6 +270,10 @@ def test_binding_refuses():
     with pytest.raises(SwcHipError, match="elements, expected 2"):
         u = lambda n: e(n, dtype=np.uint8)   # noqa: E731
         rt.adamw8([e(257)], [e(257)], [u(257)], [e(1)], [u(257)], [e(2)], state, 1e-3, 0.9, 0.99, 1e-8, 0.0)
+    with pytest.raises(SwcHipError, match="a factor is one value"):
+        rt.adamw([e(3)], [e(3)], [e(3)], [e(3)], state, 1e-3, 0.9, 0.99, 1e-8, 0.0, grad_factor=e(2))
+    with pytest.raises(SwcHipError, match="beyond 2"):
+        rt.matrixMatrixFCActAdd(e(1 << 31, 1), e(1, 1))
     with pytest.raises(SwcHipError, match="state: shape"):
         rt.adamwAdvance(e(7, dtype=np.int32), 0.9, 0.99)
 
@@ -290,6 +314,36 @@ def test_fc_integers_bit_exact(rt, kind, m, n, k):
         np.testing.assert_array_equal(kind.down(c), kind.values(act64(z, act) + res))
     plain = rt.matrixMatrixFCActAdd(kind.up(rt, a), kind.up(rt, b))
     np.testing.assert_array_equal(kind.down(plain), kind.values(z - bias))
+
+
+# few rows: the forms for decoding and the first sizes beyond them; contractions of less than a wavefront's share to several
+# rounds of all of them, whole slices and not, and past the longest of them
+FEW_SHAPES = [(2, 520, 64), (8, 33, 72), (3, 1000, 1088), (4, 72, 2056), (5, 264, 3080), (8, 130, 4096), (1, 48, 8192), (8, 40, 8192),
+              (8, 72, 8200), (9, 520, 4096), (2, 4104, 1028), (4, 4099, 513)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pad", [0, 8, 3])
+@pytest.mark.parametrize("m,n,k", FEW_SHAPES)
+def test_fc_few_rows_bit_exact(rt, kind, pad, m, n, k):
+    print("case fc few", kind.name, pad, m, n, k, flush=True)
+    rng = np.random.default_rng(m * 7 + n * 3 + k)
+    a, b, res = small_ints(rng, m, k), small_ints(rng, k, n), small_ints(rng, m, n, top=9)
+    bias = small_ints(rng, n)
+    dbias = kind.up(rt, bias)
+    da, pa = strided(rt, kind, a, k + pad)
+    db, pb = strided(rt, kind, b, n + pad)
+    dr, pr = strided(rt, kind, res, n + pad)
+    dz, pz = strided(rt, kind, np.zeros((m, n)), n + pad)
+    dc, pc = strided(rt, kind, np.zeros((m, n)), n + pad)
+    fn = getattr(rt.lib, "swc_hip_matrixMatrixFCActAdd" + kind.suffix())
+    rt._check(fn(m, n, k, pa, k + pad, pb, n + pad, dbias.ptr, 1, pr, n + pad, pz, n + pad, pc, n + pad), "fc")
+    z = a.astype(np.float64) @ b + bias
+    for d, want in ((dz, z), (dc, np.maximum(z, 0) + res)):
+        inside, beside, behind = rows_of(kind, d, m, n, n + pad)
+        np.testing.assert_array_equal(inside, kind.values(want))
+        assert np.all(np.isnan(beside)) and np.all(np.isnan(behind))
 
 
 def fc_bound(a, b, bias, res, z, value, kind):
@@ -444,6 +498,18 @@ def test_fc_grad_integers_bit_exact(rt, kind, m, n, k):
         np.testing.assert_array_equal(kind.down(da), kind.values(dz.astype(np.float64) @ b.T))
         np.testing.assert_array_equal(kind.down(db), kind.values(a.T.astype(np.float64) @ dz))
         np.testing.assert_array_equal(kind.down(dbias), kind.values(dz.sum(0, dtype=np.float64)))
+
+
+@gpu
+def test_fc_grad_many_rows(rt):
+    """more rows than a grid's second direction has workgroups of 32 (65535): exact integers all the same"""
+    rng = np.random.default_rng(9)
+    m, n, k = 65535 * 32 + 1, 8, 8
+    dc, a, b = (rng.integers(-1, 2, s).astype(np.float32) for s in ((m, n), (m, k), (k, n)))
+    da, db, dbias = (x.numpy() for x in rt.matrixMatrixFCActAddGrad(rt.upload(dc), rt.upload(a), rt.upload(b)))
+    np.testing.assert_array_equal(da, dc @ b.T)
+    np.testing.assert_array_equal(db, a.T.astype(np.float64) @ dc)
+    np.testing.assert_array_equal(dbias, dc.sum(0, dtype=np.float64))
 
 
 def fc_grad_bounds(dz, a, b, kind, slack):
@@ -626,7 +692,8 @@ def test_loss_and_gradients(rt, kind, m, n, k):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("m,n,k,share", [(70, 301, 72, 0.5), (300, 1000, 64, 0.9), (33, 40, 16, 1.0), (1030, 130, 40, 0.3)])
+@pytest.mark.parametrize("m,n,k,share", [(70, 301, 72, 0.5), (300, 1000, 64, 0.9), (33, 40, 16, 1.0), (1030, 130, 40, 0.3),
+                                         (4096, 70, 24, 0.1), (4097, 70, 24, 0.1), (6000, 100, 19, 0.6)])
 def test_loss_rows_left_out(rt, kind, m, n, k, share):
     """rows whose class lies outside the vocabulary bring nothing, whatever they hold: here infinities and NaN"""
     print("case loss left out", kind.name, m, n, k, share, flush=True)
@@ -640,6 +707,18 @@ def test_loss_rows_left_out(rt, kind, m, n, k, share):
     grad[out] = np.nan
     with np.errstate(invalid="ignore"):
         check_loss(rt, kind, a, b, kind.values(rng.standard_normal(n)), sel, grad)
+
+
+@gpu
+@pytest.mark.parametrize("kind,m", [pytest.param(F32, 2900, id="f32"), pytest.param(BF, 5800, id="bf16")])
+def test_loss_gradient_in_pieces(rt, kind, m):
+    """a vocabulary whose dz does not fit the workspace's 256 MiB at once: two pieces, the second of 260 classes"""
+    rng = np.random.default_rng(31)
+    n, k = 23300, 16
+    a, b = kind.values(rng.standard_normal((m, k))), kind.values(rng.standard_normal((k, n)) / 2)
+    sel = rng.integers(-1, n, m)
+    sel[:40] = rng.integers(23040, n, 40)
+    check_loss(rt, kind, a, b, kind.values(rng.standard_normal(n)), sel, rng.standard_normal(m).astype(np.float32))
 
 
 @gpu
@@ -960,7 +1039,80 @@ def test_adamw_unaligned(rt, kind):
     np.testing.assert_array_equal(dc.numpy()[inside], to_bf16(got[inside]))
 
 
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+def test_adamw_large(rt, grads):
+    """a call large enough to go past the caches gives the bits of calls on its parts"""
+    rng = np.random.default_rng(17)
+    n, cut = 17_000_003, 5120 * ADAMW_BLOCK
+    w, g = rng.standard_normal(n).astype(np.float32), grads.values(rng.standard_normal(n).astype(np.float32))
+    state = rt.adamw_state()
+    rt.adamwAdvance(state, RATES["beta1"], RATES["beta2"])
+    dg = grads.up(rt, g)
+    one, two = ([rt.upload(w), rt.upload(np.zeros(n, np.float32)), rt.upload(np.zeros(n, np.float32))] for _ in range(2))
+    rt.adamw([one[0]], [dg], [one[1]], [one[2]], state, **RATES)
+    for at, size in ((0, cut), (cut, 9_000_001), (cut + 9_000_001, n - cut - 9_000_001)):
+        v = [x.offset_view(at, (size,)) for x in two]
+        rt.adamw([v[0]], [dg.offset_view(at, (size,))], [v[1]], [v[2]], state, **RATES)
+    for x, y in zip(one, two):
+        np.testing.assert_array_equal(x.numpy(), y.numpy())
+    # 8 bits: the random numbers are an element's in its tensor, so only the first part is the same
+    count = -(-n // ADAMW_BLOCK)
+    one, two = ([rt.upload(w), rt.upload(np.zeros(n, np.uint8)), rt.upload(np.zeros(n, np.uint8)), rt.upload(np.zeros(count, np.float32)),
+                 rt.upload(np.zeros(count, np.float32))] for _ in range(2))
+    rt.adamw8([one[0]], [dg], [one[1]], [one[3]], [one[2]], [one[4]], state, **RATES)
+    v = [x.offset_view(0, (cut,)) for x in two[:3]] + [x.offset_view(0, (cut // ADAMW_BLOCK,)) for x in two[3:]]
+    rt.adamw8([v[0]], [dg.offset_view(0, (cut,))], [v[1]], [v[3]], [v[2]], [v[4]], state, **RATES)
+    for x, y in zip(one[:3], two):
+        np.testing.assert_array_equal(x.numpy()[:cut], y.numpy()[:cut])
+    assert one[0].numpy()[-1] != w[-1]
+
+
 # ---------------------------------------------------------------- together, workspaces, graphs and streams
+TORCH_VIEWS = """
+import torch
+assert torch.cuda.is_available()
+from swcompiler_amd.hip import SwcHipError, runtime
+rt = runtime()
+gen = torch.Generator().manual_seed(3)
+base = torch.randint(-3, 4, (80, 200), generator=gen).to("cuda", torch.bfloat16)
+weight = torch.randint(-3, 4, (64, 136), generator=gen).to("cuda", torch.bfloat16)
+out, pre = torch.zeros(70, 300, device="cuda", dtype=torch.bfloat16), torch.zeros(140, 136, device="cuda", dtype=torch.bfloat16)
+torch.cuda.synchronize()
+a, c, z = base[5:75, 3:67], out[:, 100:236], pre[::2]
+rt.matrixMatrixFCActAdd(a, weight, None, "relu", None, z, c)
+rt.sync()
+want = a.float().cpu() @ weight.float().cpu()
+assert torch.equal(z.float().cpu(), want.bfloat16().float())
+assert torch.equal(c.float().cpu(), want.clamp(min=0).bfloat16().float())
+assert not out[:, :100].any() and not out[:, 236:].any() and not pre[1::2].any()
+rt.use_default_stream()     # torch's: no waits between its work and the library's
+for _ in range(20):
+    x = base[:70, :64] * 2
+    y = torch.empty(70, 136, device="cuda", dtype=torch.bfloat16)
+    rt.matrixMatrixFCActAdd(x, weight, out=y)
+    y = y - (x.float() @ weight.float()).bfloat16()
+    assert not y.any()
+for bad, message in ((weight.t(), "not contiguous"), (a[:1].expand(70, 64), "rows overlap")):
+    try:
+        rt.matrixMatrixFCActAdd(bad, base[:bad.shape[1], :8].contiguous())
+    except SwcHipError as e:
+        assert message in str(e), e
+    else:
+        raise AssertionError(message)
+print("views done")
+"""
+
+
+@gpu
+def test_torch_views():
+    """torch tensors as they are: columns of a wider one, rows of a longer one, outputs too; on torch's own stream.  In a
+    process of its own: torch brings its own HIP runtime, which has to be the first one loaded"""
+    done = subprocess.run([sys.executable, "-c", TORCH_VIEWS],
+                          cwd=ROOT, capture_output=True, text=True, timeout=110)
+    assert done.returncode == 0 and "views done" in done.stdout, done.stderr[-2000:]
+
+
 def make_step(rt, rng, kind, m=150, d=72, h=200, n=1003):
     """a small language-model step: two layers with a residual, the loss, all gradients, AdamW on fp32 weights with
     bfloat16 copies feeding the products -> (run, parameters, everything the step writes)"""
