@@ -127,6 +127,26 @@ int grad_product(const char *who, const Plan &p, const Shape<T> &s, T *out, long
     return join_parts<T>(out, ld, part, p.splits, s.m, s.n);
 }
 
+// Both products in one launch, where both take 64 x 64 tiles and all of their workgroups fit the chip at once: 512 x 1024 x 784
+// fp32 37.9 us in two launches, 33.5 in one, bf16 18.7 and 14.5.
+bool pairs(const Plan &pa, const Plan &pb, int m, int n, int k) {
+    auto groups = [](const Plan &p, long rows, long cols) { return ((rows + 63) / 64) * ((cols + 63) / 64) * p.splits; };
+    return pa.kind == kSmall && pb.kind == kSmall && groups(pa, m, k) + groups(pb, k, n) <= 3L * num_cus();
+}
+template <class T>
+int pair_product(const Plan &pa, Shape<T> sa, T *da, long ldda, float *part_a, const Plan &pb, Shape<T> sb, T *db, long lddb, float *part_b) {
+    sa.k_per_split = pa.k_per_split, sb.k_per_split = pb.k_per_split;
+    auto ends = [](const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
+        return StoreEither<T>{{out, ld}, {p.splits > 1 ? part : nullptr, (long)s.m * s.n, s.n, false}};
+    };
+    if (int rc = launch_pair<T, Small, kAlongK, kAlongK, kAcross, kAcross>(sa, pa.splits, ends(pa, sa, da, ldda, part_a), sb, pb.splits,
+                                                                          ends(pb, sb, db, lddb, part_b)))
+        return rc;
+    if (pa.splits > 1)
+        if (int rc = join_parts<T>(da, ldda, part_a, pa.splits, sa.m, sa.n)) return rc;
+    return pb.splits > 1 ? join_parts<T>(db, lddb, part_b, pb.splits, sb.m, sb.n) : (int)SWC_HIP_OK;
+}
+
 template <class T>
 int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda_, const T *b, int ldb_, const T *preact,
               int ldp, int act, T *da, int ldda, T *db, int lddb, T *dbias) {
@@ -145,7 +165,9 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
     const bool tail = da && n % kChunk<T>;
     const bool own_dz = (da || db) && (act != SWC_HIP_ACT_NONE || !aligned_rows(dc, lddc) || tail);
     const bool pack_a = db && !aligned_rows(a, lda), pack_b = da && (!aligned_rows(b, ldb) || tail);
-    const size_t partials = larger(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
+    const bool pair = da && db && pairs(pa, pb, m, n, k);
+    const size_t partials = pair ? pa.partial_bytes(m, k) + pb.partial_bytes(k, n)
+                                 : larger(da ? pa.partial_bytes(m, k) : 0, db ? pb.partial_bytes(k, n) : 0);
     const size_t need = space<T>(nullptr, m, n, k, own_dz, pack_a, pack_b, partials, dbias).bytes;
     Space<T> w{};
     if (need) {
@@ -165,15 +187,22 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
         return rc;
     if (pack_a) a = w.a, lda = row_length<T>(k);
     if (pack_b) b = w.b, ldb = padded;
+    const Shape<T> sa{dz, b, lddz, ldb, m, k, n, 0, nullptr}, sb{a, dz, lda, lddz, k, n, m, 0, nullptr};
+    if (pair) return pair_product<T>(pa, sa, da, ldda, w.part, pb, sb, db, lddb, w.part + pa.partial_bytes(m, k) / sizeof(float));
     if (da)
-        if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, {dz, b, lddz, ldb, m, k, n, 0, nullptr}, da, ldda, w.part)) return rc;
+        if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, sa, da, ldda, w.part)) return rc;
     if (db)
-        if (int rc = grad_product<kAcross, kAcross, T>(who, pb, {a, dz, lda, lddz, k, n, m, 0, nullptr}, db, lddb, w.part)) return rc;
+        if (int rc = grad_product<kAcross, kAcross, T>(who, pb, sb, db, lddb, w.part)) return rc;
     return SWC_HIP_OK;
 }
 
 template <class T> size_t most(int m, int n, int k) {
-    const size_t partials = k > 0 ? larger(plan_product<T>(m, k, n).partial_bytes(m, k), plan_product<T>(k, n, m).partial_bytes(k, n)) : 0;
+    size_t partials = 0;
+    if (k > 0) {
+        const Plan pa = plan_product<T>(m, k, n), pb = plan_product<T>(k, n, m);
+        const size_t a = pa.partial_bytes(m, k), b = pb.partial_bytes(k, n);
+        partials = pairs(pa, pb, m, n, k) ? a + b : larger(a, b);
+    }
     return space<T>(nullptr, m, n, k > 0 ? k : 0, true, true, true, partials, true).bytes;
 }
 

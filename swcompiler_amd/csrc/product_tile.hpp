@@ -533,10 +533,9 @@ template <class T, class P> struct ColumnData {
 // Workgroup id -> tile: ids that land on one XCD (every eighth) are renumbered to be consecutive, and consecutive ids walk
 // the tiles in column strips four tall, so the 32 tiles an XCD holds at a time are 4 x 8: they share operand tiles in its
 // L2.  (Strips of 8: 4096 x 16384 x 4096 442 us against 430, 8192^3 the same; of 16: 494.)
-__device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int &tile_m, int &tile_n) {
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &tile_m, int &tile_n) {
     const int total = tiles_m * tiles_n;
     constexpr int kXcd = swc::devices::HipDevice::xcds, kStrip = 4;
-    int id = blockIdx.x;
     if (total % kXcd == 0) id = (id % kXcd) * (total / kXcd) + id / kXcd;
     const int strip = id / (kStrip * tiles_n), first = strip * kStrip;
     const int rows = tiles_m - first < kStrip ? tiles_m - first : kStrip;
@@ -547,10 +546,9 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int &tile_m, i
 
 // An epilogue receives, once per wavefront, its accumulators and where they lie:
 //     ep.template finish<P>(acc, row0, col0, m, n, lane, split): P a Place, (row0, col0) the wavefront's part of C
-template <class T, class C, Layout LA, Layout LB, class Ep>
-__global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) {
 #if __HIP_DEVICE_COMPILE__
-    extern __shared__ __align__(16) char lds_bytes[];
+template <class T, class C, Layout LA, Layout LB, class Ep>
+__device__ __forceinline__ void product_tile(const Shape<T> &s, const Ep &ep, int id, int split, char *lds_bytes) {
     int m = s.m, k = s.k;
     if (s.rows) {   // rows left out of a loss: the count is known on the device only
         const int have = __builtin_amdgcn_readfirstlane(*s.rows);
@@ -558,10 +556,10 @@ __global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) 
         else k = have < k ? have : k;
     }
     int tile_m, tile_n;
-    tile_of((s.m + C::BM - 1) / C::BM, (s.n + C::BN - 1) / C::BN, tile_m, tile_n);
+    tile_of(id, (s.m + C::BM - 1) / C::BM, (s.n + C::BN - 1) / C::BN, tile_m, tile_n);
     const int m0 = tile_m * C::BM, n0 = tile_n * C::BN;
     if (m0 >= m) return;
-    const int k_begin = blockIdx.y * s.k_per_split;
+    const int k_begin = split * s.k_per_split;
     const int k_end = k_begin + s.k_per_split < k ? k_begin + s.k_per_split : k;
     v16f acc[C::TM][C::TN];
     if (k_begin < k_end) {
@@ -576,7 +574,25 @@ __global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) 
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ep.template finish<Place<T, LA, LB, C::TM, C::TN>>(acc, m0 + (wave / C::WN) * 32 * C::TM, n0 + (wave % C::WN) * 32 * C::TN, m, s.n,
-                                                       (int)(threadIdx.x & 63), (int)blockIdx.y);
+                                                       (int)(threadIdx.x & 63), split);
+}
+#endif
+
+template <class T, class C, Layout LA, Layout LB, class Ep>
+__global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) {
+#if __HIP_DEVICE_COMPILE__
+    extern __shared__ __align__(16) char lds_bytes[];
+    product_tile<T, C, LA, LB>(s, ep, (int)blockIdx.x, (int)blockIdx.y, lds_bytes);
+#endif
+}
+// Two products in one launch, the second's workgroups behind the first's `groups`, each with its tiles split by split.
+template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
+__global__ __launch_bounds__(C::kThreads) void product_pair(Shape<T> s, Ep ep, int tiles, int groups, Shape<T> s2, Ep ep2, int tiles2) {
+#if __HIP_DEVICE_COMPILE__
+    extern __shared__ __align__(16) char lds_bytes[];
+    const int id = blockIdx.x;
+    if (id < groups) product_tile<T, C, LA, LB>(s, ep, id % tiles, id / tiles, lds_bytes);
+    else product_tile<T, C, LC, LD>(s2, ep2, (id - groups) % tiles2, (id - groups) / tiles2, lds_bytes);
 #endif
 }
 
@@ -640,6 +656,19 @@ struct StorePartial {
 #endif
 };
 
+// the one or the other: partial sums where `part.out` is given
+template <class T> struct StoreEither {
+    Store<T> whole;
+    StorePartial part;
+#if __HIP_DEVICE_COMPILE__
+    template <class P, int TM, int TN>
+    __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int split) const {
+        if (part.out) part.finish<P>(acc, row0, col0, m, n, lane, split);
+        else whole.template finish<P>(acc, row0, col0, m, n, lane, split);
+    }
+#endif
+};
+
 template <class T, class C, Layout LA, Layout LB, class Ep>
 int launch_product(const Shape<T> &s, int splits, const Ep &ep, const char *who) {
     const long tiles = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN);
@@ -655,6 +684,23 @@ int launch_product(const Shape<T> &s, int splits, const Ep &ep, const char *who)
         attr_set = true;
     }
     kern<<<dim3((unsigned)tiles, (unsigned)splits), C::kThreads, C::kLdsBytes, stream()>>>(s, ep);
+    SWC_LAUNCH_CHECK();
+    return SWC_HIP_OK;
+}
+
+template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
+int launch_pair(const Shape<T> &s, int splits, const Ep &ep, const Shape<T> &s2, int splits2, const Ep &ep2) {
+    auto tiles = [](const Shape<T> &x) { return ((x.m + C::BM - 1) / C::BM) * ((x.n + C::BN - 1) / C::BN); };
+    note_kernel("product_pair<%s,%dx%d> x%d x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, splits, splits2);
+    auto kern = product_pair<T, C, LA, LB, LC, LD, Ep>;
+    static bool attr_set = false;
+    if (!attr_set) {
+        SWC_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                        C::kLdsBytes));
+        attr_set = true;
+    }
+    const int groups = tiles(s) * splits, groups2 = tiles(s2) * splits2;
+    kern<<<groups + groups2, C::kThreads, C::kLdsBytes, stream()>>>(s, ep, tiles(s), groups, s2, ep2, tiles(s2));
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
