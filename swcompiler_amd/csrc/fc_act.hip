@@ -20,6 +20,9 @@ template <class T, int ACT> struct FcEpilogue {
     const T *bias, *residual;
     T *preact, *c;
     long ldr, ldp, ldc;
+    FcEpilogue from(int j) const {
+        return {bias ? bias + j : nullptr, residual ? residual + j : nullptr, preact ? preact + j : nullptr, c + j, ldr, ldp, ldc};
+    }
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void end(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {

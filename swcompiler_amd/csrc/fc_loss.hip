@@ -135,6 +135,8 @@ template <class T> struct RowStats {
     float *picked;    // [row]: z of the row's class
     const int *sel;
     const T *bias;
+    int first;        // the product's first column
+    RowStats from(int j) const { return {part + j / 64, blocks, picked, sel, bias ? bias + j : nullptr, first + j}; }   // (64: Big's)
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void reduce(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -144,7 +146,7 @@ template <class T> struct RowStats {
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int row = row0 + P::row(tm, l32);
-            const int want = (row < m ? sel[row] : -1) - col0;
+            const int want = (row < m ? sel[row] : -1) - first - col0;
             float z[P::kValues];
             float top = -__builtin_inff();
 #pragma unroll
@@ -242,15 +244,17 @@ __global__ __launch_bounds__(1024) void mean_loss(const float2 *part, int blocks
 }
 
 // ---------------------------------------------------------------- gradients
-// dz of a piece of the vocabulary whose first class is `first`, zeros in the columns that pad it to whole 16 bytes
+// dz of a piece of the vocabulary, zeros in the columns that pad it to whole 16 bytes
 template <class T> struct StoreDz {
     static constexpr bool kHeavy = true, kThinToo = true;
     T *dz;
     long ld;
-    int first;
+    int width;       // columns of dz from the product's first one on
+    int first;       // class of that column
     const int *sel;
     const float *lse, *grad;
-    const T *bias;   // of the piece
+    const T *bias;   // from that class on
+    StoreDz from(int j) const { return {dz + j, ld, width - j, first + j, sel, lse, grad, bias ? bias + j : nullptr}; }
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -280,7 +284,7 @@ template <class T> struct StoreDz {
                 x[u] *= g;
                 if (!WHOLE && col0 + P::column(u, h) >= n) x[u] = 0.f;
             }
-            store_row<P, WHOLE>(dz + row * ld, ok, col0, (int)ld, h, x);
+            store_row<P, WHOLE>(dz + row * ld, ok, col0, width, h, x);
         }
     }
     template <class P, int TM, int TN>
@@ -367,7 +371,12 @@ Rows take_rows(Carver &c, int m, bool gradients) {
 
 // Whole rows of the contraction: the epilogues of this file need finished sums.
 template <class T> Plan whole_plan(int m, int n, int k) { return plan_product<T>(m, n, k, true); }
-int block_columns(const Plan &p) { return p.kind == kThin || p.kind == kSmall ? 32 : 64; }
+// blocks of columns that RowStats writes for a row
+int block_columns(Kind kind) { return kind == kThin || kind == kSmall ? 32 : 64; }
+int row_blocks(const Plan &p, int n) {
+    if (p.first > 0 && p.first < n) return p.first / block_columns(p.kind) + ceil_div(n - p.first, block_columns(p.rest));
+    return ceil_div(n, block_columns(p.kind));
+}
 static_assert(Big::TN == 2 && Mid::TN == 2 && Low::TN == 2 && Small::TN == 1 && Thin::TN == 1, "columns of a wavefront");
 
 template <class T> struct ForwardSpace {
@@ -383,7 +392,7 @@ template <class T> ForwardSpace<T> forward_space(char *base, const Plan &p, int 
     s.rows = take_rows(c, m, false);
     s.a = c.take<T>((size_t)m * row_length<T>(k));
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
-    s.part = c.take<float2>((size_t)m * ((n + block_columns(p) - 1) / block_columns(p)));
+    s.part = c.take<float2>((size_t)m * row_blocks(p, n));
     s.picked = c.take<float>(m);
     s.bytes = c.used;
     return s;
@@ -445,9 +454,9 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
         if (int rc = copy_operands<T>({}, {w.b, b, row_length<T>(n), ldb, k, n})) return rc;
         b = w.b, ldb = row_length<T>(n);
     }
-    const int blocks = (n + block_columns(p) - 1) / block_columns(p);
+    const int blocks = row_blocks(p, n);
     const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, w.rows.count};
-    if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias}, who)) return rc;
+    if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias, 0}, who)) return rc;
     if (m <= 64) {
         mean_loss<true><<<1, 1024, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse, loss);
     } else {
@@ -491,7 +500,7 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
         const int cols = n - first < w.piece ? n - first : w.piece;
         const long ld = row_length<T>(cols);
         const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, w.rows.count};
-        const StoreDz<T> ep{w.dz, ld, first, w.rows.sel, w.rows.lse, w.rows.grad, bias ? bias + first : nullptr};
+        const StoreDz<T> ep{w.dz, ld, (int)ld, first, w.rows.sel, w.rows.lse, w.rows.grad, bias ? bias + first : nullptr};
         if (int rc = run_product<kAlongK, kAcross>(whole_plan<T>(m, cols, k), z, ep, who)) return rc;
         if (da) {
             const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, w.rows.count};

@@ -17,6 +17,8 @@ enum Kind { kBig, kDeep, kMid, kLow, kSmall, kThin };
 struct Plan {
     Kind kind;
     int splits, k_per_split;
+    int first = 0;        // > 0: these columns on tiles of `kind`, those behind them on tiles of `rest`, uncut
+    Kind rest = kMid;
     size_t partial_bytes(int m, int n) const { return splits > 1 ? (size_t)splits * m * n * sizeof(float) : 0; }
 };
 
@@ -32,8 +34,8 @@ constexpr size_t kMaxPartials = (size_t)256 << 20;
 // joining), 512 x 4096 x 4096 24.4 (64 x 128 whole; 128 x 128 in two 23.0 and the joining), 2048 x 4096 x 4096 63.5 (128 x
 // 128; 256 x 256 83.2), 1400 x 1024 x 50264 175 (256 x 256 in eight; 128 x 128 in four 250).  An fp32 slice is half as many
 // products at a sixteenth of the rate: the matrix cores set its time.
-// one: only whole contractions.
-template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
+// one: only whole contractions.  The cost goes to *cost.
+template <class T> Plan plan_uniform(int m, int n, int k, bool one, double *cost_of) {
     struct Tile {
         Kind kind;
         int bm, bn, per_cu;
@@ -58,7 +60,8 @@ template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
             const int each = (slices + splits - 1) / splits, s = (slices + each - 1) / each;
             if (s > 1 && (one || each < 4 || (size_t)s * m * n * sizeof(float) > kMaxPartials)) break;
             const double groups = (double)tiles * s;
-            const double q = groups <= cus ? 1 : groups >= 4.0 * t.per_cu * cus ? groups / cus : (double)((long)((groups + cus - 1) / cus));
+            const bool smooth = t.per_cu > 1 && groups >= 4.0 * t.per_cu * cus;   // (ends that do not fall together)
+            const double q = groups <= cus ? 1 : smooth ? groups / cus : (double)((long)((groups + cus - 1) / cus));
             const double rounds = q <= t.per_cu ? 1 : q / t.per_cu;
             double work = each * (t.alone > q * t.busy ? t.alone : q * t.busy);
             work = work > operands ? work : operands;
@@ -67,17 +70,45 @@ template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
             if (cost < least) least = cost, best = Plan{t.kind, s, each * kPer};
         }
     }
+    *cost_of = least;
+    return best;
+}
+// A product on 256 x 256 tiles whose last round is a small part of the chip leaves the columns of that round to smaller tiles
+// in a second launch (3 us): bf16 8192 x 8800 x 4096 492 -> 472 us, 2048 x 9000 x 4096 158 -> 139, fp32 1999 x 50257 x 1024
+// 1811 -> 1681.
+template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
+    double cost = 0;
+    Plan best = plan_uniform<T>(m, n, k, one, &cost);
+    const int cus = num_cus();
+    const long tall = (m + 255) / 256, wide = (n + 255) / 256, rounds = tall * wide / cus, cols = rounds * cus / tall;
+    if (rounds > 0 && cols > 0 && cols < wide && m > 32) {
+        const double f = kIsBf16<T> ? 10.8 : 12, busy = kIsBf16<T> ? 1.2 : 7.2;
+        const int slices = (k + kSlice<T> - 1) / kSlice<T>, first = (int)cols * 256;
+        double tail = 0;
+        const Plan rest = plan_uniform<T>(m, n - first, k, true, &tail);
+        const double both = rounds * (f + slices * busy) + sizeof(T) * (double)m * first / 4.5e6 + tail + 3;
+        if (both < cost && rest.kind != kBig) best = Plan{kBig, 1, slices * kSlice<T>, first, rest.kind};
+    }
     // one wavefront per SIMD pays where the end of a tile is a small part of it: bf16 8192^3 785 -> 757 us, K = 4096 412 -> 417
     if (best.kind == kBig && kIsBf16<T> && best.k_per_split >= 6144) best.kind = kDeep;
     return best;
 }
 
-// The epilogues with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
+// An epilogue's from(j) is itself for the product's columns from j on.  Those with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
 // wavefront per SIMD has nothing beside it while they run; those without kThinToo never run on 32-row tiles.
 template <Layout LA, Layout LB, class T, class Ep>
 int run_product(const Plan &p, const Shape<T> &s, const Ep &ep, const char *who) {
     Shape<T> t = s;
     t.k_per_split = p.k_per_split;
+    if (p.first > 0 && p.first < s.n) {
+        Plan whole = p, rest = p;
+        whole.first = rest.first = 0, rest.kind = p.rest;
+        t.n = p.first;
+        if (int rc = run_product<LA, LB>(whole, t, ep, who)) return rc;
+        t.b += LB == kAlongK ? p.first * s.ldb : (long)p.first;
+        t.n = s.n - p.first;
+        return run_product<LA, LB>(rest, t, ep.from(p.first), who);
+    }
     if constexpr (!Ep::kHeavy && kIsBf16<T>)
         if (p.kind == kDeep) return launch_product<T, Deep, LA, LB>(t, p.splits, ep, who);
     if constexpr (Ep::kThinToo)

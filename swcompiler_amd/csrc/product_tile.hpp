@@ -601,6 +601,7 @@ template <class T> struct Store {
     static constexpr bool kHeavy = false, kThinToo = true;
     T *out;
     long ld;
+    Store from(int j) const { return {out + j, ld}; }
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -629,6 +630,7 @@ struct StorePartial {
     long split_stride;   // elements between the splits' matrices
     long ld;
     bool add;            // out += : a product summed over several calls
+    StorePartial from(int j) const { return {out + j, split_stride, ld, add}; }
 #if __HIP_DEVICE_COMPILE__
     template <class P, int TM, int TN>
     __device__ __forceinline__ void finish(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane, int split) const {
