@@ -400,7 +400,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda_, const T 
         return rc;
     if (pack_a) a = w.a, lda = row_length<T>(k);
     if (pack_b) b = w.b, ldb = row_length<T>(n);
-    const Shape<T> s{a, b, lda, ldb, m, n, k, 0, nullptr};
+    const Shape<T> s{a, b, lda, ldb, m, n, k, 0, 1, nullptr};
     if (!partial_sums(p)) {
         return with_act(act, [&]<int ACT>() {
             return run_product<kAlongK, kAcross>(p, s, FcEpilogue<T, ACT>{bias, residual, preact, c, ldr, ldp, ldc}, who);

@@ -135,11 +135,12 @@ bool pairs(const Plan &pa, const Plan &pb, int m, int n, int k) {
 }
 template <class T>
 int pair_product(const Plan &pa, Shape<T> sa, T *da, long ldda, float *part_a, const Plan &pb, Shape<T> sb, T *db, long lddb, float *part_b) {
-    sa.k_per_split = pa.k_per_split, sb.k_per_split = pb.k_per_split;
+    sa.k_per_split = pa.k_per_split, sa.splits = pa.splits;
+    sb.k_per_split = pb.k_per_split, sb.splits = pb.splits;
     auto ends = [](const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
         return StoreEither<T>{{out, ld}, {p.splits > 1 ? part : nullptr, (long)s.m * s.n, s.n, false}};
     };
-    if (int rc = launch_pair<T, Small, kAlongK, kAlongK, kAcross, kAcross>(sa, pa.splits, ends(pa, sa, da, ldda, part_a), sb, pb.splits,
+    if (int rc = launch_pair<T, Small, kAlongK, kAlongK, kAcross, kAcross>(sa, ends(pa, sa, da, ldda, part_a), sb,
                                                                           ends(pb, sb, db, lddb, part_b)))
         return rc;
     if (pa.splits > 1)
@@ -187,7 +188,7 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
         return rc;
     if (pack_a) a = w.a, lda = row_length<T>(k);
     if (pack_b) b = w.b, ldb = padded;
-    const Shape<T> sa{dz, b, lddz, ldb, m, k, n, 0, nullptr}, sb{a, dz, lda, lddz, k, n, m, 0, nullptr};
+    const Shape<T> sa{dz, b, lddz, ldb, m, k, n, 0, 1, nullptr}, sb{a, dz, lda, lddz, k, n, m, 0, 1, nullptr};
     if (pair) return pair_product<T>(pa, sa, da, ldda, w.part, pb, sb, db, lddb, w.part + pa.partial_bytes(m, k) / sizeof(float));
     if (da)
         if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, sa, da, ldda, w.part)) return rc;

@@ -455,7 +455,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
         b = w.b, ldb = row_length<T>(n);
     }
     const int blocks = row_blocks(p, n);
-    const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, w.rows.count};
+    const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, 1, w.rows.count};
     if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias, 0}, who)) return rc;
     if (m <= 64) {
         mean_loss<true><<<1, 1024, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse, loss);
@@ -499,15 +499,15 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
     for (int first = 0; first < n; first += w.piece) {
         const int cols = n - first < w.piece ? n - first : w.piece;
         const long ld = row_length<T>(cols);
-        const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, w.rows.count};
+        const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, 1, w.rows.count};
         const StoreDz<T> ep{w.dz, ld, (int)ld, first, w.rows.sel, w.rows.lse, w.rows.grad, bias ? bias + first : nullptr};
         if (int rc = run_product<kAlongK, kAcross>(whole_plan<T>(m, cols, k), z, ep, who)) return rc;
         if (da) {
-            const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, w.rows.count};
+            const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, 1, w.rows.count};
             if (int rc = run_product<kAlongK, kAlongK>(w.pa, s, StorePartial{w.da, (long)m * k, k, first > 0}, who)) return rc;
         }
         if (db) {
-            const Shape<T> s{w.a, w.dz, ldw, ld, k, cols, m, 0, w.rows.count};
+            const Shape<T> s{w.a, w.dz, ldw, ld, k, cols, m, 0, 1, w.rows.count};
             if (w.pb.splits == 1) {
                 const Store<T> out{db + first, lddb};
                 if (int rc = run_product<kAcross, kAcross>(w.pb, s, out, who)) return rc;

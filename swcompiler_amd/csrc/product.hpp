@@ -99,7 +99,7 @@ template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
 template <Layout LA, Layout LB, class T, class Ep>
 int run_product(const Plan &p, const Shape<T> &s, const Ep &ep, const char *who) {
     Shape<T> t = s;
-    t.k_per_split = p.k_per_split;
+    t.k_per_split = p.k_per_split, t.splits = p.splits;
     if (p.first > 0 && p.first < s.n) {
         Plan whole = p, rest = p;
         whole.first = rest.first = 0, rest.kind = p.rest;
@@ -110,14 +110,14 @@ int run_product(const Plan &p, const Shape<T> &s, const Ep &ep, const char *who)
         return run_product<LA, LB>(rest, t, ep.from(p.first), who);
     }
     if constexpr (!Ep::kHeavy && kIsBf16<T>)
-        if (p.kind == kDeep) return launch_product<T, Deep, LA, LB>(t, p.splits, ep, who);
+        if (p.kind == kDeep) return launch_product<T, Deep, LA, LB>(t, ep, who);
     if constexpr (Ep::kThinToo)
-        if (p.kind == kThin) return launch_product<T, Thin, LA, LB>(t, p.splits, ep, who);
+        if (p.kind == kThin) return launch_product<T, Thin, LA, LB>(t, ep, who);
     switch (p.kind) {
-    case kMid: return launch_product<T, Mid, LA, LB>(t, p.splits, ep, who);
-    case kLow: return launch_product<T, Low, LA, LB>(t, p.splits, ep, who);
-    case kSmall: return launch_product<T, Small, LA, LB>(t, p.splits, ep, who);
-    default: return launch_product<T, Big, LA, LB>(t, p.splits, ep, who);
+    case kMid: return launch_product<T, Mid, LA, LB>(t, ep, who);
+    case kLow: return launch_product<T, Low, LA, LB>(t, ep, who);
+    case kSmall: return launch_product<T, Small, LA, LB>(t, ep, who);
+    default: return launch_product<T, Big, LA, LB>(t, ep, who);
     }
 }
 

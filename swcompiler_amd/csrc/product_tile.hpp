@@ -81,7 +81,8 @@ template <class T> struct Shape {
     const T *b;
     long lda, ldb;
     int m, n, k;
-    int k_per_split;   // multiple of the slice; grid.y = number of splits
+    int k_per_split;   // multiple of the slice
+    int splits;        // ranges of the contraction
     const int *rows;   // device count of the rows (of A when along k, of both operands' contraction when across) that
                        // exist, at most m resp. k; null: all of them
 };
@@ -530,13 +531,17 @@ template <class T, class P> struct ColumnData {
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-// Workgroup id -> tile: ids that land on one XCD (every eighth) are renumbered to be consecutive, and consecutive ids walk
-// the tiles in column strips four tall, so the 32 tiles an XCD holds at a time are 4 x 8: they share operand tiles in its
-// L2.  (Strips of 8: 4096 x 16384 x 4096 442 us against 430, 8192^3 the same; of 16: 494.)
+// Workgroup id -> number of its work, of `total`: those that land on one XCD (every eighth) are consecutive.  Work is
+// numbered range by range of the contraction and tile by tile within one, and the tiles in column strips four tall, so that
+// the 32 tiles an XCD holds at a time are 4 x 8 of one range: they share operand tiles in its L2.  (Strips of 8: 4096 x 16384
+// x 4096 442 us against 430, 8192^3 the same; of 16: 494.)
+__device__ __forceinline__ int xcd_order(int id, int total) {
+    constexpr int kXcd = swc::devices::HipDevice::xcds;
+    const int x = id % kXcd, more = total % kXcd;
+    return x * (total / kXcd) + (x < more ? x : more) + id / kXcd;
+}
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &tile_m, int &tile_n) {
-    const int total = tiles_m * tiles_n;
-    constexpr int kXcd = swc::devices::HipDevice::xcds, kStrip = 4;
-    if (total % kXcd == 0) id = (id % kXcd) * (total / kXcd) + id / kXcd;
+    constexpr int kStrip = 4;
     const int strip = id / (kStrip * tiles_n), first = strip * kStrip;
     const int rows = tiles_m - first < kStrip ? tiles_m - first : kStrip;
     const int in = id - strip * kStrip * tiles_n;
@@ -548,17 +553,21 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &t
 //     ep.template finish<P>(acc, row0, col0, m, n, lane, split): P a Place, (row0, col0) the wavefront's part of C
 #if __HIP_DEVICE_COMPILE__
 template <class T, class C, Layout LA, Layout LB, class Ep>
-__device__ __forceinline__ void product_tile(const Shape<T> &s, const Ep &ep, int id, int split, char *lds_bytes) {
+__device__ __forceinline__ void product_tile(const Shape<T> &s, const Ep &ep, int id, char *lds_bytes) {
     int m = s.m, k = s.k;
     if (s.rows) {   // rows left out of a loss: the count is known on the device only
         const int have = __builtin_amdgcn_readfirstlane(*s.rows);
         if (LA == kAlongK) m = have < m ? have : m;
         else k = have < k ? have : k;
     }
+    // (of the tiles that exist: with rows left out their work would otherwise fall to some XCDs alone)
+    const int tiles_m = (m + C::BM - 1) / C::BM, tiles_n = (s.n + C::BN - 1) / C::BN, tiles = tiles_m * tiles_n;
+    if (id >= tiles * s.splits) return;
+    id = xcd_order(id, tiles * s.splits);
+    const int split = id / tiles;
     int tile_m, tile_n;
-    tile_of(id, (s.m + C::BM - 1) / C::BM, (s.n + C::BN - 1) / C::BN, tile_m, tile_n);
+    tile_of(id - split * tiles, tiles_m, tiles_n, tile_m, tile_n);
     const int m0 = tile_m * C::BM, n0 = tile_n * C::BN;
-    if (m0 >= m) return;
     const int k_begin = split * s.k_per_split;
     const int k_end = k_begin + s.k_per_split < k ? k_begin + s.k_per_split : k;
     v16f acc[C::TM][C::TN];
@@ -582,17 +591,17 @@ template <class T, class C, Layout LA, Layout LB, class Ep>
 __global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) {
 #if __HIP_DEVICE_COMPILE__
     extern __shared__ __align__(16) char lds_bytes[];
-    product_tile<T, C, LA, LB>(s, ep, (int)blockIdx.x, (int)blockIdx.y, lds_bytes);
+    product_tile<T, C, LA, LB>(s, ep, (int)blockIdx.x, lds_bytes);
 #endif
 }
-// Two products in one launch, the second's workgroups behind the first's `groups`, each with its tiles split by split.
+// Two products in one launch, the second's workgroups behind the first's `groups`.
 template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
-__global__ __launch_bounds__(C::kThreads) void product_pair(Shape<T> s, Ep ep, int tiles, int groups, Shape<T> s2, Ep ep2, int tiles2) {
+__global__ __launch_bounds__(C::kThreads) void product_pair(Shape<T> s, Ep ep, int groups, Shape<T> s2, Ep ep2) {
 #if __HIP_DEVICE_COMPILE__
     extern __shared__ __align__(16) char lds_bytes[];
     const int id = blockIdx.x;
-    if (id < groups) product_tile<T, C, LA, LB>(s, ep, id % tiles, id / tiles, lds_bytes);
-    else product_tile<T, C, LC, LD>(s2, ep2, (id - groups) % tiles2, (id - groups) / tiles2, lds_bytes);
+    if (id < groups) product_tile<T, C, LA, LB>(s, ep, id, lds_bytes);
+    else product_tile<T, C, LC, LD>(s2, ep2, id - groups, lds_bytes);
 #endif
 }
 
@@ -623,7 +632,7 @@ template <class T> struct Store {
 #endif
 };
 
-// fp32 partial sums of split blockIdx.y (or the whole product when there is one): out[split][m][n], ld = n
+// fp32 partial sums of a range (or the whole product when there is one): out[split][m][n], ld = n
 struct StorePartial {
     static constexpr bool kHeavy = false, kThinToo = true;
     float *out;
@@ -672,12 +681,12 @@ template <class T> struct StoreEither {
 };
 
 template <class T, class C, Layout LA, Layout LB, class Ep>
-int launch_product(const Shape<T> &s, int splits, const Ep &ep, const char *who) {
-    const long tiles = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN);
+int launch_product(const Shape<T> &s, const Ep &ep, const char *who) {
+    const long groups = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN) * s.splits;
     // (a grid has at most 2^32 - 1 threads in each direction)
-    if (tiles > 0xffffffffL / C::kThreads || splits > 65535) return fail(SWC_HIP_EUNSUPPORTED, "%s: too many tiles", who);
+    if (groups > 0xffffffffL / C::kThreads) return fail(SWC_HIP_EUNSUPPORTED, "%s: too many tiles", who);
     note_kernel("product<%s,%dx%d,%d,%d,%s%s> x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, C::SA, C::SB, LA == kAlongK ? "k" : "m",
-                LB == kAlongK ? "k" : "n", splits);
+                LB == kAlongK ? "k" : "n", s.splits);
     auto kern = product_tiles<T, C, LA, LB, Ep>;
     static bool attr_set = false;
     if (!attr_set) {
@@ -685,15 +694,15 @@ int launch_product(const Shape<T> &s, int splits, const Ep &ep, const char *who)
                                         C::kLdsBytes));
         attr_set = true;
     }
-    kern<<<dim3((unsigned)tiles, (unsigned)splits), C::kThreads, C::kLdsBytes, stream()>>>(s, ep);
+    kern<<<(unsigned)groups, C::kThreads, C::kLdsBytes, stream()>>>(s, ep);
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
 
 template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
-int launch_pair(const Shape<T> &s, int splits, const Ep &ep, const Shape<T> &s2, int splits2, const Ep &ep2) {
-    auto tiles = [](const Shape<T> &x) { return ((x.m + C::BM - 1) / C::BM) * ((x.n + C::BN - 1) / C::BN); };
-    note_kernel("product_pair<%s,%dx%d> x%d x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, splits, splits2);
+int launch_pair(const Shape<T> &s, const Ep &ep, const Shape<T> &s2, const Ep &ep2) {
+    auto groups = [](const Shape<T> &x) { return ((x.m + C::BM - 1) / C::BM) * ((x.n + C::BN - 1) / C::BN) * x.splits; };
+    note_kernel("product_pair<%s,%dx%d> x%d x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, s.splits, s2.splits);
     auto kern = product_pair<T, C, LA, LB, LC, LD, Ep>;
     static bool attr_set = false;
     if (!attr_set) {
@@ -701,8 +710,7 @@ int launch_pair(const Shape<T> &s, int splits, const Ep &ep, const Shape<T> &s2,
                                         C::kLdsBytes));
         attr_set = true;
     }
-    const int groups = tiles(s) * splits, groups2 = tiles(s2) * splits2;
-    kern<<<groups + groups2, C::kThreads, C::kLdsBytes, stream()>>>(s, ep, tiles(s), groups, s2, ep2, tiles(s2));
+    kern<<<groups(s) + groups(s2), C::kThreads, C::kLdsBytes, stream()>>>(s, ep, groups(s), s2, ep2);
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }
