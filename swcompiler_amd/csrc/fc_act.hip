@@ -307,17 +307,11 @@ template <class T> constexpr int kFewRows = kIsBf16<T> ? 1 : 4;
 
 // Rows into copies whose rows start on 16-byte boundaries, zeros behind their end: 16 bytes a thread, both operands of a
 // product in one launch.
-template <class T> __device__ __forceinline__ void copy_chunk(const Copy<T> &c, long row, long j) {
-    *reinterpret_cast<v4u *>(c.dst + row * c.ld + j) = chunk_at(c.src + row * c.lds + j, c.cols - j);
-}
 template <class T> __global__ __launch_bounds__(256) void copy_chunks(Copy<T> a, Copy<T> b, long chunks_a, long chunks) {
 #if __HIP_DEVICE_COMPILE__
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (long)gridDim.x * 256) {
-        const bool first = i < chunks_a;
-        const long per = (first ? a.ld : b.ld) / kChunk<T>, at = first ? i : i - chunks_a;
-        const long row = at / per, j = (at - row * per) * kChunk<T>;
-        if (first) copy_chunk(a, row, j);
-        else copy_chunk(b, row, j);
+        if (i < chunks_a) a.chunk(i);
+        else b.chunk(i - chunks_a);
     }
 #endif
 }
@@ -416,7 +410,7 @@ namespace swc_hip {
 namespace product {
 
 template <class T> int copy_operands(const Copy<T> &a, const Copy<T> &b) {
-    const long na = a.dst ? a.rows * (a.ld / kChunk<T>) : 0, nb = b.dst ? b.rows * (b.ld / kChunk<T>) : 0;
+    const long na = a.chunks(), nb = b.chunks();
     if (!(na + nb)) return SWC_HIP_OK;
     copy_chunks<T><<<grid_of(na + nb), 256, 0, stream()>>>(a, b, na, na + nb);
     SWC_LAUNCH_CHECK();

@@ -17,7 +17,7 @@ namespace {
 // threads side by side hold four columns each, four rows at a time.  Bound by memory: three passes over m x n.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums,
-                                                int each) {
+                                                T *dbias, int each) {
 #if __HIP_DEVICE_COMPILE__
     __shared__ float part[4][256];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, lon
     const int have = n - j;
     float sum[4] = {};
     if (have > 0) {
-#pragma unroll 4
+#pragma unroll 8
         for (int r = r0 + ty; r < r1; r += 4) {
             float g[4];
             load4(dc + r * ldc + j, have, g);
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, lon
         const float none[4] = {};
         for (int r = r0 + ty; r < r1; r += 4) store4(dz + r * ld + j, (int)ld - j, none);
     }
-    if (!sums) return;
+    if (!sums && !dbias) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[ty][tx * 4 + e] = sum[e];
     __syncthreads();
@@ -56,7 +56,9 @@ __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, lon
     float s = 0.f;
 #pragma unroll
     for (int y = 0; y < 4; ++y) s += part[y][threadIdx.x];
-    if (col < n) sums[(size_t)blockIdx.y * n + col] = s;
+    if (col >= n) return;
+    if (dbias) store_any(dbias + col, s);   // (one block of rows)
+    else sums[(size_t)blockIdx.y * n + col] = s;
 #endif
 }
 
@@ -81,19 +83,21 @@ int check_grad(const char *who, int m, int n, int k, const T *dc, int lddc, cons
 }
 
 // Rows a workgroup takes: 32, or 8 where that leaves the chip short of workgroups (512 x 1024: 10 us and 4); more where a
-// grid's 65535 rows of workgroups would not cover them.
-int sum_rows(int m, int n) {
+// grid's 65535 rows of workgroups would not cover them.  Up to 32 rows are one block where column sums are wanted: no
+// kernel for the blocks' sums.
+int sum_rows(int m, int n, bool sums) {
+    if (m <= 32 && sums) return 32;
     if ((m + 31) / 32 > 65535) return (m + 65534) / 65535;
     return (long)((m + 31) / 32) * ((n + 255) / 256) >= 4L * swc::devices::HipDevice::computeUnits ? 32 : 8;
 }
-int sum_blocks(int m, int n) { return (m + sum_rows(m, n) - 1) / sum_rows(m, n); }
+int sum_blocks(int m, int n, bool sums) { return (m + sum_rows(m, n, sums) - 1) / sum_rows(m, n, sums); }
 
 template <class T>
-int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums) {
+int launch_act_grad(T *dz, long ld, const T *dc, long lddc, const T *z, long ldz, int act, int m, int n, float *sums, T *dbias) {
     if (!dz) ld = 0;
-    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m, n));
+    const dim3 grid(ceil_div(ld > n ? ld : n, 256), sum_blocks(m, n, dbias));
     return with_act(act, [&]<int ACT>() {
-        act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums, sum_rows(m, n));
+        act_grad<T, ACT><<<grid, 256, 0, stream()>>>(dz, ld, dc, lddc, z, ldz, m, n, sums, sums ? nullptr : dbias, sum_rows(m, n, dbias));
         SWC_LAUNCH_CHECK();
         return (int)SWC_HIP_OK;
     });
@@ -112,41 +116,12 @@ Space<T> space(char *base, int m, int n, int k, bool own_dz, bool pack_a, bool p
     s.a = pack_a ? c.take<T>((size_t)m * row_length<T>(k)) : nullptr;
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.part = partials ? c.take<float>(partials / sizeof(float)) : nullptr;
-    s.sums = bias ? c.take<float>((size_t)sum_blocks(m, n) * n) : nullptr;
+    s.sums = bias && sum_blocks(m, n, true) > 1 ? c.take<float>((size_t)sum_blocks(m, n, true) * n) : nullptr;
     s.bytes = c.used;
     return s;
 }
 
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
-
-// one product of the gradients: whole tiles straight to the output, or cut along the contraction and joined
-template <Layout LA, Layout LB, class T>
-int grad_product(const char *who, const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
-    if (p.splits == 1) return run_product<LA, LB>(p, s, Store<T>{out, ld}, who);
-    if (int rc = run_product<LA, LB>(p, s, StorePartial{part, (long)s.m * s.n, s.n, false}, who)) return rc;
-    return join_parts<T>(out, ld, part, p.splits, s.m, s.n);
-}
-
-// Both products in one launch, where both take 64 x 64 tiles and all of their workgroups fit the chip at once: 512 x 1024 x 784
-// fp32 37.9 us in two launches, 33.5 in one, bf16 18.7 and 14.5.
-bool pairs(const Plan &pa, const Plan &pb, int m, int n, int k) {
-    auto groups = [](const Plan &p, long rows, long cols) { return ((rows + 63) / 64) * ((cols + 63) / 64) * p.splits; };
-    return pa.kind == kSmall && pb.kind == kSmall && groups(pa, m, k) + groups(pb, k, n) <= 3L * num_cus();
-}
-template <class T>
-int pair_product(const Plan &pa, Shape<T> sa, T *da, long ldda, float *part_a, const Plan &pb, Shape<T> sb, T *db, long lddb, float *part_b) {
-    sa.k_per_split = pa.k_per_split, sa.splits = pa.splits;
-    sb.k_per_split = pb.k_per_split, sb.splits = pb.splits;
-    auto ends = [](const Plan &p, const Shape<T> &s, T *out, long ld, float *part) {
-        return StoreEither<T>{{out, ld}, {p.splits > 1 ? part : nullptr, (long)s.m * s.n, s.n, false}};
-    };
-    if (int rc = launch_pair<T, Small, kAlongK, kAlongK, kAcross, kAcross>(sa, ends(pa, sa, da, ldda, part_a), sb,
-                                                                          ends(pb, sb, db, lddb, part_b)))
-        return rc;
-    if (pa.splits > 1)
-        if (int rc = join_parts<T>(da, ldda, part_a, pa.splits, sa.m, sa.n)) return rc;
-    return pb.splits > 1 ? join_parts<T>(db, lddb, part_b, pb.splits, sb.m, sb.n) : (int)SWC_HIP_OK;
-}
 
 template <class T>
 int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const T *a, int lda_, const T *b, int ldb_, const T *preact,
@@ -178,9 +153,9 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
     }
     const long padded = row_length<T>(n);
     if (own_dz || dbias) {
-        if (int rc = launch_act_grad<T>(w.dz, padded, dc, lddc, preact, ldp, act, m, n, w.sums)) return rc;
-        if (dbias)
-            if (int rc = sum_parts<T>(dbias, w.sums, sum_blocks(m, n), n)) return rc;
+        if (int rc = launch_act_grad<T>(w.dz, padded, dc, lddc, preact, ldp, act, m, n, w.sums, dbias)) return rc;
+        if (w.sums)
+            if (int rc = sum_parts<T>(dbias, w.sums, sum_blocks(m, n, true), n)) return rc;
     }
     const T *dz = own_dz ? w.dz : dc;
     const long lddz = own_dz ? padded : lddc;
@@ -189,11 +164,11 @@ int gradients(const char *who, int m, int n, int k, const T *dc, int lddc, const
     if (pack_a) a = w.a, lda = row_length<T>(k);
     if (pack_b) b = w.b, ldb = padded;
     const Shape<T> sa{dz, b, lddz, ldb, m, k, n, 0, 1, nullptr}, sb{a, dz, lda, lddz, k, n, m, 0, 1, nullptr};
-    if (pair) return pair_product<T>(pa, sa, da, ldda, w.part, pb, sb, db, lddb, w.part + pa.partial_bytes(m, k) / sizeof(float));
+    if (pair) return grad_pair<T>(pa, sa, {da, ldda}, w.part, pb, sb, {db, lddb}, w.part + pa.partial_bytes(m, k) / sizeof(float));
     if (da)
-        if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, sa, da, ldda, w.part)) return rc;
+        if (int rc = grad_product<kAlongK, kAlongK, T>(who, pa, sa, {da, ldda}, w.part)) return rc;
     if (db)
-        if (int rc = grad_product<kAcross, kAcross, T>(who, pb, sb, db, lddb, w.part)) return rc;
+        if (int rc = grad_product<kAcross, kAcross, T>(who, pb, sb, {db, lddb}, w.part)) return rc;
     return SWC_HIP_OK;
 }
 

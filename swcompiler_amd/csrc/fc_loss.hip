@@ -38,6 +38,12 @@ struct RowsFrom {
     const float *lse, *row_grad;
     float *row_loss, *lse_out;
 };
+// a matrix whose rows left out become zeros (null: none)
+template <class T> struct Cleared {
+    T *out;
+    long ld;
+    int cols;
+};
 __device__ __forceinline__ void take_row(const RowsFrom &from, const Rows &to, int r, bool in, int at, int sel) {
     to.place[r] = in ? at : -1;
     if (in) {
@@ -82,12 +88,19 @@ __global__ __launch_bounds__(256) void copy_dense(const T *a, long lda, int k, T
         *reinterpret_cast<v4u *>(dense + r * ld + j) = chunk_at(a + rows.index[r] * lda + j, k - j);
 #endif
 }
-// Few rows: a workgroup per row counts the rows before its own and copies it, one launch instead of two.
+// Few rows: a workgroup per row counts the rows before its own and copies it; workgroups behind them copy B onto the 16-byte
+// grid where it has to be.  One launch instead of three.
 constexpr int kCountRows = 4096;
 template <class T>
-__global__ __launch_bounds__(256) void count_and_copy(RowsFrom from, Rows to, const T *a, long lda, int k, T *dense, long ld) {
+__global__ __launch_bounds__(256) void count_and_copy(RowsFrom from, Rows to, const T *a, long lda, int k, T *dense, long ld,
+                                                      Cleared<T> cleared, Copy<T> b, long chunks) {
 #if __HIP_DEVICE_COMPILE__
     __shared__ int sums[2][4];
+    if ((int)blockIdx.x >= from.m) {
+        const long step = (long)(gridDim.x - from.m) * 256;
+        for (long i = (long)(blockIdx.x - from.m) * 256 + threadIdx.x; i < chunks; i += step) b.chunk(i);
+        return;
+    }
     const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int before = 0, all = 0;
     for (int r0 = 0; r0 < from.m; r0 += 256) {
@@ -106,16 +119,24 @@ __global__ __launch_bounds__(256) void count_and_copy(RowsFrom from, Rows to, co
         take_row(from, to, row, in, at, sel);
         if (row == 0) *to.count = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
     }
-    if (!in) return;
+    if (!in) {
+        if (cleared.out)
+            for (int j = threadIdx.x; j < cleared.cols; j += 256) cleared.out[row * cleared.ld + j] = T(0);
+        return;
+    }
     for (long j = threadIdx.x * kChunk<T>; j < ld; j += 256 * kChunk<T>)
         *reinterpret_cast<v4u *>(dense + at * ld + j) = chunk_at(a + row * lda + j, k - j);
 #endif
 }
-template <class T> int gather_rows(const RowsFrom &from, const Rows &to, const T *a, long lda, int k, T *dense) {
+// The dense rows, and b's copy; cleared: only with up to kCountRows rows.
+template <class T>
+int gather_rows(const RowsFrom &from, const Rows &to, const T *a, long lda, int k, T *dense, const Cleared<T> &cleared, const Copy<T> &b) {
     const long ld = row_length<T>(k);
     if (from.m <= kCountRows) {
-        count_and_copy<T><<<from.m, 256, 0, stream()>>>(from, to, a, lda, k, dense, ld);
+        const long chunks = b.chunks();
+        count_and_copy<T><<<from.m + (chunks ? grid_of(chunks) : 0), 256, 0, stream()>>>(from, to, a, lda, k, dense, ld, cleared, b, chunks);
     } else {
+        if (int rc = copy_operands<T>({}, b)) return rc;
         pick_rows<<<1, kPickThreads, 0, stream()>>>(from, to);
         SWC_LAUNCH_CHECK();
         copy_dense<T><<<dim3(ceil_div(ld / kChunk<T>, 256), from.m < 32768 ? from.m : 32768), 256, 0, stream()>>>(a, lda, k, dense, ld, to);
@@ -331,6 +352,23 @@ int launch_spread(T *out, long ld, const float *part, int parts, long stride, in
     return SWC_HIP_OK;
 }
 
+// Few rows: a piece's column sums at once, 32 columns and eight ranges of the rows a workgroup.
+constexpr int kFewSums = 512;
+template <class T> __global__ __launch_bounds__(256) void few_column_sums(const T *dz, long ld, int cols, Rows rows, T *out) {
+    __shared__ float sums[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, j = blockIdx.x * 32 + tx;
+    const int count = *rows.count, each = (count + 7) / 8, r0 = ty * each, r1 = r0 + each < count ? r0 + each : count;
+    float s = 0.f;
+    if (j < cols)
+#pragma unroll 8
+        for (int r = r0; r < r1; ++r) s += load_any(dz + r * ld + j);
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty || j >= cols) return;
+#pragma unroll
+    for (int y = 1; y < 8; ++y) s += sums[y][tx];
+    store_any(out + j, s);
+}
 // sums over blocks of kSumRows dense rows of a piece's columns
 constexpr int kSumRows = 64;
 template <class T>
@@ -398,8 +436,9 @@ template <class T> ForwardSpace<T> forward_space(char *base, const Plan &p, int 
     return s;
 }
 
-// Classes per piece of the gradients' dz: 256 MiB of it.  Fewer would make dA's sums travel more often (at 8192 x 4096 the
-// 268 MB of them cost a twelfth of a piece of 4096 classes), more gain nothing.
+// Classes per piece of the gradients' dz: 256 MiB of it, about what the last-level cache holds.  Fewer make dA's sums travel
+// more often (4799 x 25615 x 768: 774 us whole, 874 in pieces of 128 MiB, 981 of 64), more leave the cache (7477 x 56867 x 64:
+// 786 us, 924 in pieces of 512 MiB; 8192 x 128256 x 4096 gains 1.5 %).
 int piece_columns(int m, int n, size_t bytes) {
     size_t p = ((size_t)256 << 20) / bytes / m / 256 * 256;
     if (p < 256) p = 256;
@@ -412,6 +451,7 @@ template <class T> struct GradSpace {
     float *da, *part, *sums;
     int piece;
     Plan pa, pb;
+    bool direct, pair;   // dA's rows go straight to their places; both products of the one piece in one launch
     size_t bytes;
 };
 template <class T> GradSpace<T> grad_space(char *base, int m, int n, int k, bool pack_b, bool da, bool db, bool dbias) {
@@ -420,13 +460,15 @@ template <class T> GradSpace<T> grad_space(char *base, int m, int n, int k, bool
     s.piece = piece_columns(m, n, sizeof(T));
     s.pa = plan_product<T>(m, k, s.piece);
     s.pb = plan_product<T>(k, s.piece, m);
+    s.direct = s.piece == n && s.pa.splits == 1 && m <= kCountRows;
+    s.pair = da && db && s.piece == n && (s.direct || s.pa.splits > 1) && pairs(s.pa, s.pb, m, n, k);
     s.rows = take_rows(c, m, true);
     s.a = c.take<T>((size_t)m * row_length<T>(k));
     s.b = pack_b ? c.take<T>((size_t)k * row_length<T>(n)) : nullptr;
     s.dz = c.take<T>((size_t)m * row_length<T>(s.piece));
-    s.da = da ? c.take<float>((size_t)s.pa.splits * m * k) : nullptr;
+    s.da = da && !s.direct ? c.take<float>((size_t)s.pa.splits * m * k) : nullptr;
     s.part = db && s.pb.splits > 1 ? c.take<float>((size_t)s.pb.splits * k * s.piece) : nullptr;
-    s.sums = dbias ? c.take<float>((size_t)((m + kSumRows - 1) / kSumRows) * s.piece) : nullptr;
+    s.sums = dbias && m > kFewSums ? c.take<float>((size_t)((m + kSumRows - 1) / kSumRows) * s.piece) : nullptr;
     s.bytes = c.used;
     return s;
 }
@@ -449,11 +491,10 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
     char *base = static_cast<char *>(workspace(forward_space<T>(nullptr, p, m, n, k, pack_b).bytes, who));
     if (!base) return fail_code();
     const ForwardSpace<T> w = forward_space<T>(base, p, m, n, k, pack_b);
-    if (int rc = gather_rows<T>({selected, m, n, nullptr, nullptr, row_loss, lse}, w.rows, a, lda, k, w.a)) return rc;
-    if (pack_b) {
-        if (int rc = copy_operands<T>({}, {w.b, b, row_length<T>(n), ldb, k, n})) return rc;
-        b = w.b, ldb = row_length<T>(n);
-    }
+    if (int rc = gather_rows<T>({selected, m, n, nullptr, nullptr, row_loss, lse}, w.rows, a, lda, k, w.a, {},
+                                {w.b, b, row_length<T>(n), ldb, k, n}))
+        return rc;
+    if (pack_b) b = w.b, ldb = row_length<T>(n);
     const int blocks = row_blocks(p, n);
     const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, 1, w.rows.count};
     if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias, 0}, who)) return rc;
@@ -491,39 +532,40 @@ int gradients(const char *who, int m, int n, int k, const T *a, int lda, const T
     if (!base) return fail_code();
     const GradSpace<T> w = grad_space<T>(base, m, n, k, pack_b, da, db, dbias);
     const long ldw = row_length<T>(k);
-    if (int rc = gather_rows<T>({selected, m, n, lse, row_grad, nullptr, nullptr}, w.rows, a, lda, k, w.a)) return rc;
-    if (pack_b) {
-        if (int rc = copy_operands<T>({}, {w.b, b, row_length<T>(n), ldb, k, n})) return rc;
-        b = w.b, ldb = row_length<T>(n);
-    }
+    if (int rc = gather_rows<T>({selected, m, n, lse, row_grad, nullptr, nullptr}, w.rows, a, lda, k, w.a,
+                                {w.direct ? da : nullptr, ldda, k}, {w.b, b, row_length<T>(n), ldb, k, n}))
+        return rc;
+    if (pack_b) b = w.b, ldb = row_length<T>(n);
     for (int first = 0; first < n; first += w.piece) {
         const int cols = n - first < w.piece ? n - first : w.piece;
         const long ld = row_length<T>(cols);
         const Shape<T> z{w.a, b + first, ldw, ldb, m, cols, k, 0, 1, w.rows.count};
         const StoreDz<T> ep{w.dz, ld, (int)ld, first, w.rows.sel, w.rows.lse, w.rows.grad, bias ? bias + first : nullptr};
         if (int rc = run_product<kAlongK, kAcross>(whole_plan<T>(m, cols, k), z, ep, who)) return rc;
-        if (da) {
-            const Shape<T> s{w.dz, b + first, ld, ldb, m, k, cols, 0, 1, w.rows.count};
-            if (int rc = run_product<kAlongK, kAlongK>(w.pa, s, StorePartial{w.da, (long)m * k, k, first > 0}, who)) return rc;
+        const Shape<T> sa{w.dz, b + first, ld, ldb, m, k, cols, 0, 1, w.rows.count}, sb{w.a, w.dz, ldw, ld, k, cols, m, 0, 1, w.rows.count};
+        const Store<T, true> out_a{w.direct ? da : nullptr, ldda, w.rows.index};
+        if (w.pair) {
+            // (dA's partial sums stay dense: they are joined by the spreading kernel below)
+            if (int rc = grad_pair<T>(w.pa, sa, out_a, w.da, w.pb, sb, {db, lddb}, w.part)) return rc;
+        } else {
+            const StorePartial sums{w.da, (long)m * k, k, first > 0};
+            if (da)
+                if (int rc = w.direct ? run_product<kAlongK, kAlongK>(w.pa, sa, out_a, who) : run_product<kAlongK, kAlongK>(w.pa, sa, sums, who))
+                    return rc;
+            if (db)
+                if (int rc = grad_product<kAcross, kAcross, T>(who, w.pb, sb, {db + first, lddb}, w.part)) return rc;
         }
-        if (db) {
-            const Shape<T> s{w.a, w.dz, ldw, ld, k, cols, m, 0, 1, w.rows.count};
-            if (w.pb.splits == 1) {
-                const Store<T> out{db + first, lddb};
-                if (int rc = run_product<kAcross, kAcross>(w.pb, s, out, who)) return rc;
-            } else {
-                if (int rc = run_product<kAcross, kAcross>(w.pb, s, StorePartial{w.part, (long)k * cols, cols, false}, who)) return rc;
-                if (int rc = join_parts<T>(db + first, lddb, w.part, w.pb.splits, k, cols)) return rc;
-            }
-        }
-        if (dbias) {
+        if (dbias && m <= kFewSums) {
+            few_column_sums<T><<<ceil_div(cols, 32), 256, 0, stream()>>>(w.dz, ld, cols, w.rows, dbias + first);
+            SWC_LAUNCH_CHECK();
+        } else if (dbias) {
             const int parts = (m + kSumRows - 1) / kSumRows;
             column_sums<T><<<dim3(ceil_div(cols, 256), parts), 256, 0, stream()>>>(w.dz, ld, cols, w.rows, w.sums);
             SWC_LAUNCH_CHECK();
             if (int rc = sum_parts<T>(dbias + first, w.sums, parts, cols)) return rc;
         }
     }
-    return da ? launch_spread(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place) : (int)SWC_HIP_OK;
+    return da && !w.direct ? launch_spread(da, ldda, w.da, w.pa.splits, (long)m * k, m, k, w.rows.place) : (int)SWC_HIP_OK;
 }
 
 } // namespace

@@ -594,23 +594,25 @@ __global__ __launch_bounds__(C::kThreads) void product_tiles(Shape<T> s, Ep ep) 
     product_tile<T, C, LA, LB>(s, ep, (int)blockIdx.x, lds_bytes);
 #endif
 }
-// Two products in one launch, the second's workgroups behind the first's `groups`.
-template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
-__global__ __launch_bounds__(C::kThreads) void product_pair(Shape<T> s, Ep ep, int groups, Shape<T> s2, Ep ep2) {
+// The two products of a layer's gradients in one launch, dB's workgroups behind dA's `groups`.
+template <class T, class CA, class CB, class Ep>
+__global__ __launch_bounds__(CA::kThreads) void product_pair(Shape<T> a, Ep ep_a, int groups, Shape<T> b, Ep ep_b) {
+    static_assert(CA::kThreads == CB::kThreads, "");
 #if __HIP_DEVICE_COMPILE__
     extern __shared__ __align__(16) char lds_bytes[];
     const int id = blockIdx.x;
-    if (id < groups) product_tile<T, C, LA, LB>(s, ep, id, lds_bytes);
-    else product_tile<T, C, LC, LD>(s2, ep2, id - groups, lds_bytes);
+    if (id < groups) product_tile<T, CA, kAlongK, kAlongK>(a, ep_a, id, lds_bytes);
+    else product_tile<T, CB, kAcross, kAcross>(b, ep_b, id - groups, lds_bytes);
 #endif
 }
 
-// The matrix of the product in its type.
-template <class T> struct Store {
+// The matrix of the product in its type.  PLACED: its rows go where `rows` says (null: in order).
+template <class T, bool PLACED = false> struct Store {
     static constexpr bool kHeavy = false, kThinToo = true;
     T *out;
     long ld;
-    Store from(int j) const { return {out + j, ld}; }
+    const int *rows = nullptr;
+    Store from(int j) const { return {out + j, ld, rows}; }
 #if __HIP_DEVICE_COMPILE__
     template <class P, bool WHOLE, int TM, int TN>
     __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], int row0, int col0, int m, int n, int lane) const {
@@ -621,7 +623,9 @@ template <class T> struct Store {
             float x[P::kValues];
 #pragma unroll
             for (int u = 0; u < P::kValues; ++u) x[u] = P::value(acc[tm], u);
-            store_row<P, WHOLE>(out + row * ld, row < m, col0, n, h, x);
+            const bool ok = WHOLE || row < m;
+            const long at = PLACED && rows && ok ? rows[row] : row;
+            store_row<P, WHOLE>(out + at * ld, ok, col0, n, h, x);
         }
     }
     template <class P, int TM, int TN>
@@ -669,7 +673,7 @@ struct StorePartial {
 
 // the one or the other: partial sums where `part.out` is given
 template <class T> struct StoreEither {
-    Store<T> whole;
+    Store<T, true> whole;
     StorePartial part;
 #if __HIP_DEVICE_COMPILE__
     template <class P, int TM, int TN>
@@ -699,18 +703,19 @@ int launch_product(const Shape<T> &s, const Ep &ep, const char *who) {
     return SWC_HIP_OK;
 }
 
-template <class T, class C, Layout LA, Layout LB, Layout LC, Layout LD, class Ep>
-int launch_pair(const Shape<T> &s, const Ep &ep, const Shape<T> &s2, const Ep &ep2) {
-    auto groups = [](const Shape<T> &x) { return ((x.m + C::BM - 1) / C::BM) * ((x.n + C::BN - 1) / C::BN) * x.splits; };
-    note_kernel("product_pair<%s,%dx%d> x%d x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, s.splits, s2.splits);
-    auto kern = product_pair<T, C, LA, LB, LC, LD, Ep>;
+template <class T, class CA, class CB, class Ep>
+int launch_pair(const Shape<T> &a, const Ep &ep_a, const Shape<T> &b, const Ep &ep_b) {
+    constexpr int kLds = CA::kLdsBytes > CB::kLdsBytes ? CA::kLdsBytes : CB::kLdsBytes;
+    note_kernel("product_pair<%s,%dx%d,%dx%d> x%d x%d", kIsBf16<T> ? "bf16" : "fp32", CA::BM, CA::BN, CB::BM, CB::BN, a.splits, b.splits);
+    auto kern = product_pair<T, CA, CB, Ep>;
     static bool attr_set = false;
     if (!attr_set) {
-        SWC_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                        C::kLdsBytes));
+        SWC_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
         attr_set = true;
     }
-    kern<<<groups(s) + groups(s2), C::kThreads, C::kLdsBytes, stream()>>>(s, ep, groups(s), s2, ep2);
+    const unsigned groups = ceil_div(a.m, CA::BM) * ceil_div(a.n, CA::BN) * a.splits;
+    const unsigned groups_b = ceil_div(b.m, CB::BM) * ceil_div(b.n, CB::BN) * b.splits;
+    kern<<<groups + groups_b, CA::kThreads, kLds, stream()>>>(a, ep_a, (int)groups, b, ep_b);
     SWC_LAUNCH_CHECK();
     return SWC_HIP_OK;
 }

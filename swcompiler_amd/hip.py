@@ -196,37 +196,46 @@ class _Arg:
     """What an op needs of an operand: its address, shape, element type and row stride.  Operands are DeviceArrays or
     torch tensors on the runtime's device (taken as they are: any row stride, columns contiguous)."""
 
-    __slots__ = ("ptr", "shape", "type", "ld", "size")
+    __slots__ = ("ptr", "shape", "type", "ld")
 
-    def __init__(self, rt, x, what):
-        self.shape = shape = tuple(x.shape)
+    def __init__(self, rt, x, what, name):
+        self.shape = shape = x.shape
         self.ld = shape[-1] if shape else 1
         if isinstance(x, DeviceArray):
-            self.ptr, self.type, self.size = x.ptr, _NUMPY_TYPES.get(x.dtype.name), x.size
+            self.ptr, self.type = x.ptr, _NUMPY_TYPES.get(x.dtype.name)
             return
-        self.ptr, self.type, self.size = _torch_operand(rt, x, what)
+        self.ptr, self.type = _torch_operand(rt, x, what, name)
         if x.is_contiguous():
             return
         stride = x.stride()
         if len(shape) > 2 or (shape[-1] > 1 and stride[-1] != 1):
-            raise SwcHipError(f"{what}: the elements of a row are not contiguous (strides {stride})")
+            raise SwcHipError(f"{what}: {name}: the elements of a row are not contiguous (strides {stride})")
         if len(shape) == 2 and shape[0] > 1:
             self.ld = stride[0]
             if self.ld < shape[1]:
-                raise SwcHipError(f"{what}: rows overlap (stride {self.ld}, {shape[1]} columns)")
-            _int32(self.ld, what + ": row stride")
+                raise SwcHipError(f"{what}: {name}: rows overlap (stride {self.ld}, {shape[1]} columns)")
+            _int32(self.ld, f"{what}: {name}: row stride")
+
+    @property
+    def size(self):
+        n = 1
+        for d in self.shape:
+            n *= d
+        return n
 
 
-def _torch_operand(rt, x, what):
-    """-> (address, element type, elements) of a torch tensor on the runtime's device"""
-    if not hasattr(x, "data_ptr"):
-        raise SwcHipError(f"{what}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
-    if x.get_device() != rt.device:
-        raise SwcHipError(f"{what}: the tensor is on {x.device}, the runtime on device {rt.device}")
-    kind = _TORCH_KINDS.get(x.dtype)
+def _torch_operand(rt, x, what, name):
+    """-> (address, element type) of a torch tensor on the runtime's device"""
+    try:
+        if x.get_device() != rt.device:
+            raise SwcHipError(f"{what}: {name}: the tensor is on {x.device}, the runtime on device {rt.device}")
+        kind = _TORCH_KINDS.get(x.dtype)
+        ptr = x.data_ptr()
+    except AttributeError:
+        raise SwcHipError(f"{what}: {name}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}") from None
     if kind is None:
         kind = _TORCH_KINDS[x.dtype] = _TORCH_TYPES.get(str(x.dtype), "?")
-    return x.data_ptr() or None, kind, x.numel()
+    return ptr or None, kind
 
 
 _TORCH_KINDS = {}     # torch.dtype -> element type, filled as they are met (this module does not import torch)
@@ -693,15 +702,17 @@ class SwcHip:
         return out
 
     # -- operators of language models (matrices fp32 or bfloat16; DeviceArrays or torch tensors) --
-    def _arg(self, x, what, types, shape=None):
+    def _arg(self, x, what, name, types, shape=None):
         """the operand as an _Arg; None for None"""
         if x is None:
             return None
-        a = _Arg(self, x, what)
+        if not hasattr(x, "shape"):
+            raise SwcHipError(f"{what}: {name}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
+        a = _Arg(self, x, what, name)
         if a.type not in types:
-            raise SwcHipError(f"{what}: element type {a.type or x.dtype} is not one of {', '.join(types)}")
+            raise SwcHipError(f"{what}: {name}: element type {a.type or x.dtype} is not one of {', '.join(types)}")
         if shape is not None and a.shape != shape:
-            raise SwcHipError(f"{what}: shape {a.shape}, expected {shape}")
+            raise SwcHipError(f"{what}: {name}: shape {tuple(a.shape)}, expected {shape}")
         return a
 
     @staticmethod
@@ -716,7 +727,7 @@ class SwcHip:
         return out if out is not None else self.empty(shape, np.float32 if like == "f32" else np.uint16)
 
     def _product(self, a, b, what):
-        a, b = self._arg(a, what + ": a", ("f32", "bf16")), self._arg(b, what + ": b", ("f32", "bf16"))
+        a, b = self._arg(a, what, "a", ("f32", "bf16")), self._arg(b, what, "b", ("f32", "bf16"))
         if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0] or a.type != b.type:
             raise SwcHipError(f"{what}: a {a.shape} {a.type} and b {b.shape} {b.type} do not multiply")
         m, n, k = _int32(a.shape[0], what), _int32(b.shape[1], what), _int32(a.shape[1], what)
@@ -734,9 +745,9 @@ class SwcHip:
         a, b, m, n, k, t, suffix = self._product(a, b, what)
         act = self._activation(act)
         out = self._out(out, (m, n), t[0])
-        c = self._arg(out, what + ": out", t, (m, n))
-        bias, r = self._arg(bias, what + ": bias", t, (n,)), self._arg(residual, what + ": residual", t, (m, n))
-        z = self._arg(preact, what + ": preact", t, (m, n))
+        c = self._arg(out, what, "out", t, (m, n))
+        bias, r = self._arg(bias, what, "bias", t, (n,)), self._arg(residual, what, "residual", t, (m, n))
+        z = self._arg(preact, what, "preact", t, (m, n))
         self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAdd" + suffix)(
             m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), act, self._p(r), self._ld(r), self._p(z),
             self._ld(z), c.ptr, c.ld), what)
@@ -749,9 +760,9 @@ class SwcHip:
         act = self._activation(act)
         if da is None and db is None and dbias is None:
             da, db, dbias = self._out(None, (m, k), t[0]), self._out(None, (k, n), t[0]), self._out(None, (n,), t[0])
-        g, z = self._arg(dc, what + ": dc", t, (m, n)), self._arg(preact, what + ": preact", t, (m, n))
-        ga, gb = self._arg(da, what + ": da", t, (m, k)), self._arg(db, what + ": db", t, (k, n))
-        gbias = self._arg(dbias, what + ": dbias", t, (n,))
+        g, z = self._arg(dc, what, "dc", t, (m, n)), self._arg(preact, what, "preact", t, (m, n))
+        ga, gb = self._arg(da, what, "da", t, (m, k)), self._arg(db, what, "db", t, (k, n))
+        gbias = self._arg(dbias, what, "dbias", t, (n,))
         self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAddGrad" + suffix)(
             m, n, k, g.ptr, g.ld, a.ptr, a.ld, b.ptr, b.ld, self._p(z), self._ld(z), act, self._p(ga),
             self._ld(ga), self._p(gb), self._ld(gb), self._p(gbias)), what)
@@ -762,11 +773,11 @@ class SwcHip:
         what = "matrixFCSoftmaxWithLoss"
         a, b, m, n, k, t, suffix = self._product(a, b, what)
         loss, row_loss, lse = self._out(loss, (), "f32"), self._out(row_loss, (m,), "f32"), self._out(lse, (m,), "f32")
-        bias, sel = self._arg(bias, what + ": bias", t, (n,)), self._arg(selected, what + ": selected", ("i32",), (m,))
-        one = self._arg(loss, what + ": loss", ("f32",))
+        bias, sel = self._arg(bias, what, "bias", t, (n,)), self._arg(selected, what, "selected", ("i32",), (m,))
+        one = self._arg(loss, what, "loss", ("f32",))
         if one.size != 1:
             raise SwcHipError(f"{what}: loss: shape {one.shape}, expected one value")
-        rl, ls = self._arg(row_loss, what + ": row_loss", ("f32",), (m,)), self._arg(lse, what + ": lse", ("f32",), (m,))
+        rl, ls = self._arg(row_loss, what, "row_loss", ("f32",), (m,)), self._arg(lse, what, "lse", ("f32",), (m,))
         self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLoss" + suffix)(
             m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, rl.ptr, ls.ptr, one.ptr), what)
         return loss, row_loss, lse
@@ -778,10 +789,10 @@ class SwcHip:
         a, b, m, n, k, t, suffix = self._product(a, b, what)
         if da is None and db is None and dbias is None:
             da, db, dbias = self._out(None, (m, k), t[0]), self._out(None, (k, n), t[0]), self._out(None, (n,), t[0])
-        bias, sel = self._arg(bias, what + ": bias", t, (n,)), self._arg(selected, what + ": selected", ("i32",), (m,))
-        ls, rg = self._arg(lse, what + ": lse", ("f32",), (m,)), self._arg(row_grad, what + ": row_grad", ("f32",), (m,))
-        ga, gb = self._arg(da, what + ": da", t, (m, k)), self._arg(db, what + ": db", t, (k, n))
-        gbias = self._arg(dbias, what + ": dbias", t, (n,))
+        bias, sel = self._arg(bias, what, "bias", t, (n,)), self._arg(selected, what, "selected", ("i32",), (m,))
+        ls, rg = self._arg(lse, what, "lse", ("f32",), (m,)), self._arg(row_grad, what, "row_grad", ("f32",), (m,))
+        ga, gb = self._arg(da, what, "da", t, (m, k)), self._arg(db, what, "db", t, (k, n))
+        gbias = self._arg(dbias, what, "dbias", t, (n,))
         self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLossGrad" + suffix)(
             m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, ls.ptr, self._p(rg), self._p(ga), self._ld(ga),
             self._p(gb), self._ld(gb), self._p(gbias)), what)
@@ -794,7 +805,7 @@ class SwcHip:
         return state
 
     def _state(self, state, what):
-        return self._arg(state, what + ": state", ("i32",), (ADAMW_STATE_WORDS,)).ptr
+        return self._arg(state, what, "state", ("i32",), (ADAMW_STATE_WORDS,)).ptr
 
     def adamwAdvance(self, state, beta1, beta2):
         """begins a step: counts it and prepares the bias corrections of the updates that follow"""
@@ -825,7 +836,7 @@ class SwcHip:
                 if isinstance(x, DeviceArray):
                     ptr, t, n = x.ptr, _NUMPY_TYPES.get(x.dtype.name), x.size
                 else:
-                    ptr, t, n = _torch_operand(self, x, f"{what}: {name} of tensor {i}")
+                    (ptr, t), n = _torch_operand(self, x, what, f"{name} of tensor {i}"), x.numel()
                     if not x.is_contiguous():
                         raise SwcHipError(f"{what}: {name} of tensor {i} is not contiguous")
                 if t not in types:
@@ -851,7 +862,7 @@ class SwcHip:
             pointers = [pw, pg, pm, pv]
         pointers.append(None if copies is None else addresses(copies, ("bf16",), sizes, "copies")[0])
         sizes = (C.c_size_t * count)(*sizes)
-        factors = [self._arg(x, f"{what}: factor", ("f32",)) for x in (lr_factor, grad_factor)]
+        factors = [self._arg(x, what, "factor", ("f32",)) for x in (lr_factor, grad_factor)]
         if any(x is not None and x.size != 1 for x in factors):
             raise SwcHipError(f"{what}: a factor is one value")
         one = [self._p(x) for x in factors]

@@ -693,7 +693,9 @@ def test_loss_and_gradients(rt, kind, m, n, k):
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m,n,k,share", [(70, 301, 72, 0.5), (300, 1000, 64, 0.9), (33, 40, 16, 1.0), (1030, 130, 40, 0.3),
-                                         (4096, 70, 24, 0.1), (4097, 70, 24, 0.1), (6000, 100, 19, 0.6)])
+                                         (4096, 70, 24, 0.1), (4097, 70, 24, 0.1), (6000, 100, 19, 0.6),
+                                         (5000, 320, 64, 0.2), (2048, 700, 200, 0.5), (28, 1000, 320, 0.3), (28, 9000, 65, 0.3),
+                                         (600, 130, 1028, 0.2)])
 def test_loss_rows_left_out(rt, kind, m, n, k, share):
     """rows whose class lies outside the vocabulary bring nothing, whatever they hold: here infinities and NaN"""
     print("case loss left out", kind.name, m, n, k, share, flush=True)
