@@ -145,7 +145,8 @@ int gather_rows(const RowsFrom &from, const Rows &to, const T *a, long lda, int 
     return SWC_HIP_OK;
 }
 
-// bf16: the exponential instruction (relative error |x| 2^-24 and a little); fp32: the library function
+// bf16: the exponential instruction (relative error |x| 2^-24 and a little); fp32: the library function.  (Its factor and the
+// maximum are not fused into one operation: of values near the type's lowest the product overflows.)
 template <class T> __device__ __forceinline__ float exponential(float x) { return kIsBf16<T> ? fast_exp(x) : expf(x); }
 
 // ---------------------------------------------------------------- forward
@@ -373,13 +374,30 @@ template <class T> __global__ __launch_bounds__(256) void few_column_sums(const 
 constexpr int kSumRows = 64;
 template <class T>
 __global__ __launch_bounds__(256) void column_sums(const T *dz, long ld, int cols, Rows rows, float *sums) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= cols) return;
+#if __HIP_DEVICE_COMPILE__
+    __shared__ float part[4][256];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, j = (blockIdx.x * 64 + tx) * 4;
     const int count = *rows.count, r0 = blockIdx.y * kSumRows;
     const int r1 = r0 + kSumRows < count ? r0 + kSumRows : count;
-    float s = 0.f;
-    for (int r = r0; r < r1; ++r) s += load_any(dz + r * ld + j);
-    sums[(size_t)blockIdx.y * cols + j] = s;
+    float s[4] = {};
+    if (j < cols)   // (dz's rows end on a multiple of four)
+#pragma unroll 8
+        for (int r = r0 + ty; r < r1; r += 4) {
+            float x[4];
+            load4(dz + r * ld + j, 4, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += x[e];
+        }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[ty][tx * 4 + e] = s[e];
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= cols) return;
+    float all = 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) all += part[y][threadIdx.x];
+    sums[(size_t)blockIdx.y * cols + col] = all;
+#endif
 }
 
 // ---------------------------------------------------------------- the calls
