@@ -9,7 +9,8 @@
 
 #include <algorithm>
 #include <cmath>
-#include <vector>
+#include <memory>
+#include <new>
 
 using namespace swc_hip;
 
@@ -301,18 +302,20 @@ int check(const char *who, int count, const void *const *w, const void *const *d
     for (int i = 0; i < count; ++i)
         if (sizes[i] > (size_t)kMaxChunks * kChunk) return fail(SWC_HIP_EUNSUPPORTED, "%s: tensor %d has %zu elements", who, i, sizes[i]);
     // one parameter given twice (tied weights) would be stepped by two workgroups at a time
-    std::vector<const void *> seen;
-    seen.reserve(count);
+    if (count < 2) return SWC_HIP_OK;
+    const std::unique_ptr<const void *[]> seen(new (std::nothrow) const void *[count]);
+    if (!seen) return fail(SWC_HIP_ERUNTIME, "%s: out of host memory", who);
+    int n = 0;
     for (int i = 0; i < count; ++i)
-        if (sizes[i]) seen.push_back(w[i]);
-    std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return fail(SWC_HIP_EINVAL, "%s: a tensor is given twice", who);
+        if (sizes[i]) seen[n++] = w[i];
+    std::sort(seen.get(), seen.get() + n);
+    if (std::adjacent_find(seen.get(), seen.get() + n) != seen.get() + n) return fail(SWC_HIP_EINVAL, "%s: a tensor is given twice", who);
     return SWC_HIP_OK;
 }
 
 // Fills tables of up to N tensors and launches one kernel for each.
 template <class T, int N, class Fill, class Launch>
-int launch_tables(const char *who, int count, const size_t *sizes, Fill fill, Launch launch) {
+int launch_tables(int count, const size_t *sizes, Fill fill, Launch launch) {
     Table<T, N> tab;
     int next = 0;
     while (next < count) {
@@ -352,7 +355,7 @@ int adamw(const char *who, int count, float *const *w, const G *const *dw, float
     const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1),
                  (float)(1. - beta2), eps, decay};
     return launch_tables<Tensor, kTensors>(
-        who, count, sizes,
+        count, sizes,
         [&](Tensor &t, int i) { t = Tensor{w[i], dw[i], mom[i], var[i], copies ? copies[i] : nullptr, sizes[i]}; },
         [&](const Table<Tensor, kTensors> &tab, unsigned chunks) {
             auto kern = streams(sizes, count, sizeof(float)) ? adamw_tensors<G, true> : adamw_tensors<G, false>;
@@ -372,7 +375,7 @@ int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint
     const Step s{static_cast<const Header *>(state), lr_factor, grad_factor, lr, (float)beta1, (float)beta2, (float)(1. - beta1),
                  (float)(1. - beta2), eps, decay};
     return launch_tables<Tensor8, kTensors8>(
-        who, count, sizes,
+        count, sizes,
         [&](Tensor8 &t, int i) {
             t.w = w[i], t.dw = dw[i], t.mom = mom8[i], t.var = var8[i], t.copy = copies ? copies[i] : nullptr;
             t.size = sizes[i], t.mom_scale = mom_scale[i], t.var_scale = var_scale[i];

@@ -5,8 +5,8 @@
 //
 // One product on the core of product_tile.hpp, with everything behind the sums in its epilogue; a product cut along k
 // (few tiles) leaves fp32 partial sums in the workspace and ends in fc_finish; few rows take fc_stream or fc_few.
-// 4096 x 16384 x 4096 bf16 with bias, tanh gelu and residual: 461 us, 1190 TFLOP/s (the product alone 412; the residual's 134
-// MB another 30).  2048 x 4096 x 4096 fp32 with gelu and residual 498 us, 138 TFLOP/s of the 152 that a large product reaches.
+// 4096 x 16384 x 4096 bf16 with bias, tanh gelu and residual: 462-467 us, 1180 TFLOP/s (the product alone 412; the residual's 134
+// MB another 30).  2048 x 4096 x 4096 fp32 with gelu and residual 500 us, 137 TFLOP/s of the 152 that a large product reaches.
 #include "act.hpp"
 #include "product.hpp"
 

@@ -4,7 +4,7 @@
 //
 // The two products on the core of product_tile.hpp, no matrix transposed in memory; dZ in one pass (three times its size
 // at the memory's rate), rounded to the matrices' type once for both products, its column sums before that rounding.
-// Without an activation dZ is dC itself.  4096 x 16384 x 4096 bf16 with tanh gelu: 872 us, 1260 TFLOP/s.
+// Without an activation dZ is dC itself.  4096 x 16384 x 4096 bf16 with tanh gelu: 876-896 us, 1240 TFLOP/s.
 #include "act.hpp"
 #include "product.hpp"
 

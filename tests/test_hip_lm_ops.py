@@ -294,7 +294,9 @@ def small_ints(rng, *shape, top=3):
 FC_SHAPES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (1, 4096, 520), (5, 257, 1000), (16, 128, 64), (17, 130, 72), (31, 1000, 33),
              (32, 127, 64), (33, 200, 136), (64, 128, 512), (65, 72, 264), (70, 301, 75), (100, 65, 2048), (128, 128, 128),
              (129, 255, 63), (200, 511, 300), (256, 256, 64), (257, 300, 65), (300, 513, 1000), (513, 260, 96), (1000, 2056, 520),
-             (1025, 4104, 200), (4097, 4360, 72)]
+             (1025, 4104, 200), (4097, 4360, 72),
+             # a last round of large tiles left to smaller ones: of the layer, of its weights' gradient
+             (2048, 8400, 1000), (1000, 8400, 2048)]
 
 
 @gpu
@@ -676,7 +678,8 @@ def check_loss(rt, kind, a, b, bias, sel, row_grad=None, grad=True):
 
 
 LOSS_SHAPES = [(1, 1, 8), (1, 100, 8), (2, 3, 1), (5, 33, 40), (17, 64, 64), (33, 1000, 64), (64, 257, 72), (70, 301, 75),
-               (130, 4100, 136), (257, 513, 200), (300, 50, 264), (520, 20003, 96), (1000, 2056, 520)]
+               (130, 4100, 136), (257, 513, 200), (300, 50, 264), (520, 20003, 96), (1000, 2056, 520),
+               (2048, 8401, 1000)]
 
 
 @gpu
