@@ -138,6 +138,7 @@ __device__ __forceinline__ void put4_bf16(uint16_t *p, const float (&x)[4]) {
 constexpr unsigned kChunk = 4 * kThreads;
 constexpr unsigned kMaxChunks = 0xffffffffu / kThreads;
 
+// 265M parameters with bf16 gradients and copies, 7.4 GB: 1286-1300 us, 5.7 TB/s.
 template <class G, bool NT>
 __global__ __launch_bounds__(kThreads) void adamw_tensors(Table<Tensor, kTensors> tab, Step s) {
     const int which = tensor_of(tab, blockIdx.x);
@@ -207,7 +208,9 @@ __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
     return (unsigned)(8 * (e + 7) + q - 8);
 }
 
-// A wavefront owns a block of 256 elements, a lane four consecutive ones of them (FULL: the block is whole).
+// A wavefront owns a block of 256 elements, a lane four consecutive ones of them (FULL: the block is whole): a block's scale
+// is one exchange within the wavefront.  99M parameters with bf16 gradients and copies, 1.6 GB: 339-351 us, 4.6 TB/s: the
+// encodings' arithmetic, two divisions in 64 bits a lane among it, stands beside the memory.
 template <class G, bool FULL, bool NT>
 __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int lane, unsigned number, const Scalars &k, const Step &s) {
     uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);

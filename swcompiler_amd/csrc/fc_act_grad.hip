@@ -14,7 +14,8 @@ using namespace swc_hip::product;
 namespace {
 
 // dZ = dC act'(Z) into dz (zeros in columns n .. ld), and each block of rows' column sums of the unrounded values.  64
-// threads side by side hold four columns each, four rows at a time.  Bound by memory: three passes over m x n.
+// threads side by side hold four columns each, four rows at a time.  Bound by memory: three passes over m x n (4096 x 16384
+// bf16, 403 MB, 86 us, 4.7 TB/s: the copy's rate less what the slope costs).
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, long ldc, const T *z, long ldz, int m, int n, float *sums,
                                                 T *dbias, int each) {
