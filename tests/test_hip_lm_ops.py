@@ -503,6 +503,26 @@ def test_fc_grad_integers_bit_exact(rt, kind, m, n, k):
 
 
 @gpu
+def test_fc_beyond_32_bits(rt):
+    """a matrix of 2.8e9 elements, written by the layer and read by its gradients: C = A B in exact small integers, so that
+    dA = C B^T = A (B B^T), dB = A^T C = (A^T A) B and the column sums are known without C"""
+    rng = np.random.default_rng(41)
+    m, n, k = 70001, 40000, 8
+    a, b = small_ints(rng, m, k, top=2), small_ints(rng, k, n, top=2)     # |C| <= 32; sums below 2^24 / 2
+    da_, db_ = BF.up(rt, a), BF.up(rt, b)
+    c = rt.empty((m, n), np.uint16)
+    rt.matrixMatrixFCActAdd(da_, db_, out=c)
+    a, b = a.astype(np.float64), b.astype(np.float64)
+    for row in (0, 1, 53686, 53687, 53688, 69999, 70000):     # 53687 n passes 2^31
+        got = from_bf16(c.offset_view(row * n, (n,)).numpy())
+        np.testing.assert_array_equal(got, a[row] @ b)
+    ga, gb, gbias = (BF.down(x) for x in rt.matrixMatrixFCActAddGrad(c, da_, db_))
+    np.testing.assert_array_equal(ga, BF.values(a @ (b @ b.T)))
+    np.testing.assert_array_equal(gb, BF.values((a.T @ a) @ b))
+    np.testing.assert_array_equal(gbias, BF.values(a.sum(0) @ b))
+
+
+@gpu
 def test_fc_grad_many_rows(rt):
     """more rows than a grid's second direction has workgroups of 32 (65535): exact integers all the same"""
     rng = np.random.default_rng(9)
