@@ -147,7 +147,8 @@ const char *swc_hip_last_kernel(void);
  * this to have them read again — not while a graph is being recorded.  No counterpart in the reference. */
 int swc_hip_reload_switches(void);
 void *swc_hip_stream(void);                   /* the hipStream_t ops are launched on */
-int swc_hip_set_stream(void *hip_stream);     /* launch on a caller-owned stream (NULL: back to the library's own) */
+int swc_hip_set_stream(void *hip_stream);     /* launch on a caller-owned stream (NULL: back to the library's own;
+                                               * hipStreamLegacy: the null stream, which cannot be recorded) */
 const char *swc_hip_device_name(void);        /* gcnArchName of the selected device */
 int swc_hip_device_cus(void);                 /* its compute units (what the split plans divide work over); 0 before init */
 

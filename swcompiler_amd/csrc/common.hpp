@@ -20,7 +20,7 @@ int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();
 int fail_code();   // the code of this thread's last fail() (for callers of helpers that return null on failure)
 
-// The stream every op launches on; nullptr until swc_hip_init succeeded.
+// The stream every op launches on (nullptr: the null stream; ready() says whether swc_hip_init has succeeded).
 hipStream_t stream();
 bool ready();
 // Records which kernel variant an op dispatched to (printf-style), for swc_hip_last_kernel().

@@ -22,7 +22,7 @@ struct State {
     int device = -1;
     int cus = 0;
     hipStream_t own = nullptr;   // created by init
-    hipStream_t cur = nullptr;   // where ops launch (own or caller's)
+    hipStream_t cur = nullptr;   // where ops launch (own or caller's; nullptr: the null stream)
     bool cur_is_own = true;
     hipStream_t copy = nullptr;  // uploads that overlap the ops (created on first use)
     hipEvent_t ev_ops = nullptr, ev_copy = nullptr;
@@ -423,13 +423,15 @@ const char *swc_hip_last_error(void) { return g_err; }
 
 const char *swc_hip_last_kernel(void) { return g_kernel; }
 
-void *swc_hip_stream(void) { return (void *)g.cur; }
+// The null stream is named by its handle here, where NULL means the library's own; inside it is the null pointer, which
+// every call of the HIP runtime takes (hipEventRecord ends the process on the handle).
+void *swc_hip_stream(void) { return g.ready && !g.cur ? (void *)hipStreamLegacy : (void *)g.cur; }
 
 int swc_hip_set_stream(void *s) {
     SWC_REQUIRE_INIT();
     std::lock_guard<std::mutex> lk(g.mu);
     if (s) {
-        g.cur = (hipStream_t)s;
+        g.cur = (hipStream_t)s == hipStreamLegacy ? nullptr : (hipStream_t)s;
         g.cur_is_own = false;
     } else {
         g.cur = g.own;
@@ -462,6 +464,7 @@ float swc_hip_timer_elapsed_ms(void) { return g.last_ms; }
 int swc_hip_graph_begin(void) {
     SWC_REQUIRE_INIT();
     if (g.capturing) return fail(SWC_HIP_EINVAL, "swc_hip_graph_begin: a capture is already open");
+    if (!stream()) return fail(SWC_HIP_EINVAL, "swc_hip_graph_begin: the null stream cannot be recorded");
     SWC_HIP_TRY(hipStreamBeginCapture(stream(), hipStreamCaptureModeRelaxed));
     g.capturing = true;
     return SWC_HIP_OK;
