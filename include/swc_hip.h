@@ -147,8 +147,13 @@ const char *swc_hip_last_kernel(void);
  * this to have them read again — not while a graph is being recorded.  No counterpart in the reference. */
 int swc_hip_reload_switches(void);
 void *swc_hip_stream(void);                   /* the hipStream_t ops are launched on */
-int swc_hip_set_stream(void *hip_stream);     /* launch on a caller-owned stream (NULL: back to the library's own;
-                                               * hipStreamLegacy: the null stream, which cannot be recorded) */
+/* Launch on a caller-owned stream (NULL: back to the library's own; hipStreamLegacy:
+ * the null stream, which cannot be recorded).  The ops share one workspace, so work
+ * on the new stream waits for the work already launched on the library's own stream
+ * or the null stream when it leaves one of these; who leaves a stream of their own,
+ * or enters one that is being recorded into a graph, orders the two (synchronise
+ * first).  Not while swc_hip_graph_begin is open. */
+int swc_hip_set_stream(void *hip_stream);
 const char *swc_hip_device_name(void);        /* gcnArchName of the selected device */
 int swc_hip_device_cus(void);                 /* its compute units (what the split plans divide work over); 0 before init */
 

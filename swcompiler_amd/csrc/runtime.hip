@@ -26,6 +26,7 @@ struct State {
     bool cur_is_own = true;
     hipStream_t copy = nullptr;  // uploads that overlap the ops (created on first use)
     hipEvent_t ev_ops = nullptr, ev_copy = nullptr;
+    hipEvent_t ev_switch = nullptr;   // the end of the work on a stream that is left (swc_hip_set_stream)
     hipEvent_t t0 = nullptr, t1 = nullptr;
     float last_ms = -1.f;
     hipEvent_t slots[kEventSlots] = {};
@@ -193,6 +194,7 @@ int swc_hip_init(int device) {
     SWC_HIP_TRY(hipStreamCreateWithFlags(&g.own, hipStreamNonBlocking));
     SWC_HIP_TRY(hipEventCreate(&g.t0));
     SWC_HIP_TRY(hipEventCreate(&g.t1));
+    SWC_HIP_TRY(hipEventCreateWithFlags(&g.ev_switch, hipEventDisableTiming));
     g.cur = g.own;
     g.cur_is_own = true;
     g.device = device;
@@ -221,6 +223,7 @@ int swc_hip_shutdown(void) {
     for (void *&h : g.graphs_on_own_ws) h = nullptr;
     (void)hipEventDestroy(g.t0);
     (void)hipEventDestroy(g.t1);
+    (void)hipEventDestroy(g.ev_switch);
     if (g.copy) {
         (void)hipStreamSynchronize(g.copy);
         (void)hipStreamDestroy(g.copy);
@@ -238,7 +241,7 @@ int swc_hip_shutdown(void) {
     g.last_ms = -1.f;
     (void)hipStreamDestroy(g.own);
     g.own = g.cur = nullptr;
-    g.t0 = g.t1 = nullptr;
+    g.t0 = g.t1 = g.ev_switch = nullptr;
     g.ready = false;
     g.device = -1;
     return SWC_HIP_OK;
@@ -427,16 +430,37 @@ const char *swc_hip_last_kernel(void) { return g_kernel; }
 // every call of the HIP runtime takes (hipEventRecord ends the process on the handle).
 void *swc_hip_stream(void) { return g.ready && !g.cur ? (void *)hipStreamLegacy : (void *)g.cur; }
 
+namespace {
+// (the null stream is never recorded; asking about it can fail while another stream is)
+int is_recorded(hipStream_t s, bool *yes) {
+    *yes = false;
+    if (!s) return SWC_HIP_OK;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    SWC_HIP_TRY(hipStreamIsCapturing(s, &status));
+    *yes = status != hipStreamCaptureStatusNone;
+    return SWC_HIP_OK;
+}
+} // namespace
+
+// The workspace, and whatever else the ops on the stream that is left still write, is used on the new one: its work waits
+// for theirs.  A caller's stream may have been destroyed before it is left, so only the library's own and the null stream
+// are waited for; a stream that is being recorded must not wait for work outside its graph.
 int swc_hip_set_stream(void *s) {
     SWC_REQUIRE_INIT();
     std::lock_guard<std::mutex> lk(g.mu);
-    if (s) {
-        g.cur = (hipStream_t)s == hipStreamLegacy ? nullptr : (hipStream_t)s;
-        g.cur_is_own = false;
-    } else {
-        g.cur = g.own;
-        g.cur_is_own = true;
+    if (g.capturing) return fail(SWC_HIP_EINVAL, "swc_hip_set_stream: not while a graph is being recorded");
+    const hipStream_t next = !s ? g.own : (hipStream_t)s == hipStreamLegacy ? nullptr : (hipStream_t)s;
+    if (next != g.cur && (!g.cur || g.cur == g.own)) {
+        bool left = false, entered = false;
+        if (int rc = is_recorded(g.cur, &left)) return rc;
+        if (int rc = is_recorded(next, &entered)) return rc;
+        if (!left && !entered) {
+            SWC_HIP_TRY(hipEventRecord(g.ev_switch, g.cur));
+            SWC_HIP_TRY(hipStreamWaitEvent(next, g.ev_switch, 0));
+        }
     }
+    g.cur = next;
+    g.cur_is_own = !s;
     return SWC_HIP_OK;
 }
 
