@@ -107,7 +107,10 @@ int swc_hip_set_workspace(void *dptr, size_t bytes);
  * that call ops of many shapes; a generated program never needs it.  The
  * library's buffer is not replaced while a graph is being recorded, nor while an
  * executable graph recorded on it is still alive (the call that would need it
- * fails instead, and so does swc_hip_set_workspace). */
+ * fails instead, and so does swc_hip_set_workspace).  A graph recorded by other
+ * means than swc_hip_graph_begin (the caller captures the stream that
+ * swc_hip_set_stream names) is seen when its ops are recorded: the buffer they use
+ * is never freed before swc_hip_shutdown, also when a larger one replaces it. */
 int swc_hip_enable_auto_workspace(int enable);
 /* No counterpart in the reference.  Workspace a matrixMatrixMul_f /
  * matrixMatrixFCBias_f call of this shape uses on the initialised device (0 for

@@ -42,6 +42,11 @@ struct State {
     // address, so it is neither freed nor replaced before the last of them is destroyed
     void *graphs_on_own_ws[kGraphSlots] = {};
     int n_graphs_on_own_ws = 0;
+    // a graph that a caller recorded by other means (the stream was being captured, not by swc_hip_graph_begin) may hold the
+    // own buffer's address for as long as the process runs: such a buffer, once replaced, is kept until shutdown
+    bool ws_kept = false;
+    void *kept[kGraphSlots] = {};
+    int n_kept = 0;
 } g;
 
 Switches g_switches;
@@ -110,15 +115,53 @@ hipStream_t stream() { return g.cur; }
 bool ready() { return g.ready; }
 int num_cus() { return g.cus; }
 
+namespace {
+// Whether work on `s` goes into a graph.  (The null stream is never recorded; asking about it can fail while another is.)
+int is_recorded(hipStream_t s, bool *yes) {
+    *yes = false;
+    if (!s) return SWC_HIP_OK;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    SWC_HIP_TRY(hipStreamIsCapturing(s, &status));
+    *yes = status != hipStreamCaptureStatusNone;
+    return SWC_HIP_OK;
+}
+
+// Lets go of the library's own buffer, which no later op uses: freed, or kept for the graphs that may hold its address.
+int drop_own_workspace(const char *who) {
+    if (g.ws_kept) {
+        if (g.n_kept == kGraphSlots)
+            return fail(SWC_HIP_ERUNTIME, "%s: %d buffers are kept for recorded graphs; provide a workspace large enough for every "
+                        "op with swc_hip_set_workspace before recording", who, kGraphSlots);
+        g.kept[g.n_kept++] = g.ws;
+    } else {
+        SWC_HIP_TRY(hipStreamSynchronize(g.cur));   // earlier ops may still be using it
+        SWC_HIP_TRY(hipFree(g.ws));
+    }
+    g.ws = nullptr;
+    g.ws_bytes = 0;
+    g.ws_kept = false;
+    return SWC_HIP_OK;
+}
+} // namespace
+
 // Device memory an op may use until it returns control to the stream's next op
 // (all ops run on one in-order stream, so one buffer serves them all).  Ops never
 // allocate: the buffer is the caller's (swc_hip_set_workspace), sized with the
 // swc_hip_*_workspace_bytes queries.  Only a caller that opted in with
 // swc_hip_enable_auto_workspace lets the library keep one of its own, grown on
 // demand — never while a graph is being recorded, where allocating is not
-// allowed, and never while a recorded graph still holds the old buffer's address.
+// allowed, and never while a recorded graph still holds the old buffer's address;
+// behind a graph recorded by other means than swc_hip_graph_begin the old buffer
+// is kept.
 void *workspace(size_t bytes, const char *who) {
-    if (bytes <= g.ws_bytes && g.ws) return g.ws;
+    const bool fits = bytes <= g.ws_bytes && g.ws;
+    if (fits && (!g.ws_owned || g.ws_kept)) return g.ws;
+    bool recorded = false;
+    if (is_recorded(g.cur, &recorded) != SWC_HIP_OK) return nullptr;
+    if (fits) {
+        g.ws_kept = recorded && !g.capturing;   // (a graph of swc_hip_graph_begin is counted at its end)
+        return g.ws;
+    }
     if (g.ws && !g.ws_owned) {
         fail(SWC_HIP_EINVAL, "%s: the workspace given to swc_hip_set_workspace has %zu bytes, %zu are needed", who,
              g.ws_bytes, bytes);
@@ -131,7 +174,7 @@ void *workspace(size_t bytes, const char *who) {
              "swc_hip_enable_auto_workspace lets the library keep a buffer of its own)", who, bytes);
         return nullptr;
     }
-    if (g.capturing) {
+    if (recorded || g.capturing) {
         fail(SWC_HIP_ERUNTIME, "%s: needs a %zu-byte workspace, which cannot be allocated while a graph is recorded; "
              "run the op once eagerly first or provide one with swc_hip_set_workspace", who, bytes);
         return nullptr;
@@ -143,12 +186,7 @@ void *workspace(size_t bytes, const char *who) {
              g.ws_bytes);
         return nullptr;
     }
-    if (g.ws) {
-        (void)hipStreamSynchronize(g.cur);   // earlier ops may still be using it
-        (void)hipFree(g.ws);
-        g.ws = nullptr;
-        g.ws_bytes = 0;
-    }
+    if (g.ws && drop_own_workspace(who) != SWC_HIP_OK) return nullptr;
     const size_t want = (bytes + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
     hipError_t e = hipMalloc(&g.ws, want);
     if (e != hipSuccess) {
@@ -219,6 +257,8 @@ int swc_hip_shutdown(void) {
     g.ws_bytes = 0;
     g.ws_owned = false;
     g.ws_auto = false;
+    g.ws_kept = false;
+    while (g.n_kept) (void)hipFree(g.kept[--g.n_kept]);
     g.n_graphs_on_own_ws = 0;
     for (void *&h : g.graphs_on_own_ws) h = nullptr;
     (void)hipEventDestroy(g.t0);
@@ -257,8 +297,10 @@ int swc_hip_set_workspace(void *dptr, size_t bytes) {
         if (g.n_graphs_on_own_ws > 0)
             return fail(SWC_HIP_ERUNTIME, "swc_hip_set_workspace: %d recorded graph(s) still use the library's own "
                         "buffer; destroy them before replacing it", g.n_graphs_on_own_ws);
-        SWC_HIP_TRY(hipStreamSynchronize(g.cur));
-        SWC_HIP_TRY(hipFree(g.ws));
+        bool recorded = false;
+        if (int rc = is_recorded(g.cur, &recorded)) return rc;
+        if (recorded) return fail(SWC_HIP_EINVAL, "swc_hip_set_workspace: not while a graph is being recorded");
+        if (int rc = drop_own_workspace("swc_hip_set_workspace")) return rc;
     }
     g.ws = dptr;
     g.ws_bytes = bytes;
@@ -429,18 +471,6 @@ const char *swc_hip_last_kernel(void) { return g_kernel; }
 // The null stream is named by its handle here, where NULL means the library's own; inside it is the null pointer, which
 // every call of the HIP runtime takes (hipEventRecord ends the process on the handle).
 void *swc_hip_stream(void) { return g.ready && !g.cur ? (void *)hipStreamLegacy : (void *)g.cur; }
-
-namespace {
-// (the null stream is never recorded; asking about it can fail while another stream is)
-int is_recorded(hipStream_t s, bool *yes) {
-    *yes = false;
-    if (!s) return SWC_HIP_OK;
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    SWC_HIP_TRY(hipStreamIsCapturing(s, &status));
-    *yes = status != hipStreamCaptureStatusNone;
-    return SWC_HIP_OK;
-}
-} // namespace
 
 // The workspace, and whatever else the ops on the stream that is left still write, is used on the new one: its work waits
 // for theirs.  A caller's stream may have been destroyed before it is left, so only the library's own and the null stream

@@ -1,12 +1,22 @@
 """Streams and recorded graphs of the operators of language models: the null stream, and what is ordered when the launch
 stream changes."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 
 EINVAL = 1
 gpu = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def run_with_torch(program):
+    """in a process of its own: torch brings its own HIP runtime, which has to be the first one loaded"""
+    done = subprocess.run([sys.executable, "-u", "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=110)
+    assert done.returncode == 0 and done.stdout.endswith("done\n"), done.stdout[-1000:] + done.stderr[-2000:]
 
 
 @pytest.fixture(scope="module")
@@ -100,3 +110,54 @@ def test_no_change_of_stream_while_recording(rt):
     finally:
         rt._check(rt.lib.swc_hip_graph_end(C.byref(graph)), "end")
     rt._check(rt.lib.swc_hip_graph_destroy(graph), "destroy")
+
+
+RECORDED_BY_TORCH = """
+import torch
+assert torch.cuda.is_available()
+from swcompiler_amd.hip import SwcHipError, runtime
+rt = runtime()
+rt.use_default_stream()
+gen = torch.Generator().manual_seed(3)
+ints = lambda *s: torch.randint(-3, 4, s, generator=gen).to("cuda", torch.bfloat16)
+m, n, k = 70, 301, 75          # (rows off the 16-byte grid: both operands are copied into the workspace)
+a, b = ints(m, k), ints(k, n)
+c = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+large, weight = ints(3000, 1001), ints(1001, 3001)
+side = torch.cuda.Stream()
+rt.matrixMatrixFCActAdd(a, b, out=c)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    rt._check(rt.lib.swc_hip_set_stream(side.cuda_stream), "set_stream")
+    rt.matrixMatrixFCActAdd(a, b, None, "relu", out=c)
+    try:                       # more than the buffer holds: refused, and the recording goes on
+        rt.matrixMatrixFCActAdd(large, weight, out=torch.empty(3000, 3001, dtype=torch.bfloat16, device="cuda"))
+    except SwcHipError as e:
+        assert "while a graph is recorded" in str(e), e
+    else:
+        raise AssertionError("a workspace was allocated during a recording")
+torch.cuda.synchronize()
+rt.use_default_stream()
+for i in range(4):
+    print("replay", i, flush=True)
+    # the library's buffer is replaced by a larger one; what was freed would be reused here
+    big = torch.empty(3000 - i, 3001, dtype=torch.bfloat16, device="cuda")
+    rt.matrixMatrixFCActAdd(large[i:], weight, out=big)
+    other = [torch.full((1 << 18,), float("nan"), device="cuda") for _ in range(64)]
+    a.copy_(ints(m, k))
+    c.fill_(7)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = (a.float() @ b.float()).clamp(min=0).bfloat16()
+    assert torch.equal(c, want), (c - want).abs().max()
+    assert all(bool(x.isnan().all()) for x in other)
+    assert torch.equal(big, (large[i:].float() @ weight.float()).bfloat16())
+print("done")
+"""
+
+
+@gpu
+def test_a_graph_recorded_by_torch_keeps_its_workspace():
+    """ops recorded into a torch graph replay correctly after a larger call has replaced the library's own workspace"""
+    run_with_torch(RECORDED_BY_TORCH)
