@@ -5,14 +5,16 @@ Method names and argument order mirror the reference's CPU kernels
 parity test reads like a call sequence of the reference's generated program.
 Data lives in DeviceArray objects (device memory + shape); numpy arrays cross
 only through upload()/download().  The operators of language models take torch tensors too, as
-they are; a program that uses torch imports it before this library is loaded
-(torch brings a HIP runtime of its own, and a process has one), and shares its
-stream (use_default_stream) or synchronises between the two.
+they are, and order themselves with the work on torch's current stream; a program
+that uses torch imports it before this library is loaded (torch brings a HIP
+runtime of its own, and a process has one).  Sharing a stream
+(use_default_stream) saves the waits between the two.
 
 No fallback: a missing library or device raises SwcHipError.
 """
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -199,7 +201,10 @@ class _Arg:
     __slots__ = ("ptr", "shape", "type", "ld")
 
     def __init__(self, rt, x, what, name):
-        self.shape = shape = x.shape
+        try:
+            self.shape = shape = x.shape
+        except AttributeError:
+            raise _no_operand(x, what, name) from None
         self.ld = shape[-1] if shape else 1
         if isinstance(x, DeviceArray):
             self.ptr, self.type = x.ptr, _NUMPY_TYPES.get(x.dtype.name)
@@ -224,6 +229,10 @@ class _Arg:
         return n
 
 
+def _no_operand(x, what, name):
+    return SwcHipError(f"{what}: {name}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
+
+
 def _torch_operand(rt, x, what, name):
     """-> (address, element type) of a torch tensor on the runtime's device"""
     try:
@@ -232,12 +241,14 @@ def _torch_operand(rt, x, what, name):
         kind = _TORCH_KINDS.get(x.dtype)
         ptr = x.data_ptr()
     except AttributeError:
-        raise SwcHipError(f"{what}: {name}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}") from None
+        raise _no_operand(x, what, name) from None
     if kind is None:
         kind = _TORCH_KINDS[x.dtype] = _TORCH_TYPES.get(str(x.dtype), "?")
+    rt._torch_given = True
     return ptr or None, kind
 
 
+_NULL_STREAM = 1      # the library's name for the null stream (hipStreamLegacy); torch's is 0
 _TORCH_KINDS = {}     # torch.dtype -> element type, filled as they are met (this module does not import torch)
 _NUMPY_TYPES = {"float32": "f32", "int32": "i32", "uint16": "bf16", "uint8": "u8"}   # bfloat16 travels as its bits
 _TORCH_TYPES = {"torch.float32": "f32", "torch.int32": "i32", "torch.bfloat16": "bf16", "torch.uint16": "bf16",
@@ -295,6 +306,8 @@ class DeviceArray:
 class SwcHip:
     """One process-wide runtime: device 0 unless told otherwise."""
 
+    _torch_given = False   # whether an operand of the call being made is a torch tensor
+
     def __init__(self, device=0, auto_workspace=True):
         """auto_workspace: let the library keep (and grow) a scratch buffer of its own, as a harness that calls
         ops of many shapes wants; False: ops that need scratch fail until set_workspace() provides it, as in a
@@ -322,7 +335,7 @@ class SwcHip:
 
     def use_default_stream(self):
         """launch on the device's default (null) stream, the one torch uses unless told otherwise"""
-        self._check(self.lib.swc_hip_set_stream(C.c_void_p(1)), "swc_hip_set_stream")   # hipStreamLegacy
+        self._check(self.lib.swc_hip_set_stream(C.c_void_p(_NULL_STREAM)), "swc_hip_set_stream")
 
     # -- plumbing --------------------------------------------------------
     def _check(self, rc, what):
@@ -702,26 +715,48 @@ class SwcHip:
         return out
 
     # -- operators of language models (matrices fp32 or bfloat16; DeviceArrays or torch tensors) --
+    def _launch(self, what, fn, *args):
+        """The library's call.  With torch tensors among the operands it comes behind the work on torch's current stream,
+        and that stream's later work (and whatever reuses the operands' memory there) behind it."""
+        if self._torch_given:
+            self._torch_given = False
+            # (half a microsecond a call: torch.cuda's own forms of these questions take three times that)
+            torch = sys.modules["torch"]
+            device, theirs, ours = torch._C._cuda_getDevice(), torch._C._cuda_getCurrentRawStream(self.device), self.lib.swc_hip_stream()
+            if device != self.device:
+                raise SwcHipError(f"{what}: the current device is {device}, the runtime's {self.device}")
+            if theirs != ours and (theirs or ours != _NULL_STREAM):
+                return self._launch_between(what, torch, ours, fn, args)
+        rc = fn(*args)
+        if rc:
+            self._check(rc, what)
+
+    def _launch_between(self, what, torch, ours, fn, args):
+        """_launch where torch's stream is not the library's"""
+        theirs = torch.cuda.current_stream(self.device)
+        if torch.cuda.is_current_stream_capturing():
+            raise SwcHipError(f"{what}: torch is recording a graph on another stream than the library's: name it with "
+                              "swc_hip_set_stream first")
+        ours = torch.cuda.default_stream(self.device) if ours == _NULL_STREAM else torch.cuda.ExternalStream(ours, self.device)
+        with torch.cuda.stream(ours):
+            recording = torch.cuda.is_current_stream_capturing()
+        if recording:   # (into a graph, which is ordered where it is launched)
+            return self._check(fn(*args), what)
+        ours.wait_stream(theirs)
+        rc = fn(*args)
+        theirs.wait_stream(ours)
+        self._check(rc, what)
+
     def _arg(self, x, what, name, types, shape=None):
         """the operand as an _Arg; None for None"""
         if x is None:
             return None
-        if not hasattr(x, "shape"):
-            raise SwcHipError(f"{what}: {name}: expected a DeviceArray or a torch tensor on the GPU, got {type(x).__name__}")
         a = _Arg(self, x, what, name)
         if a.type not in types:
             raise SwcHipError(f"{what}: {name}: element type {a.type or x.dtype} is not one of {', '.join(types)}")
         if shape is not None and a.shape != shape:
             raise SwcHipError(f"{what}: {name}: shape {tuple(a.shape)}, expected {shape}")
         return a
-
-    @staticmethod
-    def _p(a):
-        return None if a is None else a.ptr
-
-    @staticmethod
-    def _ld(a, other=0):
-        return other if a is None else a.ld
 
     def _out(self, out, shape, like):
         return out if out is not None else self.empty(shape, np.float32 if like == "f32" else np.uint16)
@@ -730,7 +765,8 @@ class SwcHip:
         a, b = self._arg(a, what, "a", ("f32", "bf16")), self._arg(b, what, "b", ("f32", "bf16"))
         if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0] or a.type != b.type:
             raise SwcHipError(f"{what}: a {a.shape} {a.type} and b {b.shape} {b.type} do not multiply")
-        m, n, k = _int32(a.shape[0], what), _int32(b.shape[1], what), _int32(a.shape[1], what)
+        (m, k), n = a.shape, b.shape[1]
+        _int32(m if m > n and m > k else n if n > k else k, what)
         return a, b, m, n, k, (a.type,), "_f" if a.type == "f32" else "_bf"
 
     @staticmethod
@@ -748,9 +784,9 @@ class SwcHip:
         c = self._arg(out, what, "out", t, (m, n))
         bias, r = self._arg(bias, what, "bias", t, (n,)), self._arg(residual, what, "residual", t, (m, n))
         z = self._arg(preact, what, "preact", t, (m, n))
-        self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAdd" + suffix)(
-            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), act, self._p(r), self._ld(r), self._p(z),
-            self._ld(z), c.ptr, c.ld), what)
+        self._launch(what, getattr(self.lib, "swc_hip_matrixMatrixFCActAdd" + suffix),
+                     m, n, k, a.ptr, a.ld, b.ptr, b.ld, bias and bias.ptr, act, r and r.ptr, r.ld if r else 0, z and z.ptr,
+                     z.ld if z else 0, c.ptr, c.ld)
         return out
 
     def matrixMatrixFCActAddGrad(self, dc, a, b, preact=None, act="none", da=None, db=None, dbias=None):
@@ -763,9 +799,9 @@ class SwcHip:
         g, z = self._arg(dc, what, "dc", t, (m, n)), self._arg(preact, what, "preact", t, (m, n))
         ga, gb = self._arg(da, what, "da", t, (m, k)), self._arg(db, what, "db", t, (k, n))
         gbias = self._arg(dbias, what, "dbias", t, (n,))
-        self._check(getattr(self.lib, "swc_hip_matrixMatrixFCActAddGrad" + suffix)(
-            m, n, k, g.ptr, g.ld, a.ptr, a.ld, b.ptr, b.ld, self._p(z), self._ld(z), act, self._p(ga),
-            self._ld(ga), self._p(gb), self._ld(gb), self._p(gbias)), what)
+        self._launch(what, getattr(self.lib, "swc_hip_matrixMatrixFCActAddGrad" + suffix),
+                     m, n, k, g.ptr, g.ld, a.ptr, a.ld, b.ptr, b.ld, z and z.ptr, z.ld if z else 0, act, ga and ga.ptr,
+                     ga.ld if ga else 0, gb and gb.ptr, gb.ld if gb else 0, gbias and gbias.ptr)
         return da, db, dbias
 
     def matrixFCSoftmaxWithLoss(self, a, b, bias, selected, row_loss=None, lse=None, loss=None):
@@ -778,8 +814,8 @@ class SwcHip:
         if one.size != 1:
             raise SwcHipError(f"{what}: loss: shape {one.shape}, expected one value")
         rl, ls = self._arg(row_loss, what, "row_loss", ("f32",), (m,)), self._arg(lse, what, "lse", ("f32",), (m,))
-        self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLoss" + suffix)(
-            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, rl.ptr, ls.ptr, one.ptr), what)
+        self._launch(what, getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLoss" + suffix),
+                     m, n, k, a.ptr, a.ld, b.ptr, b.ld, bias and bias.ptr, sel.ptr, rl.ptr, ls.ptr, one.ptr)
         return loss, row_loss, lse
 
     def matrixFCSoftmaxWithLossGrad(self, a, b, bias, selected, lse, row_grad=None, da=None, db=None, dbias=None):
@@ -793,9 +829,9 @@ class SwcHip:
         ls, rg = self._arg(lse, what, "lse", ("f32",), (m,)), self._arg(row_grad, what, "row_grad", ("f32",), (m,))
         ga, gb = self._arg(da, what, "da", t, (m, k)), self._arg(db, what, "db", t, (k, n))
         gbias = self._arg(dbias, what, "dbias", t, (n,))
-        self._check(getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLossGrad" + suffix)(
-            m, n, k, a.ptr, a.ld, b.ptr, b.ld, self._p(bias), sel.ptr, ls.ptr, self._p(rg), self._p(ga), self._ld(ga),
-            self._p(gb), self._ld(gb), self._p(gbias)), what)
+        self._launch(what, getattr(self.lib, "swc_hip_matrixFCSoftmaxWithLossGrad" + suffix),
+                     m, n, k, a.ptr, a.ld, b.ptr, b.ld, bias and bias.ptr, sel.ptr, ls.ptr, rg and rg.ptr, ga and ga.ptr, ga.ld if ga else 0,
+                     gb and gb.ptr, gb.ld if gb else 0, gbias and gbias.ptr)
         return da, db, dbias
 
     def adamw_state(self):
@@ -810,7 +846,7 @@ class SwcHip:
     def adamwAdvance(self, state, beta1, beta2):
         """begins a step: counts it and prepares the bias corrections of the updates that follow"""
         state = self._state(state, "adamwAdvance")
-        self._check(self.lib.swc_hip_adamwAdvance(state, beta1, beta2), "adamwAdvance")
+        self._launch("adamwAdvance", self.lib.swc_hip_adamwAdvance, state, beta1, beta2)
 
     def _adamw(self, what, w, dw, states, scales, copies, state, lr, beta1, beta2, eps, decay, lr_factor, grad_factor):
         count = len(w)
@@ -825,6 +861,7 @@ class SwcHip:
                 if kind in types and all([x.is_contiguous() and x.get_device() == self.device for x in values]):
                     found = [x.numel() for x in values]
                     if sizes is None or found == sizes:
+                        self._torch_given = True
                         return (C.c_void_p * count)(*[x.data_ptr() for x in values]), found, kind
             except AttributeError:
                 pass
@@ -865,9 +902,9 @@ class SwcHip:
         factors = [self._arg(x, what, "factor", ("f32",)) for x in (lr_factor, grad_factor)]
         if any(x is not None and x.size != 1 for x in factors):
             raise SwcHipError(f"{what}: a factor is one value")
-        one = [self._p(x) for x in factors]
+        one = [x and x.ptr for x in factors]
         fn = getattr(self.lib, f"swc_hip_{what}" + ("_bf" if dtype == "bf16" else "_f"))
-        self._check(fn(count, *pointers, sizes, self._state(state, what), lr, beta1, beta2, eps, decay, *one), what)
+        self._launch(what, fn, count, *pointers, sizes, self._state(state, what), lr, beta1, beta2, eps, decay, *one)
 
     def adamw(self, w, dw, mom, var, state, lr, beta1, beta2, eps, decay, copies=None, lr_factor=None, grad_factor=None):
         """one AdamW step of the tensors in the lists w, dw, mom, var (and their bfloat16 copies), in place"""

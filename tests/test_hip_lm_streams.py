@@ -1,5 +1,5 @@
-"""Streams and recorded graphs of the operators of language models: the null stream, and what is ordered when the launch
-stream changes."""
+"""Streams and recorded graphs of the operators of language models: the null stream, what is ordered when the launch stream
+changes, and calls with torch tensors."""
 import ctypes as C
 import os
 import subprocess
@@ -7,6 +7,9 @@ import sys
 
 import numpy as np
 import pytest
+
+from swcompiler_amd import hip
+from swcompiler_amd.hip import SwcHipError
 
 EINVAL = 1
 gpu = pytest.mark.gpu
@@ -161,3 +164,184 @@ print("done")
 def test_a_graph_recorded_by_torch_keeps_its_workspace():
     """ops recorded into a torch graph replay correctly after a larger call has replaced the library's own workspace"""
     run_with_torch(RECORDED_BY_TORCH)
+
+
+# ------------------------------------------------------------------------- torch's streams: who waits for whom (no device)
+class _FakeTorch:
+    """as much of torch as the binding asks about streams, and a log of what it is told"""
+
+    def __init__(self, current=0, device=0, capturing=()):
+        self.log, self.now, self.device, self.capturing = [], current, device, capturing
+        self.cuda, self._C = self, self
+
+    def stream_of(self, handle):
+        fake = self
+
+        class Stream:
+            cuda_stream = handle
+
+            def wait_stream(self, other):
+                fake.log.append(f"{handle} waits for {other.cuda_stream}")
+
+            def __enter__(self):
+                self.before, fake.now = fake.now, handle
+
+            def __exit__(self, *_):
+                fake.now = self.before
+        return Stream()
+
+    def _cuda_getDevice(self):
+        return self.device
+
+    def _cuda_getCurrentRawStream(self, device):
+        return self.now
+
+    def current_stream(self, device):
+        return self.stream_of(self.now)
+
+    def default_stream(self, device):
+        return self.stream_of(0)
+
+    def ExternalStream(self, handle, device):
+        return self.stream_of(handle)
+
+    def stream(self, s):
+        return s
+
+    def is_current_stream_capturing(self):
+        return self.now in self.capturing
+
+
+class _FakeTensor:
+    dtype, shape = "torch.float32", (4, 8)
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return 1 << 20
+
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return 32
+
+
+class _FakeLib:
+    def __init__(self, fake, stream):
+        self.fake, self.handle = fake, stream
+
+    def swc_hip_stream(self):
+        return self.handle
+
+    def __getattr__(self, name):
+        return lambda *args: self.fake.log.append("call") or 0
+
+
+def call_with(monkeypatch, ours, **kw):
+    fake = _FakeTorch(**kw)
+    monkeypatch.setitem(sys.modules, "torch", fake)
+    rt = object.__new__(hip.SwcHip)
+    rt.device, rt.lib = 0, _FakeLib(fake, ours)
+    a, b, c = _FakeTensor(), _FakeTensor(), _FakeTensor()
+    b.shape, c.shape = (8, 8), (4, 8)
+    try:
+        rt.matrixMatrixFCActAdd(a, b, out=c)
+        first, fake.log = fake.log, []
+        rt.adamw([a], [a], [a], [a], _state(), 1e-3, 0.9, 0.99, 1e-8, 0.0)
+        assert fake.log == first
+        return first
+    finally:
+        hip._TORCH_KINDS.clear()
+
+
+def _state():
+    x = _FakeTensor()
+    x.dtype, x.shape = "torch.int32", (hip.ADAMW_STATE_WORDS,)
+    return x
+
+
+def test_calls_with_torch_operands_are_ordered(monkeypatch):
+    assert call_with(monkeypatch, 1) == ["call"]                   # both the null stream
+    assert call_with(monkeypatch, 77, current=77) == ["call"]
+    assert call_with(monkeypatch, 77) == ["77 waits for 0", "call", "0 waits for 77"]
+    assert call_with(monkeypatch, 1, current=5) == ["0 waits for 5", "call", "5 waits for 0"]
+    assert call_with(monkeypatch, 77, capturing=(77,)) == ["call"]     # recorded by the library: ordered where launched
+
+
+def test_torch_operands_are_refused_where_they_cannot_be_ordered(monkeypatch):
+    with pytest.raises(SwcHipError, match="torch is recording a graph on another stream"):
+        call_with(monkeypatch, 77, current=5, capturing=(5,))
+    with pytest.raises(SwcHipError, match="the current device is 1, the runtime's 0"):
+        call_with(monkeypatch, 1, device=1)
+
+
+TORCH_STREAMS = """
+import torch
+assert torch.cuda.is_available()
+from swcompiler_amd.hip import SwcHipError, runtime
+rt = runtime()
+gen = torch.Generator().manual_seed(3)
+n = 2048
+ints = lambda *s: torch.randint(-2, 3, s, generator=gen).to("cuda")
+eye, w = torch.eye(n, device="cuda"), ints(64, 200).bfloat16()
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+
+
+def late(value):
+    # `value` behind some milliseconds of torch's work
+    x = eye
+    for _ in range(30):
+        x = x @ eye
+    return value * x[:1, :1].bfloat16()
+
+
+def check(name):
+    for i in range(5):
+        a = late(ints(70, 64).bfloat16())
+        c = torch.full((70, 200), 7, device="cuda", dtype=torch.bfloat16)
+        rt.matrixMatrixFCActAdd(a, w, None, "relu", out=c)
+        got = c.float()                       # torch's next work reads the result ...
+        want = (a.float() @ w.float()).clamp(min=0).bfloat16().float()
+        del a, c                              # ... and its allocator reuses the operands
+        junk = [torch.full((70, 200), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(8)]
+        g = late(ints(300).bfloat16())[0] * 0.5
+        p, m, v = (torch.zeros(300, device="cuda") for _ in range(3))
+        state = torch.zeros(8, dtype=torch.int32, device="cuda")
+        rt.adamwAdvance(state, 0.9, 0.99)
+        rt.adamw([p], [g], [m], [v], state, 1e-3, 0.9, 0.99, 1e-8, 0.0)
+        steps, mean = state[0].clone(), m * 10
+        torch.cuda.current_stream().synchronize()
+        assert torch.equal(got, want), name
+        assert int(steps) == 1 and torch.allclose(mean, g.float(), rtol=1e-5), name
+
+
+for library in ("own", "null"):
+    if library == "null":
+        rt.use_default_stream()
+    print("library on its", library, "stream", flush=True)
+    check(library + ", torch on its default stream")
+    with torch.cuda.stream(side):
+        check(library + ", torch on a side stream")
+torch.cuda.synchronize()
+graph, c = torch.cuda.CUDAGraph(), torch.empty(70, 200, device="cuda", dtype=torch.bfloat16)
+a = ints(70, 64).bfloat16()
+with torch.cuda.graph(graph):
+    c.fill_(1)
+    try:
+        rt.matrixMatrixFCActAdd(a, w, out=c)
+    except SwcHipError as e:
+        assert "torch is recording" in str(e), e
+    else:
+        raise AssertionError("an op that the graph would lack")
+print("done")
+"""
+
+
+@gpu
+def test_torch_streams():
+    """torch on its default and on a side stream, the library on its own and on the null stream: results are ordered with
+    the work before and behind the calls, no synchronisation between them"""
+    run_with_torch(TORCH_STREAMS)
