@@ -447,7 +447,7 @@ size_t swc_hip_conv2dFusedMaxpool_workspace_bytes(const size_t *cdims, const siz
 /* the activations */
 enum {
     SWC_HIP_ACT_NONE = 0,
-    SWC_HIP_ACT_RELU = 1,
+    SWC_HIP_ACT_RELU = 1,       /* z where z > 0, else 0: also of a NaN, as in relu_f */
     SWC_HIP_ACT_GELU = 2,       /* z/2 (1 + erf(z / sqrt 2)) */
     SWC_HIP_ACT_GELU_TANH = 3,  /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
     SWC_HIP_ACT_SILU = 4        /* z / (1 + e^-z) */
@@ -472,7 +472,8 @@ size_t swc_hip_matrixMatrixFCActAdd_workspace_bytes(int m, int n, int k, int bf)
 /* Its gradients from cGrad, the gradient of C:
  *     dZ = cGrad * act'(preact)      aGrad[m,k] = dZ * B^T
  *     bGrad[k,n] = A^T * dZ          biasGrad[n] = column sums of dZ
- * (the gradient of the residual is cGrad itself).  Any of aGrad, bGrad and
+ * (the gradient of the residual is cGrad itself).  Where a ReLU's preact is not
+ * positive dZ is 0 whatever cGrad holds, as in reluGrad_f.  Any of aGrad, bGrad and
  * biasGrad may be NULL and is then not computed; all are overwritten.  preact
  * may be NULL when act is SWC_HIP_ACT_NONE.  The _bf form holds dZ in bfloat16
  * for the two products and in fp32 for the column sums. */

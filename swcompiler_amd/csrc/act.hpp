@@ -54,11 +54,10 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z
     return z;
 }
 
-// The slope at z.  The second terms vanish long before |z| = 40; z is held there so that infinities times zero do not
+// The slope of a smooth activation at z.  The second terms vanish long before |z| = 40; z is held there so that infinities times zero do not
 // make them NaN.
 template <int ACT, bool FAST> __device__ __forceinline__ float act_slope(float z) {
-    if (ACT == SWC_HIP_ACT_NONE) return 1.f;
-    if (ACT == SWC_HIP_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    static_assert(ACT >= SWC_HIP_ACT_GELU, "the others have no slope to compute");
     const float y = fminf(fmaxf(z, -40.f), 40.f);
     float s = 1.f;
     if (ACT == SWC_HIP_ACT_GELU) {
@@ -73,6 +72,13 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_slope(float z
         s = p * (1.f + y * (1.f - p));
     }
     return z == z ? s : z;   // (fminf and fmaxf drop a NaN)
+}
+
+// The gradient g of a value, taken to its argument z.  An inactive ReLU passes nothing on, not even infinities and NaN (as
+// reluGrad_f): in the products behind it one of them would fill a row and a column.
+template <int ACT, bool FAST> __device__ __forceinline__ float act_grad_value(float z, float g) {
+    if constexpr (ACT == SWC_HIP_ACT_RELU) return z > 0.f ? g : 0.f;
+    else return g * act_slope<ACT, FAST>(z);
 }
 #endif
 

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void act_grad(T *dz, long ld, const T *dc, lon
                 float y[4];
                 load4(z + r * ldz + j, have, y);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) g[e] *= act_slope<ACT, kIsBf16<T>>(y[e]);
+                for (int e = 0; e < 4; ++e) g[e] = act_grad_value<ACT, kIsBf16<T>>(y[e], g[e]);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
