@@ -689,8 +689,8 @@ int launch_product(const Shape<T> &s, const Ep &ep, const char *who) {
     const long groups = (long)((s.m + C::BM - 1) / C::BM) * ((s.n + C::BN - 1) / C::BN) * s.splits;
     // (a grid has at most 2^32 - 1 threads in each direction)
     if (groups > 0xffffffffL / C::kThreads) return fail(SWC_HIP_EUNSUPPORTED, "%s: too many tiles", who);
-    note_kernel("product<%s,%dx%d,%d,%d,%s%s> x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, C::SA, C::SB, LA == kAlongK ? "k" : "m",
-                LB == kAlongK ? "k" : "n", s.splits);
+    note_kernel("product<%s,%dx%d,%d,%d,%d,%s%s> x%d", kIsBf16<T> ? "bf16" : "fp32", C::BM, C::BN, C::NW, C::SA, C::SB,
+                LA == kAlongK ? "k" : "m", LB == kAlongK ? "k" : "n", s.splits);
     auto kern = product_tiles<T, C, LA, LB, Ep>;
     static bool attr_set = false;
     if (!attr_set) {
