@@ -566,13 +566,17 @@ int swc_hip_adamw_bf(int count, float *const *w, const swc_hip_bf16 *const *dw, 
  * 448, no infinities).  A step decodes both, updates as above in fp32 and encodes
  * them again with scale = (largest finite magnitude of the block) * (1/448 as an
  * fp32), or 0, and the block as zeros, where that magnitude is at most 2^-100:
- * mom / scale, as an fp32, to the nearest value, ties to even; sqrt(var) up or
- * down at random with the probabilities that keep its expectation (a variance
- * decays by less per step than half the distance of two values, and would never
- * move if it were rounded to the nearest), but a positive one never to zero.  The
+ * mom / scale, as an fp32, to the nearest value, ties to even, where beta1 is
+ * below 15/16; sqrt(var), and mom / scale from there on, up or down at random with
+ * the probabilities that keep the expectation (a variance decays by less per step
+ * than half the distance of two values, and would never move if it were rounded to
+ * the nearest; nor would such a mean), but a positive sqrt(var) never to zero.  (To
+ * the nearest, a mean stops moving once (1 - beta1) |g - mom| is less than half the
+ * distance of two values, at most mom/16: under a gradient that never changes it can
+ * stay off it by mom / (16 (1 - beta1)), 0.6 mom at beta1 0.9.)  The
  * random number of element i of tensor t in step s is 20 bits of a hash of
- * (i + t * 0x9E3779B9 + s * 0x85EBCA6B) modulo 2^32: the same step gives the same
- * bits.  A value that is not
+ * (i + t * 0x9E3779B9 + s * 0x85EBCA6B) modulo 2^32, for mom of that sum's
+ * complement: the same step gives the same bits.  A value that is not
  * finite is held as NaN.  w is updated from the unrounded states.  momScale and
  * varScale hold (size + SWC_HIP_ADAMW_BLOCK - 1) / SWC_HIP_ADAMW_BLOCK floats per tensor;
  * all zero is the state before the first step. */

@@ -170,6 +170,9 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// A published 32-bit mixing function (C. Wellons, 2018: two multiplications between shifts, its constants found by a search for
+// the least bias).  What goes into it keeps elements, tensors and steps apart: a tensor's number times 2^32 over the golden
+// ratio, a step's times an odd constant (from A. Appleby's published 32-bit mixer).
 __device__ __forceinline__ unsigned random20(unsigned x) {
     x = (x ^ (x >> 16)) * 0x7FEB352Du;
     x = (x ^ (x >> 15)) * 0x846CA68Bu;
@@ -199,19 +202,20 @@ __device__ __forceinline__ unsigned to_e4m3(float y) {
 // 0 <= y <= 448 up or down by 20 random bits, which side settled in 64 bits: with the exponent E of y (at least that of the
 // least normal value) the values of e4m3 are 2^(E-3) apart, y is that times q + fraction, and the code of (E, q) is
 // 8 (E + 7) + q - 8 — also where q reaches 16 (the next exponent's first value) and below 8 at the least exponent (the
-// subnormal values).
-__device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
+// subnormal values).  KEPT: a positive y not to zero.
+template <bool KEPT> __device__ __forceinline__ unsigned to_e4m3_random(double y, unsigned bits20) {
     const int e = max((int)(__builtin_bit_cast(unsigned long long, y) >> 52) - 1023, -6);
     const double units = __builtin_bit_cast(double, (unsigned long long)(1023 + 3 - e) << 52);   // 2^(3 - E)
     int q = (int)(y * units + (double)bits20 * 0x1p-20);
-    if (y > 0) q = max(q, 1);
+    if (KEPT && y > 0) q = max(q, 1);
     return (unsigned)(8 * (e + 7) + q - 8);
 }
 
 // A wavefront owns a block of 256 elements, a lane four consecutive ones of them (FULL: the block is whole): a block's scale
 // is one exchange within the wavefront.  99M parameters with bf16 gradients and copies, 1.6 GB: 339-351 us, 4.6 TB/s: the
 // encodings' arithmetic, two divisions in 64 bits a lane among it, stands beside the memory.
-template <class G, bool FULL, bool NT>
+// SLOW: the mean up or down at random too (see slow_mean).
+template <class G, bool FULL, bool NT, bool SLOW>
 __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int lane, unsigned number, const Scalars &k, const Step &s) {
     uint8_t *mom8 = static_cast<uint8_t *>(t.mom), *var8 = static_cast<uint8_t *>(t.var);
     const G *dw = static_cast<const G *>(t.dw);
@@ -252,10 +256,16 @@ __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         // (the quotients by a reciprocal in 64 bits: the fp32 quotient of mom correctly rounded)
-        const float x = fminf(fmaxf((float)(m[e] * im), -kLargest), kLargest);
+        const unsigned key = (unsigned)(i0 + e) + number;
+        if constexpr (SLOW) {
+            const double x = fmin(fabs(m[e] * im), (double)kLargest);
+            mc[e] = fabsf(m[e]) < __builtin_inff() ? to_e4m3_random<false>(x, random20(~key)) | (m[e] < 0.f ? 0x80u : 0u) : kNan8;
+        } else {
+            const float x = fminf(fmaxf((float)(m[e] * im), -kLargest), kLargest);
+            mc[e] = fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8;
+        }
         const double y = fmin(r[e] * iv, (double)kLargest);
-        mc[e] = fabsf(m[e]) < __builtin_inff() ? to_e4m3(x) : kNan8;
-        vc[e] = r[e] < __builtin_inff() ? to_e4m3_random(y, random20((unsigned)(i0 + e) + number)) : kNan8;
+        vc[e] = r[e] < __builtin_inff() ? to_e4m3_random<true>(y, random20(key)) : kNan8;
     }
     if constexpr (FULL) {
         put4<NT>(t.w + i0, w);
@@ -277,7 +287,7 @@ __device__ __forceinline__ void adamw8_block(const Tensor8 &t, size_t block, int
     }
 }
 
-template <class G, bool NT>
+template <class G, bool NT, bool SLOW>
 __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTensors8> tab, Step s) {
     const int which = tensor_of(tab, blockIdx.x);
     const Tensor8 &t = tab.t[which];
@@ -285,8 +295,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_tensors(Table<Tensor8, kTenso
     const size_t block = (size_t)(blockIdx.x - tab.first[which]) * 4 + (threadIdx.x >> 6);
     if (block * kBlock >= t.size) return;   // whole wavefronts leave together
     const unsigned number = (unsigned)(tab.number0 + which) * 0x9E3779B9u + (unsigned)s.state->steps * 0x85EBCA6Bu;
-    if ((block + 1) * kBlock <= t.size) adamw8_block<G, true, NT>(t, block, threadIdx.x & 63, number, k, s);
-    else adamw8_block<G, false, NT>(t, block, threadIdx.x & 63, number, k, s);
+    if ((block + 1) * kBlock <= t.size) adamw8_block<G, true, NT, SLOW>(t, block, threadIdx.x & 63, number, k, s);
+    else adamw8_block<G, false, NT, SLOW>(t, block, threadIdx.x & 63, number, k, s);
 }
 
 int check(const char *who, int count, const void *const *w, const void *const *dw, const void *const *mom,
@@ -340,6 +350,12 @@ int launch_tables(int count, const size_t *sizes, Fill fill, Launch launch) {
     return SWC_HIP_OK;
 }
 
+// A step moves a mean by (1 - beta1) |g - mom|.  Rounded to the nearest value, of which two are up to an eighth of the lower
+// one apart, it moves at all only where that is half of it: with 1 - beta1 at most a sixteenth not even a mean whose gradient
+// has stopped (g = 0) leaves every value, and one far from its gradient stays.  There the mean is rounded at random, which
+// keeps its expectation (99M parameters 380 us, 348 to the nearest).
+bool slow_mean(double beta1) { return beta1 >= 15. / 16; }
+
 // Whether the weights of a call are large enough to be streamed past the caches.
 bool streams(const size_t *sizes, int count, size_t bytes) {
     size_t all = 0;
@@ -384,7 +400,9 @@ int adamw8(const char *who, int count, float *const *w, const G *const *dw, uint
             t.size = sizes[i], t.mom_scale = mom_scale[i], t.var_scale = var_scale[i];
         },
         [&](const Table<Tensor8, kTensors8> &tab, unsigned chunks) {
-            auto kern = streams(sizes, count, sizeof(float)) ? adamw8_tensors<G, true> : adamw8_tensors<G, false>;
+            const bool nt = streams(sizes, count, sizeof(float));
+            auto kern = slow_mean(beta1) ? (nt ? adamw8_tensors<G, true, true> : adamw8_tensors<G, false, true>)
+                                         : (nt ? adamw8_tensors<G, true, false> : adamw8_tensors<G, false, false>);
             kern<<<chunks, kThreads, 0, stream()>>>(tab, s);
         });
 }
