@@ -1,8 +1,11 @@
-"""AdamW with its states in 8 bits: the mean under slow decays (helpers and the definition as in test_hip_lm_ops.py)."""
+"""AdamW with its states in 8 bits: the mean under slow decays, copies, factors, tensors off the 16-byte grid, recorded steps
+and long runs (helpers and the definition as in test_hip_lm_ops.py)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
-from tests.test_hip_lm_ops import E4M3, KINDS, U, blocks, random20, to_bf16, within
+from tests.test_hip_lm_ops import E4M3, KINDS, SIZES, U, adamw64, blocks, random20, to_bf16, within
 from swcompiler_amd.hip import ADAMW_BLOCK
 
 gpu = pytest.mark.gpu
@@ -134,3 +137,140 @@ def test_a_slow_mean_follows_its_gradient(rt, beta1, gradient):
     got = (E4M3[m.mom[0].numpy()] * np.repeat(m.ms[0].numpy(), ADAMW_BLOCK))[small]
     want = gradient + (4 - gradient) * beta1 ** steps
     assert abs(got.mean() - want) <= 5 * 0.5 / np.sqrt((1 - beta1 ** 2) * small.sum())
+
+
+# ------------------------------------------------------------------- copies, factors, offsets, recorded and large steps
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+@pytest.mark.parametrize("sizes", SIZES, ids=[f"{len(s)}x{max(s)}" for s in SIZES])
+def test_copies(rt, grads, sizes):
+    """copies of some of the tensors, whole blocks and short ones: w rounded to bfloat16; they change nothing else"""
+    print("case copies", grads.name, len(sizes), max(sizes), flush=True)
+    rng = np.random.default_rng(sum(sizes))
+    with_, without = Model(rt, sizes), Model(rt, sizes, copies=False)
+    with_.copy = [None if i % 3 == 1 else c for i, c in enumerate(with_.copy)]
+    for _ in range(2):
+        g = [rng.standard_normal(s) for s in sizes]
+        with_.step(with_.grads(grads, g))
+        without.step(without.grads(grads, g))
+    for w, c in zip(with_.w, with_.copy):
+        if c is not None:
+            np.testing.assert_array_equal(c.numpy(), to_bf16(w.numpy()).reshape(-1))
+    with_.copy = None
+    same(with_.held(), without.held())
+
+
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+@pytest.mark.parametrize("beta1", [0.9, 0.95])
+def test_offsets(rt, grads, beta1):
+    """every array at addresses of an element's alignment only (codes at odd bytes), with gaps: the bits of aligned arrays, and
+    nothing beside the tensors changes"""
+    sizes = [300, 1, 1025, 256, 0, 1600, 2048]
+    rng = np.random.default_rng(4)
+    plain, moved = Model(rt, sizes), Model(rt, sizes, first=dict(w=1, g=3, mom=1, var=3, ms=1, vs=3, copy=5, gap=3))
+    for _ in range(3):
+        g = [rng.standard_normal(s) for s in sizes]
+        plain.step(plain.grads(grads, g), beta1=beta1)
+        moved.step(moved.grads(grads, g), beta1=beta1)
+    same(plain.held(), moved.held())
+    for name, (d, inside, fill) in moved.arena.items():
+        assert np.all(d.numpy()[~inside] == fill), name
+
+
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+def test_factors(rt, grads):
+    """factors on the device that are powers of two give the bits of a call with the rate and the gradients scaled"""
+    sizes = [700, 33]
+    rng = np.random.default_rng(2)
+    one, two = Model(rt, sizes), Model(rt, sizes)
+    half, quarter = (rt.upload(np.array([x], np.float32)) for x in (0.5, 0.25))
+    for _ in range(2):
+        g = [grads.values(rng.standard_normal(s)) for s in sizes]
+        one.step(one.grads(grads, g), lr_factor=half, grad_factor=quarter, decay=0.0)
+        two.step(two.grads(grads, [x / 4 for x in g]), lr=RATES["lr"] / 2, decay=0.0)
+    same(one.held(), two.held())
+
+
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+def test_a_recorded_step_goes_on(rt, grads):
+    """a step recorded once and replayed counts, and is bit for bit the eager step: the random numbers are those of the step"""
+    sizes = [5000, 257, 16]
+    rng = np.random.default_rng(6)
+    eager, recorded, other = Model(rt, sizes), Model(rt, sizes), Model(rt, [9000])
+    g = [rng.standard_normal(s) for s in sizes]
+    ge, gr, go = eager.grads(grads, g), recorded.grads(grads, g), other.grads(grads, [rng.standard_normal(9000)])
+    for m, x in ((eager, ge), (recorded, gr), (other, go)):
+        m.step(x, beta1=0.95)
+    graph = C.c_void_p()
+    rt._check(rt.lib.swc_hip_graph_begin(), "begin")
+    try:
+        recorded.step(gr, beta1=0.95)
+    finally:
+        rt._check(rt.lib.swc_hip_graph_end(C.byref(graph)), "end")
+    try:
+        for _ in range(4):
+            rt._check(rt.lib.swc_hip_graph_launch(graph), "launch")
+            other.step(go)
+            eager.step(ge, beta1=0.95)
+            rt.sync()
+            same(eager.held(), recorded.held())
+    finally:
+        rt._check(rt.lib.swc_hip_graph_destroy(graph), "destroy")
+    assert recorded.state.numpy()[0] == 5
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grads", KINDS)
+def test_large(rt, grads, bits):
+    """a call large enough to go past the caches (17 million elements) gives the bits, scales and copies of a small call on its
+    first part, and every copy is its weight rounded"""
+    n, cut = 17_000_003, 5120 * ADAMW_BLOCK
+    rng = np.random.default_rng(17)
+    one, two = Model(rt, [n], bits=bits), Model(rt, [n], bits=bits)
+    g = rng.standard_normal(n, np.float32)
+    go, gt = one.grads(grads, [g]), two.grads(grads, [g])
+    two.w, gt, two.mom, two.var, two.copy = ([x[0].offset_view(0, (cut,))] for x in (two.w, gt, two.mom, two.var, two.copy))
+    two.ms, two.vs = ([x[0].offset_view(0, (cut // ADAMW_BLOCK,))] for x in (two.ms, two.vs))
+    for beta1 in (0.9, 0.95):
+        one.step(go, beta1=beta1)
+        two.step(gt, beta1=beta1)
+    a, b = one.held(), two.held()
+    np.testing.assert_array_equal(a["copy"][0], to_bf16(a["w"][0]))
+    for name, value in b.items():
+        np.testing.assert_array_equal(a[name][0][:value[0].size], value[0], err_msg=name)
+    arena, inside, fill = one.arena["w"]
+    assert np.all(arena.numpy()[~inside] == fill) and a["w"][0][-1] != two.arena["w"][0].numpy()[n - 1]
+
+
+@gpu
+@pytest.mark.parametrize("grads", KINDS)
+@pytest.mark.parametrize("beta1", [0.9, 0.95])
+def test_a_long_run(rt, grads, beta1):
+    """40 steps: the first, from states of zero, has the weights that 32-bit states give, bit for bit; each later one the step in
+    64 bits from the states as held before it, no drift and no neighbour's state; the copies stay the weights rounded"""
+    sizes = [4096, 513]
+    rng = np.random.default_rng(8)
+    eight, full = Model(rt, sizes), Model(rt, sizes, bits=32)
+    rates = dict(RATES, beta1=beta1)
+    for t in range(1, 41):
+        h = eight.held()
+        g = [grads.values(rng.standard_normal(s) * 10.0 ** rng.uniform(-3, 0, s)) for s in sizes]
+        eight.step(eight.grads(grads, g), beta1=beta1)
+        if t == 1:
+            full.step(full.grads(grads, g), beta1=beta1)
+            same(dict(w=full.held()["w"]), dict(w=eight.held()["w"]))
+        for i, s in enumerate(sizes):
+            m0, r0 = (E4M3[h[a][i]] * np.repeat(h[b][i], ADAMW_BLOCK)[:s].astype(np.float64) for a, b in (("mom", "ms"), ("var", "vs")))
+            w0 = h["w"][i].astype(np.float64)
+            w1, m1, v1 = adamw64(w0, g[i].astype(np.float64), m0, r0 * r0, t, **rates)
+            # three roundings of w; some forty of the update, whose mean is off by those of its two parts where they cancel
+            parts = beta1 * np.abs(m0) + (1 - beta1) * np.abs(g[i])
+            size = rates["lr"] * (parts / (1 - beta1 ** t)) / (np.sqrt(v1 / (1 - rates["beta2"] ** t)) + rates["eps"])
+            within(eight.w[i].numpy(), w1, 3 * U * np.abs(w1) + 40 * U * (size + rates["lr"] * rates["decay"] * np.abs(w0)), f"w, step {t}")
+    h = eight.held()
+    for w, c in zip(h["w"], h["copy"]):
+        np.testing.assert_array_equal(c, to_bf16(w))
