@@ -3,7 +3,7 @@ tolerances hold here too)."""
 import numpy as np
 import pytest
 
-from tests.test_hip_lm_ops import BF, F32, KINDS, U, small_ints, within
+from tests.test_hip_lm_ops import BF, F32, KINDS, U, rows_of, small_ints, strided, within
 
 gpu = pytest.mark.gpu
 
@@ -91,89 +91,162 @@ LOSSES = [(5444, 12123, 153, 0, BIG + "kk> x"), (5153, 26804, 133, 0.1, BIG + "k
           (657, 27624, 72, 0.2, ""), (262, 87488, 200, 0, ""), (1177, 60288, 72, 0.1, ""), (909, 8472, 72, 0, ""), (1, 42770, 66, 0, "")]
 
 
+class TwoValued:
+    """logits of two values only, 0 for the classes that go with a row's feature and -128 for the others, so that the
+    probabilities are a power of two and zero, dz and all that follows small integers.  The first k1 features choose (128 in
+    one of them, against 0 or -1 in B); the others come in pairs, the same in a row of A and opposite in a column of B, and
+    cancel in the logits but not in the gradients."""
+
+    def __init__(self, m, n, k, share):
+        rng = np.random.default_rng(m + n + k)
+        k1 = k - k // 4 * 2
+        pairs = (k - k1) // 2
+        width = 256
+        while width > 1 and (width > n // 2 or width > 2 * n // k1 + 1):
+            width //= 2
+        chosen = np.stack([rng.choice(n, width, replace=False) for _ in range(k1)])      # the classes of a feature
+        b = np.empty((k, n), np.float32)
+        b[:k1] = -1
+        np.put_along_axis(b[:k1], chosen, 0, 1)
+        b[k1::2] = rng.integers(-2, 3, (pairs, n))
+        b[k1 + 1::2] = -b[k1::2]
+        feature = rng.integers(0, k1, m)
+        a = np.zeros((m, k), np.float32)
+        a[np.arange(m), feature] = 128
+        a[:, k1::2] = rng.integers(-2, 3, (m, pairs))
+        a[:, k1 + 1::2] = a[:, k1::2]
+        sel = np.where(rng.random(m) < 0.7, chosen[feature, rng.integers(0, width, m)], rng.integers(0, n, m)).astype(np.int32)
+        out = rng.random(m) < share
+        sent = a.copy()
+        sent[out] = np.nan
+        sel_sent = np.where(out, rng.choice([-1, n, n + 5], m), sel).astype(np.int32)
+        grad = (width * rng.integers(1, 3, m)).astype(np.float32)
+        self.a, self.b, self.sel, self.grad, self.width = sent, b, sel_sent, grad, width
+        self.parts = (a, sel, out, chosen, feature, k1)
+
+    def losses(self):
+        """row losses, lse and their mean"""
+        a, sel, out, chosen, feature, _ = self.parts
+        inside = (chosen[feature] == sel[:, None]).any(1)
+        row = np.log(self.width) + np.where(inside, 0.0, 128.0)
+        return np.where(out, 0, row), np.where(out, 0, np.log(self.width)), row[~out].mean() if not out.all() else 0.0
+
+    def check_losses(self, row, lse, loss):
+        want = self.losses()
+        # log and the subtraction of numbers below 134: some roundings of 2^-24 of them
+        within(lse, want[1], 4 * U * 8, "lse")
+        within(row, want[0], 4 * U * 136, "row loss")
+        within(np.reshape(loss, ()), want[2], 8 * U * 136, "loss")
+
+    def check_gradients(self, kind, *got):
+        """dA, dB and dbias, every element"""
+        a, sel, out, chosen, feature, k1 = self.parts
+        b, width, m, n, k = self.b, self.width, self.a.shape[0], self.b.shape[1], self.b.shape[0]
+        # dz = g / width at the classes of the row's feature, -g at its own (both at once where it is one of them)
+        g = np.where(out, 0, self.grad).astype(np.float64)
+        b64, a64 = b.astype(np.float64), np.where(out[:, None], 0, a).astype(np.float64)
+
+        def results(a, b, minus):
+            per_feature = np.stack([b[:, c].sum(1) for c in chosen])                    # [feature][k]
+            da = (g / width)[:, None] * per_feature[feature] + minus * g[:, None] * b[:, sel].T
+            sums, ones = np.zeros((k1, k)), np.zeros(k1)
+            np.add.at(sums, feature, (g / width)[:, None] * a)
+            np.add.at(ones, feature, g / width)
+            db, dbias = np.zeros((n, k)), np.zeros(n)
+            for i, c in enumerate(chosen):
+                db[c] += sums[i]
+                dbias[c] += ones[i]
+            np.add.at(db, sel, minus * g[:, None] * a)
+            np.add.at(dbias, sel, minus * g)
+            return da, db.T, dbias
+
+        exact = results(a64, b64, -1.0)
+        if kind is BF:      # (a probability is within 2^-18 of its power of two: rounded to bfloat16, dz is exact)
+            bounds = (0.0, 0.0, 0.0)
+        else:               # dz within 2^-20 of its parts, and the additions of at most 2 width (m) terms that are not zero
+            size = results(np.abs(a64), np.abs(b64), 1.0)
+            bounds = [(2.0 ** -20 + 2 * terms * U) * x for x, terms in zip(size, (width, min(m, 4096), min(m, 4096)))]
+        for name, x, value, bound in zip(("da", "db", "dbias"), got, exact, bounds):
+            if kind is BF:
+                np.testing.assert_array_equal(x, kind.values(value), err_msg=name)
+            else:
+                within(x, value, bound, name)
+
+
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("m,n,k,share,kernel", LOSSES)
 def test_loss_tiles(rt, kind, m, n, k, share, kernel):
-    """logits of two values only, 0 for the classes that go with a row's feature and -128 for the others, so that the
-    probabilities are a power of two and zero, dz and all that follows small integers.  The first k1 features choose (128 in
-    one of them, against 0 or -1 in B); the others come in pairs, the same in a row of A and opposite in a column of B, and
-    cancel in the logits but not in the gradients.  Every element of every result is compared."""
     print("case loss", kind.name, m, n, k, share, flush=True)
-    rng = np.random.default_rng(m + n + k)
-    k1 = k - k // 4 * 2
-    pairs = (k - k1) // 2
-    width = 256
-    while width > 1 and (width > n // 2 or width > 2 * n // k1 + 1):
-        width //= 2
-    chosen = np.stack([rng.choice(n, width, replace=False) for _ in range(k1)])      # the classes of a feature
-    b = np.empty((k, n), np.float32)
-    b[:k1] = -1
-    np.put_along_axis(b[:k1], chosen, 0, 1)
-    b[k1::2] = rng.integers(-2, 3, (pairs, n))
-    b[k1 + 1::2] = -b[k1::2]
-    feature = rng.integers(0, k1, m)
-    a = np.zeros((m, k), np.float32)
-    a[np.arange(m), feature] = 128
-    a[:, k1::2] = rng.integers(-2, 3, (m, pairs))
-    a[:, k1 + 1::2] = a[:, k1::2]
-    sel = np.where(rng.random(m) < 0.7, chosen[feature, rng.integers(0, width, m)], rng.integers(0, n, m)).astype(np.int32)
-    out = rng.random(m) < share
-    sent = a.copy()
-    sent[out] = np.nan
-    sel_sent = np.where(out, rng.choice([-1, n, n + 5], m), sel).astype(np.int32)
-    grad = (width * rng.integers(1, 3, m)).astype(np.float32)
-
-    da_, db_, dsel = kind.up(rt, sent), kind.up(rt, b), rt.upload(sel_sent)
+    t = TwoValued(m, n, k, share)
+    da_, db_, dsel = kind.up(rt, t.a), kind.up(rt, t.b), rt.upload(t.sel)
     loss, row, lse = rt.matrixFCSoftmaxWithLoss(da_, db_, None, dsel)
-    inside = (chosen[feature] == sel[:, None]).any(1)
-    want = np.log(width) + np.where(inside, 0.0, 128.0)
-    # log and the subtraction of numbers below 134: some roundings of 2^-24 of them
-    within(lse.numpy(), np.where(out, 0, np.log(width)), 4 * U * 8, "lse")
-    within(row.numpy(), np.where(out, 0, want), 4 * U * 136, "row loss")
-    within(loss.numpy().reshape(()), want[~out].mean() if not out.all() else 0.0, 8 * U * 136, "loss")
+    t.check_losses(row.numpy(), lse.numpy(), loss.numpy())
     ga, gb, gbias = (rt.empty(s, kind.numpy) for s in ((m, k), (k, n), (n,)))
-    dg = rt.upload(grad)
+    dg = rt.upload(t.grad)
     rt.matrixFCSoftmaxWithLossGrad(da_, db_, None, dsel, lse, dg, da=ga)
     ran(rt, kind, kernel)
     alone = kind.down(ga)
     rt._check(rt.lib.swc_hip_fill_i(ga.ptr, 0x7FC07FC0, ga.nbytes // 4), "fill")
     rt.matrixFCSoftmaxWithLossGrad(da_, db_, None, dsel, lse, dg, da=ga, db=gb, dbias=gbias)
-
-    # dz = g / width at the classes of the row's feature, -g at its own (both at once where it is one of them)
-    g = np.where(out, 0, grad).astype(np.float64)
-    b64, a64 = b.astype(np.float64), np.where(out[:, None], 0, a).astype(np.float64)
-
-    def results(a, b, minus):
-        per_feature = np.stack([b[:, c].sum(1) for c in chosen])                    # [feature][k]
-        da = (g / width)[:, None] * per_feature[feature] + minus * g[:, None] * b[:, sel].T
-        sums, ones = np.zeros((k1, k)), np.zeros(k1)
-        np.add.at(sums, feature, (g / width)[:, None] * a)
-        np.add.at(ones, feature, g / width)
-        db, dbias = np.zeros((n, k)), np.zeros(n)
-        for i, c in enumerate(chosen):
-            db[c] += sums[i]
-            dbias[c] += ones[i]
-        np.add.at(db, sel, minus * g[:, None] * a)
-        np.add.at(dbias, sel, minus * g)
-        return da, db.T, dbias
-
-    exact = results(a64, b64, -1.0)
-    if kind is BF:      # (a probability is within 2^-18 of its power of two: rounded to bfloat16, dz is exact)
-        bounds = (0.0, 0.0, 0.0)
-    else:               # dz within 2^-20 of its parts, and the additions of at most 2 width (m) terms that are not zero
-        size = results(np.abs(a64), np.abs(b64), 1.0)
-        bounds = [(2.0 ** -20 + 2 * terms * U) * x for x, terms in zip(size, (width, min(m, 4096), min(m, 4096)))]
-    for name, got, value, bound in zip(("da", "db", "dbias"), (ga, gb, gbias), exact, bounds):
-        got = kind.down(got)
-        if kind is BF:
-            np.testing.assert_array_equal(got, kind.values(value), err_msg=name)
-        else:
-            within(got, value, bound, name)
+    t.check_gradients(kind, kind.down(ga), kind.down(gb), kind.down(gbias))
     np.testing.assert_array_equal(alone, kind.down(ga))
 
 
-# ------------------------------------------------------------------------------------------------------- gradients
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pad,first", [(8, 8), (3, 1)])
+@pytest.mark.parametrize("m,n,k,share", [(1, 300, 40, 0), (33, 200, 136, 0.2), (300, 1000, 75, 0.3), (700, 2050, 130, 0.1), (4200, 301, 66, 0.3)])
+def test_loss_strides_exactly(rt, kind, pad, first, m, n, k, share):
+    """operands and gradients in longer rows, off the 16-byte grid, with row gradients, a bias and rows left out: every element,
+    and nothing beside the rows"""
+    print("case loss strides", kind.name, pad, first, m, n, k, flush=True)
+    t = TwoValued(m, n, k, share)
+    _da, pa = strided(rt, kind, t.a, k + pad, first)
+    _db, pb = strided(rt, kind, t.b, n + pad, first)
+    sel, g, bias = rt.upload(t.sel), rt.upload(t.grad), kind.up(rt, np.zeros(n))
+    row, lse, loss = rt.empty((m,)), rt.empty((m,)), rt.empty((1,))
+    call = lambda name: getattr(rt.lib, "swc_hip_matrixFCSoftmaxWithLoss" + name + kind.suffix())   # noqa: E731
+    rt._check(call("")(m, n, k, pa, k + pad, pb, n + pad, bias.ptr, sel.ptr, row.ptr, lse.ptr, loss.ptr), "loss")
+    t.check_losses(row.numpy(), lse.numpy(), loss.numpy())
+    ga, pga = strided(rt, kind, np.zeros((m, k)), k + 2 * pad, first)
+    gb, pgb = strided(rt, kind, np.zeros((k, n)), n + pad, first)
+    gbias = rt.empty((n,), kind.numpy)
+    rt._check(call("Grad")(m, n, k, pa, k + pad, pb, n + pad, bias.ptr, sel.ptr, lse.ptr, g.ptr, pga, k + 2 * pad, pgb, n + pad,
+                           gbias.ptr), "grad")
+    (ia, sa, ba), (ib, sb, bb) = rows_of(kind, ga, m, k, k + 2 * pad, first), rows_of(kind, gb, k, n, n + pad, first)
+    t.check_gradients(kind, ia, ib, kind.down(gbias))
+    for x in (sa, ba, sb, bb):
+        assert np.all(np.isnan(x))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_empty_operands_through_the_binding(rt, kind):
+    """no rows, no columns, no contraction: sums of nothing are zero, and nothing else is written"""
+    e = lambda *s: rt.empty(s, kind.numpy)   # noqa: E731
+    full = lambda *s: kind.up(rt, np.full(s, 7))   # noqa: E731
+    zero = lambda d: np.all(kind.down(d) == 0)   # noqa: E731
+    assert rt.matrixMatrixFCActAdd(e(0, 8), full(8, 16), full(16), "gelu").shape == (0, 16)
+    assert rt.matrixMatrixFCActAdd(full(5, 8), e(8, 0), e(0), "gelu").shape == (5, 0)
+    c, z = full(5, 16), full(5, 16)
+    rt.matrixMatrixFCActAdd(e(5, 0), e(0, 16), None, "none", full(5, 16), z, c)
+    assert zero(z) and np.all(kind.down(c) == 7)
+    _, db, dbias = rt.matrixMatrixFCActAddGrad(e(0, 16), e(0, 8), full(8, 16), e(0, 16), "silu")
+    assert zero(db) and zero(dbias)
+    da, _, _ = rt.matrixMatrixFCActAddGrad(e(5, 0), full(5, 8), e(8, 0), e(5, 0), "silu")
+    assert zero(da)
+    _, _, dbias = rt.matrixMatrixFCActAddGrad(full(5, 16), e(5, 0), e(0, 16))
+    assert np.all(kind.down(dbias) == 35)
+    loss, row, lse = rt.matrixFCSoftmaxWithLoss(e(0, 8), full(8, 16), None, rt.empty((0,), np.int32))
+    assert loss.numpy() == 0 and row.shape == lse.shape == (0,)
+    _, db, dbias = rt.matrixFCSoftmaxWithLossGrad(e(0, 8), full(8, 16), None, rt.empty((0,), np.int32), rt.empty((0,)))
+    assert zero(db) and zero(dbias)
+    loss, row, lse = rt.matrixFCSoftmaxWithLoss(full(5, 8), e(8, 0), None, rt.upload(np.zeros(5, np.int32)))
+    assert loss.numpy() == 0 and np.all(row.numpy() == 0) and np.all(lse.numpy() == 0)
+
+
+# -------------------------------------------------------------------------------------------------- values of ReLU
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 def test_an_inactive_relu_passes_nothing_on(rt, kind):
