@@ -90,7 +90,9 @@ __global__ __launch_bounds__(256) void copy_dense(const T *a, long lda, int k, T
 #endif
 }
 // Few rows: a workgroup per row counts the rows before its own and copies it; workgroups behind them copy B onto the 16-byte
-// grid where it has to be.  One launch instead of three: 1999 rows of 1024 8 us, with 1024 x 50257 of B beside them 37 us.
+// grid where it has to be.  One launch instead of three, and dA's rows may go straight to their places (see direct): 1999 rows
+// of 1024 8 us, with 1024 x 50257 of B beside them 37 us.  The counting grows with the square of the rows: bf16, k = 1024, n =
+// 256, forward and dA together, this way / the other: 2048 rows 39 / 47 us, 4096 59 / 62, 8192 122 / 89.
 constexpr int kCountRows = 4096;
 template <class T>
 __global__ __launch_bounds__(256) void count_and_copy(RowsFrom from, Rows to, const T *a, long lda, int k, T *dense, long ld,
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(256) void join_rows(const float2 *part, int blocks,
     if (row < *rows.count) join_row(row, threadIdx.x & 63, part, blocks, picked, rows, row_loss, lse);
 }
 
-// *loss = mean over the dense rows, summed in double in a fixed order; JOIN: joins the rows first (few rows: one launch)
+// *loss = mean over the dense rows, summed in double in a fixed order; JOIN: joins the rows first, sixteen at a time.
 template <bool JOIN>
 __global__ __launch_bounds__(1024) void mean_loss(const float2 *part, int blocks, const float *picked, Rows rows, float *row_loss,
                                                   float *lse, float *loss) {
@@ -268,6 +270,11 @@ __global__ __launch_bounds__(1024) void mean_loss(const float2 *part, int blocks
     }
     if (threadIdx.x == 0) *loss = count ? (float)(sums[0] / count) : 0.f;
 }
+
+// Whether joining and mean take one launch: up to sixteen rows, which go at once, and up to 64 whose blocks are one to a lane.
+// (k = 64, one launch / two: 16 x 1000 10.1 / 11.4 us, 16 x 100000 33.8 / 35.0, 32 x 1000 11.1 / 11.4, 64 x 1000 13.1 / 11.4 and
+// a launch's time on the host, 32 x 10000 14.9 / 13.1, 64 x 100000 102 / 37.)
+bool joins_in_mean(int m, int blocks) { return m <= 16 || (m <= 64 && blocks <= 64); }
 
 // ---------------------------------------------------------------- gradients
 // dz of a piece of the vocabulary, zeros in the columns that pad it to whole 16 bytes.  Bound by the product (8192 x 16384 x
@@ -359,8 +366,10 @@ int launch_spread(T *out, long ld, const float *part, int parts, long stride, in
     return SWC_HIP_OK;
 }
 
-// Few rows: a piece's column sums at once, 32 columns and eight ranges of the rows a workgroup.
-constexpr int kFewSums = 512;
+// Few rows: a piece's column sums at once, 32 columns and eight ranges of the rows a workgroup.  One launch instead of two (dz
+// and its sums with k = 64, this way / by blocks of rows below: 256 x 1000 10.4 / 11.8 us, 256 x 50000 31.4 / 30.3, 512 x 1000
+// 12.6 / 12.2, 512 x 50000 48 / 41).
+constexpr int kFewSums = 256;
 template <class T> __global__ __launch_bounds__(256) void few_column_sums(const T *dz, long ld, int cols, Rows rows, T *out) {
     __shared__ float sums[8][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, j = blockIdx.x * 32 + tx;
@@ -523,7 +532,7 @@ int forward(const char *who, int m, int n, int k, const T *a, int lda, const T *
     const int blocks = row_blocks(p, n);
     const Shape<T> s{w.a, b, row_length<T>(k), ldb, m, n, k, 0, 1, w.rows.count};
     if (int rc = run_product<kAlongK, kAcross>(p, s, RowStats<T>{w.part, blocks, w.picked, w.rows.sel, bias, 0}, who)) return rc;
-    if (m <= 64) {
+    if (joins_in_mean(m, blocks)) {
         mean_loss<true><<<1, 1024, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse, loss);
     } else {
         join_rows<<<ceil_div(m, 4), 256, 0, stream()>>>(w.part, blocks, w.picked, w.rows, row_loss, lse);

@@ -195,6 +195,20 @@ def test_loss_tiles(rt, kind, m, n, k, share, kernel):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n", [(15, 70), (16, 20000), (17, 900), (17, 5000), (64, 1000), (64, 4200), (65, 300), (255, 3000), (257, 3000)])
+def test_few_rows_of_a_loss(rt, kind, m, n):
+    """next to where the row statistics' joining and the column sums change their way; a third of the rows left out"""
+    print("case few rows", kind.name, m, n, flush=True)
+    t = TwoValued(m, n, 40, 0.33)
+    a, b, sel = kind.up(rt, t.a), kind.up(rt, t.b), rt.upload(t.sel)
+    loss, row, lse = rt.matrixFCSoftmaxWithLoss(a, b, kind.up(rt, np.zeros(n)), sel)
+    t.check_losses(row.numpy(), lse.numpy(), loss.numpy())
+    da, db, dbias = rt.matrixFCSoftmaxWithLossGrad(a, b, None, sel, lse, rt.upload(t.grad))
+    t.check_gradients(kind, kind.down(da), kind.down(db), kind.down(dbias))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("pad,first", [(8, 8), (3, 1)])
 @pytest.mark.parametrize("m,n,k,share", [(1, 300, 40, 0), (33, 200, 136, 0.2), (300, 1000, 75, 0.3), (700, 2050, 130, 0.1), (4200, 301, 66, 0.3)])
 def test_loss_strides_exactly(rt, kind, pad, first, m, n, k, share):
