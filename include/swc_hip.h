@@ -18,7 +18,10 @@
  *   - ops are asynchronous on one in-order HIP stream per process (the
  *     reference's CUDA path uses one stream per GPU,
  *     src/codegen/Codegen.cpp:166-172); call swc_hip_sync() before reading
- *     results on the host.  swc_hip_d2h synchronises by itself.
+ *     results on the host.  swc_hip_d2h synchronises by itself.  One host thread
+ *     calls ops at a time: an op may be several launches that hand data on in the
+ *     workspace, and another thread's would fall between them; for the same reason
+ *     recorded graphs that use one workspace do not run at the same time.
  * Nothing here allocates device memory except swc_hip_malloc: an op that needs
  * scratch memory (swc_hip_conv2dGrad_f, swc_hip_matrixSoftmaxWithLoss_f, and the
  * FC/GEMM and convolution entry points for shapes they cut along K) takes it

@@ -34,7 +34,7 @@ constexpr size_t kMaxPartials = (size_t)256 << 20;
 // joining), 512 x 4096 x 4096 24.4 (64 x 128 whole; 128 x 128 in two 23.0 and the joining), 2048 x 4096 x 4096 63.5 (128 x
 // 128; 256 x 256 83.2), 1400 x 1024 x 50264 175 (256 x 256 in eight; 128 x 128 in four 250).  An fp32 slice is half as many
 // products at a sixteenth of the rate: the matrix cores set its time.
-// one: only whole contractions.  The cost goes to *cost.
+// one: only whole contractions.  The cost goes to *cost_of.
 template <class T> Plan plan_uniform(int m, int n, int k, bool one, double *cost_of) {
     struct Tile {
         Kind kind;
@@ -94,8 +94,9 @@ template <class T> Plan plan_product(int m, int n, int k, bool one = false) {
     return best;
 }
 
-// An epilogue's from(j) is itself for the product's columns from j on.  Those with arithmetic of their own (kHeavy) do not take the four-wavefront form of the large tile, whose one
-// wavefront per SIMD has nothing beside it while they run; those without kThinToo never run on 32-row tiles.
+// An epilogue's from(j) is itself for the product's columns from j on.  Those with arithmetic of their own (kHeavy) do not
+// take the four-wavefront form of the large tile, whose one wavefront per SIMD has nothing beside it while they run; those
+// without kThinToo never run on 32-row tiles.
 template <Layout LA, Layout LB, class T, class Ep>
 int run_product(const Plan &p, const Shape<T> &s, const Ep &ep, const char *who) {
     Shape<T> t = s;

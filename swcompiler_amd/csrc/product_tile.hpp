@@ -30,15 +30,17 @@
 //             (k >> 1) & 1 (64) or 0 (32) puts on disjoint quarters of the banks.  fp32: 32 lanes read 128 T contiguous
 //             bytes, which is conflict-free for T >= 2; for T = 1 the half-waves' rows, four apart, are put on opposite
 //             halves of the banks.
-// Measured LDS bank conflicts: none.
+// Bank conflicts in the counters: none, in any tile and layout.
 //
 // Elements outside the matrix arrive as zeros (their lanes are given an offset beyond the buffer's record count).  The
 // buffer descriptors are based at the tile (and, for an operand stored across k, moved along with k), so that matrices
 // of any size are reached with 32-bit offsets.
 //
-// What bounds the large bf16 tiles is power: on N(0,1) data the MFMAs alone, with neither loads nor LDS reads, reach 1670
-// TFLOP/s at 8192^3 (2240 on zeros), without global loads 1530, the kernels here 1450; the clock falls to 1.6-1.9 GHz.
-// Idle matrix cycles cost power too, so what was gained came from keeping the pipe fed (in TFLOP/s at 8192^3):
+// What bounds the large bf16 tiles is power: on N(0,1) data the clock falls to 1.65-1.8 GHz, where zeros keep 2.4 (8192^3
+// without an epilogue: 1370-1395 TFLOP/s against 1980 with four wavefronts, 1290 against 1760 with eight).  The MFMAs alone,
+// with neither loads nor LDS reads, reach 1670 on N(0,1), without global loads 1530.  Idle matrix cycles cost power too, so
+// what was gained came from keeping the pipe fed (TFLOP/s at 8192^3, one after the other on one card, on which all was some 4 %
+// faster than above):
 //   one slice of loads in flight, masks and LDS addresses computed in the loop  1280
 //   + whole rounds unrolled: no vector instruction between MFMAs                1310
 //   + serpentine order, one operand changes from MFMA to MFMA                   1350
