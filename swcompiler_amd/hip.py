@@ -334,7 +334,8 @@ class SwcHip:
         self._check(self.lib.swc_hip_reload_switches(), "swc_hip_reload_switches")
 
     def use_default_stream(self):
-        """launch on the device's default (null) stream, the one torch uses unless told otherwise"""
+        """launch on the device's default (null) stream, the one torch uses unless told otherwise, behind what was launched on
+        the library's own stream (work on a stream of the caller's own is not waited for)"""
         self._check(self.lib.swc_hip_set_stream(C.c_void_p(_NULL_STREAM)), "swc_hip_set_stream")
 
     # -- plumbing --------------------------------------------------------
@@ -725,7 +726,7 @@ class SwcHip:
             device, theirs, ours = torch._C._cuda_getDevice(), torch._C._cuda_getCurrentRawStream(self.device), self.lib.swc_hip_stream()
             if device != self.device:
                 raise SwcHipError(f"{what}: the current device is {device}, the runtime's {self.device}")
-            if theirs != ours and (theirs or ours != _NULL_STREAM):
+            if theirs != ours and ours and (theirs or ours != _NULL_STREAM):   # (none: the library is shut down, and says so)
                 return self._launch_between(what, torch, ours, fn, args)
         rc = fn(*args)
         if rc:
@@ -762,6 +763,7 @@ class SwcHip:
         return out if out is not None else self.empty(shape, np.float32 if like == "f32" else np.uint16)
 
     def _product(self, a, b, what):
+        self._torch_given = False
         a, b = self._arg(a, what, "a", ("f32", "bf16")), self._arg(b, what, "b", ("f32", "bf16"))
         if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0] or a.type != b.type:
             raise SwcHipError(f"{what}: a {a.shape} {a.type} and b {b.shape} {b.type} do not multiply")
@@ -845,11 +847,13 @@ class SwcHip:
 
     def adamwAdvance(self, state, beta1, beta2):
         """begins a step: counts it and prepares the bias corrections of the updates that follow"""
+        self._torch_given = False
         state = self._state(state, "adamwAdvance")
         self._launch("adamwAdvance", self.lib.swc_hip_adamwAdvance, state, beta1, beta2)
 
     def _adamw(self, what, w, dw, states, scales, copies, state, lr, beta1, beta2, eps, decay, lr_factor, grad_factor):
         count = len(w)
+        self._torch_given = False
 
         def addresses(values, types, sizes, name):
             """-> (array of addresses, element counts, the type of all)"""

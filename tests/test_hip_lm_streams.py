@@ -270,6 +270,28 @@ def test_calls_with_torch_operands_are_ordered(monkeypatch):
     assert call_with(monkeypatch, 77, capturing=(77,)) == ["call"]     # recorded by the library: ordered where launched
 
 
+def test_a_refused_call_leaves_nothing_behind(monkeypatch):
+    """a call with torch tensors that is refused does not make the next one, without any, ask torch"""
+    fake = _FakeTorch(current=5, capturing=(5,))
+    monkeypatch.setitem(sys.modules, "torch", fake)
+    rt = object.__new__(hip.SwcHip)
+    rt.device, rt.lib = 0, _FakeLib(fake, 77)
+    rt._malloc, rt._free = lambda nbytes: 1 << 20, lambda ptr: None
+    a, b = _FakeTensor(), _FakeTensor()
+    try:
+        with pytest.raises(SwcHipError, match="do not multiply"):
+            rt.matrixMatrixFCActAdd(a, b)
+        d = hip.DeviceArray(rt, (4, 4))
+        rt.matrixMatrixFCActAdd(d, d, out=hip.DeviceArray(rt, (4, 4)))
+        assert fake.log == ["call"]
+        b.shape = (8, 8)
+        rt.lib.handle, fake.log = None, []          # shut down: the library is asked, and refuses
+        rt.matrixMatrixFCActAdd(a, b, out=_FakeTensor())
+        assert fake.log == ["call"]
+    finally:
+        hip._TORCH_KINDS.clear()
+
+
 def test_torch_operands_are_refused_where_they_cannot_be_ordered(monkeypatch):
     with pytest.raises(SwcHipError, match="torch is recording a graph on another stream"):
         call_with(monkeypatch, 77, current=5, capturing=(5,))
